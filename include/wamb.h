@@ -49,7 +49,8 @@ enum wamb_device_code {
   WAMB_DEV_WAIT_TIMEOUT = 1,  /* a bounded mbarrier wait expired; kernel returned early */
   WAMB_DEV_KV_LAYOUT = 2,     /* KV pool metadata inconsistent */
   WAMB_DEV_BAD_ROW = 3,       /* candidate_cache_rows entry outside [0, pool_batch) */
-  WAMB_DEV_POOL_FULL = 4      /* not enough slots even after eviction */
+  WAMB_DEV_POOL_FULL = 4,     /* not enough slots even after eviction */
+  WAMB_DEV_KV8 = 5            /* E4M3 cache: page id, length or count out of range, or pages that overlap */
 };
 
 /* Thread-local text of the last host-side failure. */
@@ -469,6 +470,122 @@ WAMB_API int wamb_spec_commit(const int32_t* route, const void* values, const vo
  * scale > 1, else cond. */
 WAMB_API int wamb_cfg_combine(const void* cond, const void* uncond, int32_t io_is_f32, int64_t n, float scale,
                               void* out, void* stream);
+
+/* ------------------------------------------------------------------------
+ * A KV cache held in E4M3 with one scale for each block of tokens and head
+ * (no counterpart in the reference, whose cache is bf16): write, attention,
+ * attention weights and eviction by them. Half the bytes of the bf16 pool,
+ * pages instead of a pool of slots, and sequences of unequal length.
+ *
+ * Layout: k8, v8 [pages, heads, page, 128] E4M3 codes, k_scale, v_scale
+ * [pages, heads] fp32. Position p of sequence b is row p % page of page
+ * table[b, p / page]; sequences may share pages that nobody writes. A scale
+ * is 2^n, n the smallest whole number in [-40, 119] with the block's largest
+ * magnitude <= 448 * 2^n; a value is e4m3(x / scale), rounded to nearest
+ * even, saturating; NaN stays NaN. (Scales written by others may be any
+ * positive finite number.)
+ *
+ * lens, counts, tables live on the device and are read there: a call can be
+ * captured in a graph and replayed with other lengths. A page id outside
+ * [0, pages), a length outside [0, table_width * page] or a count outside
+ * [0, tokens] is recorded as WAMB_DEV_KV8; the call then touches nothing
+ * outside the cache, but its result is not to be used.
+ * ------------------------------------------------------------------------ */
+typedef struct wamb_kv8_cache {
+  void* k8; void* v8;               /* [pages, heads, page, 128] E4M3, 16-byte aligned */
+  float* k_scale; float* v_scale;   /* [pages, heads] */
+  int32_t pages, heads;
+  int32_t page;                     /* 16, 32, 64 or 128 tokens */
+} wamb_kv8_cache;
+
+typedef struct wamb_kv8_seqs {
+  int32_t batch;
+  int32_t tokens;                   /* rows of this call per sequence (padded) */
+  int32_t table_width;
+  const int32_t* table;             /* [batch, table_width] page ids */
+  const int32_t* lens;              /* [batch] tokens in the cache */
+  const int32_t* counts;            /* [batch] valid rows of this call, or NULL: tokens */
+} wamb_kv8_seqs;
+
+/* Writes rows t < counts[b] of k, v [batch, tokens, heads, 128] (bf16, or
+ * fp32 when x_is_f32; element strides of the first three axes, multiples of
+ * 8) to positions lens[b] + t; lens is not changed. A page that holds earlier
+ * positions keeps the larger of its scale and the new rows'; where it grows,
+ * the earlier codes are rounded to it. Everything else in the cache stays as
+ * it was. No two written pages of a call may be the same. */
+typedef struct wamb_kv8_write_args {
+  wamb_kv8_cache cache;
+  wamb_kv8_seqs seqs;
+  const void* k; const void* v;
+  int64_t k_stride[3], v_stride[3];
+  int32_t x_is_f32;
+} wamb_kv8_write_args;
+WAMB_API int wamb_kv8_write(const wamb_kv8_write_args* args, void* stream);
+
+/* Attention of q [batch, tokens, q_heads, 128] bf16 over the first lens[b]
+ * positions: out (bf16, strides like q) = softmax(scale q k^T) v, and
+ * lse [batch, tokens, q_heads] fp32 (optional) = ln sum exp(scale q k^T).
+ * q_heads is a multiple of the cache's heads; query head i reads cached head
+ * i / (q_heads / heads). causal: row t of sequence b sees positions
+ * <= lens[b] - counts[b] + t (the rows are the last counts[b] positions).
+ * A row that sees nothing gives zeros and lse -inf; rows past counts[b] are
+ * left as they were. What lies past lens[b] in a page counts for nothing,
+ * but a NaN that was written as V reaches every row of the call that is
+ * computed beside its key. workspace: wamb_kv8_attention_workspace_bytes()
+ * bytes of scratch, any contents, not shared with a call that may run at the
+ * same time. Results do not depend on timing. */
+typedef struct wamb_kv8_attention_args {
+  wamb_kv8_cache cache;
+  wamb_kv8_seqs seqs;
+  const void* q;
+  int64_t q_stride[3];
+  int32_t q_heads, causal;
+  float scale;
+  void* out;
+  int64_t out_stride[3];
+  float* lse;                       /* output of attention, input of weights */
+  const float* base;                /* weights only: [batch, heads, weights_cap] or NULL (zeros) */
+  float* weights;                   /* weights only: like base, and may be base */
+  int64_t weights_cap;              /* >= table_width * page */
+  void* workspace;
+  size_t workspace_bytes;
+} wamb_kv8_attention_args;
+WAMB_API size_t wamb_kv8_attention_workspace_bytes(const wamb_kv8_attention_args* args);
+WAMB_API int wamb_kv8_attention(const wamb_kv8_attention_args* args, void* stream);
+
+/* Attention weight that each cached position received:
+ * weights[b, h, j] = base[b, h, j] + sum over the valid query rows of cached
+ * head h that see j of exp(scale q k_j - lse), lse as wamb_kv8_attention gave
+ * it for the same q, lens, counts, causal and scale (rows with lse -inf add
+ * nothing). Columns that no row sees carry the base over. out, out_stride and
+ * v8 are not read. */
+WAMB_API int wamb_kv8_weights(const wamb_kv8_attention_args* args, void* stream);
+
+/* Eviction by accumulated weight, for each cached head on its own: of sequence
+ * b's lens[b] positions the last `recent` stay, and of the earlier ones the
+ * `heavy` with the largest weight (equal weights: the lowest positions; NaN
+ * counts as largest). The kept rows move, in order, to the pages of
+ * new_table (each new page gets the scale of the values it receives);
+ * kept [batch, heads, new_width * page] lists their old positions (-1 behind
+ * the last), new_weights their weights (0 behind the last), new_lens their
+ * number min(lens[b], heavy + recent). The old pages are not changed and may
+ * be freed afterwards; a page of a sequence's old table in its new one is
+ * refused (WAMB_DEV_KV8), and no new page may be in use elsewhere.
+ * max_len: an upper bound of lens that the caller knows (at most
+ * table_width * page); min(heavy + recent, max_len) must fit new_width pages. */
+typedef struct wamb_kv8_evict_args {
+  wamb_kv8_cache cache;
+  wamb_kv8_seqs seqs;               /* counts and tokens are not read */
+  const float* weights;             /* [batch, heads, weights_cap] */
+  int64_t weights_cap;              /* >= table_width * page */
+  int64_t max_len;
+  const int32_t* new_table;         /* [batch, new_width] */
+  int32_t new_width, heavy, recent;
+  int32_t* kept;
+  float* new_weights;
+  int32_t* new_lens;                /* [batch] */
+} wamb_kv8_evict_args;
+WAMB_API int wamb_kv8_evict(const wamb_kv8_evict_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,439 @@
+// A paged KV cache held in E4M3 with one scale for each (page, head), and the
+// kernels that write it and shrink it. (Attention over it: kv8_few.cuh,
+// kv8_tc.cuh.)
+//
+// Layout: codes [pages, heads, page, 128] bytes, scale [pages, heads] fp32;
+// position p of sequence b is row p % page of page table[b, p / page].
+// A scale is a power of two, 2^n with n the smallest whole number in
+// [-40, 119] such that the block's largest magnitude is at most 448 * 2^n.
+// A power of two makes x / s exact, so that a value is rounded once (by at
+// most 2^-4 of itself), and moving a block's codes to a larger scale (a later
+// token of the block is larger) rounds again only what falls below E4M3's
+// normal range: a general scale would add a rounding at every growth.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+#include "host.cuh"
+
+namespace wamb {
+
+constexpr int KV8_EXP_MIN = -40, KV8_EXP_MAX = 119;
+constexpr int KV8_DEV_ERROR = 5;   // WAMB_DEV_KV8: page id, length or count out of range
+
+struct Kv8Cache {
+  uint8_t* k8;
+  uint8_t* v8;
+  float* k_scale;
+  float* v_scale;
+  int pages, heads, page, page_log2;
+};
+
+// The sequences of a call.
+struct Kv8Seqs {
+  const int* table;    // [batch, width] page ids
+  const int* lens;     // [batch]
+  const int* counts;   // [batch] valid tokens of this call, or null (all)
+  int batch, width, tokens;
+};
+
+// Cached tokens of sequence b; out-of-range lengths are clamped and reported.
+WAMB_DEV int kv8_len(const Kv8Seqs& s, const Kv8Cache& c, int b) {
+  const int n = __ldg(s.lens + b);
+  const long long cap = static_cast<long long>(s.width) << c.page_log2;
+  if (n < 0 || n > cap) {
+    record_error(KV8_DEV_ERROR);
+    return n < 0 ? 0 : static_cast<int>(cap);
+  }
+  return n;
+}
+WAMB_DEV int kv8_count(const Kv8Seqs& s, int b) {
+  if (s.counts == nullptr) return s.tokens;
+  const int n = __ldg(s.counts + b);
+  if (n < 0 || n > s.tokens) {
+    record_error(KV8_DEV_ERROR);
+    return n < 0 ? 0 : s.tokens;
+  }
+  return n;
+}
+// Entry `i` of a page table row; -1 (reported) when it names no page.
+WAMB_DEV int kv8_page(const int* table, int width, const Kv8Cache& c, int b, int i) {
+  const int pid = __ldg(table + static_cast<long long>(b) * width + i);
+  if (pid < 0 || pid >= c.pages) {
+    record_error(KV8_DEV_ERROR);
+    return -1;
+  }
+  return pid;
+}
+
+WAMB_DEV float pow2f_exact(int n) { return __int_as_float((n + 127) << 23); }   // -126 <= n <= 127
+
+// n of the block scale 2^n for the largest magnitude `amax` (>= 0).
+// 448 = 1.75 * 2^8: with amax = 1.m * 2^e, n = e - 8, one more when 1.m > 1.75.
+WAMB_DEV int kv8_scale_exp(float amax) {
+  const int bits = __float_as_int(fminf(amax, 3.402823466e38f));
+  const int n = (bits >> 23) - 127 - 8 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0);
+  return max(KV8_EXP_MIN, min(KV8_EXP_MAX, n));
+}
+
+// Two E4M3 codes (low 16 bits) -> f16x2, exact.
+WAMB_DEV uint32_t e4m3x2_to_f16x2(uint32_t codes) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(codes));
+  return r;
+}
+WAMB_DEV float2 e4m3x2_to_float2(uint32_t codes) {
+  const uint32_t h = e4m3x2_to_f16x2(codes);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+WAMB_DEV void e4m3x8_to_float(uint2 w, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t u = i < 2 ? w.x : w.y;
+    const float2 v = e4m3x2_to_float2((i & 1) ? u >> 16 : u & 0xffffu);
+    f[2 * i] = v.x;
+    f[2 * i + 1] = v.y;
+  }
+}
+
+// Largest of a value over a 256-thread block (fmaxf: NaN loses).
+WAMB_DEV float block_max_256(float v, float* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = red[0];
+#pragma unroll
+  for (int i = 1; i < 8; ++i) v = fmaxf(v, red[i]);
+  return v;
+}
+
+// ------------------------------------------------------------------- write
+struct Kv8WriteParams {
+  Kv8Cache c;
+  Kv8Seqs s;
+  const void* x[2];            // K, V
+  long long sb[2], st[2], sh[2];   // element strides of (batch, token, head)
+};
+
+// One block per (touched page, head, sequence, K or V): the block's new rows
+// stay in registers between the amax and the rounding, so each is read once.
+// 16 threads hold a row (8 values each), 16 rows per pass, PAGE / 16 passes.
+// Bound by memory for chunks, by the launch for single tokens.
+template <bool F32, int PAGE>
+__global__ void __launch_bounds__(256) kv8_write_kernel(const Kv8WriteParams p) {
+  pdl_wait();
+  constexpr int PASSES = PAGE / 16;
+  __shared__ float red[8];
+  const int h = blockIdx.y, b = blockIdx.z >> 1, which = blockIdx.z & 1;
+  const int start = kv8_len(p.s, p.c, b);
+  int cnt = kv8_count(p.s, b);
+  const long long cap = static_cast<long long>(p.s.width) * PAGE;
+  if (start + static_cast<long long>(cnt) > cap) {   // the table has no room for the last tokens
+    if (threadIdx.x == 0) record_error(KV8_DEV_ERROR);
+    cnt = static_cast<int>(cap - start);
+  }
+  const int pi = start / PAGE + blockIdx.x;
+  const int lo = max(start, pi * PAGE);
+  const int hi = static_cast<int>(min(static_cast<long long>(start) + cnt, (pi + 1ll) * PAGE));
+  if (lo >= hi) return;
+  const int pid = kv8_page(p.s.table, p.s.width, p.c, b, pi);
+  if (pid < 0) return;
+  const int held = lo - pi * PAGE, n = hi - lo;
+  const int c8 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+  const long long base = b * p.sb[which] + h * p.sh[which] + (lo - start) * p.st[which] + c8 * 8;
+
+  uint4 raw[F32 ? 2 * PASSES : PASSES];
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int r = r0 + 16 * i;
+    const long long off = base + r * p.st[which];
+    if constexpr (F32) {
+      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(p.x[which]) + off);
+      raw[2 * i] = r < n ? __ldg(src) : make_uint4(0, 0, 0, 0);
+      raw[2 * i + 1] = r < n ? __ldg(src + 1) : make_uint4(0, 0, 0, 0);
+    } else {
+      raw[i] = r < n ? __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.x[which]) + off))
+                     : make_uint4(0, 0, 0, 0);
+    }
+  }
+  auto value = [&](int i, float (&f)[8]) {
+    if constexpr (F32) {
+      const uint4 a = raw[2 * i], d = raw[2 * i + 1];
+      f[0] = __uint_as_float(a.x); f[1] = __uint_as_float(a.y); f[2] = __uint_as_float(a.z); f[3] = __uint_as_float(a.w);
+      f[4] = __uint_as_float(d.x); f[5] = __uint_as_float(d.y); f[6] = __uint_as_float(d.z); f[7] = __uint_as_float(d.w);
+    } else {
+      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 v = unpack_bf16(w[k]);
+        f[2 * k] = v.x;
+        f[2 * k + 1] = v.y;
+      }
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    float f[8];
+    value(i, f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(f[k]));
+  }
+  amax = block_max_256(amax, red);
+  const long long blk = static_cast<long long>(pid) * p.c.heads + h;
+  float* scale = (which ? p.c.v_scale : p.c.k_scale) + blk;
+  uint8_t* codes = (which ? p.c.v8 : p.c.k8) + blk * (PAGE * 128) + c8 * 8;
+  const float s_old = held > 0 ? *scale : 0.f;
+  const float s = fmaxf(pow2f_exact(kv8_scale_exp(amax)), s_old);
+  const float inv = 1.f / s;
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int r = r0 + 16 * i;
+    if (r >= n) continue;
+    float f[8];
+    value(i, f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] *= inv;
+    *reinterpret_cast<uint2*>(codes + (held + r) * 128) = pack_e4m3x8(f);
+  }
+  if (s > s_old) {   // earlier tokens of the block move to the larger scale
+    const float ratio = s_old * inv;
+    for (int r = r0; r < held; r += 16) {
+      uint2* at = reinterpret_cast<uint2*>(codes + r * 128);
+      float f[8];
+      e4m3x8_to_float(*at, f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] *= ratio;
+      *at = pack_e4m3x8(f);
+    }
+    __syncthreads();   // every thread has read the old scale
+    if (threadIdx.x == 0) *scale = s;
+  }
+}
+
+// ------------------------------------------------------------------ evict
+struct Kv8EvictParams {
+  Kv8Cache c;
+  Kv8Seqs s;                 // counts null
+  const float* weights;      // [batch, heads, cap]
+  long long cap;             // columns of `weights`
+  const int* new_table;      // [batch, new_width]
+  int new_width;
+  int heavy, recent;
+  int* kept;                 // [batch, heads, new_width * page]
+  float* new_weights;        // like kept
+  int* new_lens;             // [batch]
+};
+
+// Order-preserving map of a weight: larger weights have larger keys, NaN
+// (either sign) is largest, -0 equals +0.
+WAMB_DEV uint32_t weight_key(float w) {
+  if (w != w) return 0xffffffffu;
+  const uint32_t b = __float_as_uint(w + 0.f);
+  return (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+
+// Kept tokens of sequence b: all of the last `recent`, and `heavy` of the rest.
+struct Kv8Kept {
+  int len, old, heavy, total;   // positions [0, old) compete for `heavy` places
+};
+WAMB_DEV Kv8Kept kv8_kept(const Kv8EvictParams& p, int b) {
+  Kv8Kept k;
+  k.len = kv8_len(p.s, p.c, b);
+  const int cap = static_cast<int>(min(2147483647ll, static_cast<long long>(p.new_width) << p.c.page_log2));
+  const int recent = min(min(p.recent, k.len), cap);
+  k.old = k.len - recent;
+  k.heavy = min(min(p.heavy, k.old), cap - recent);
+  k.total = k.heavy + recent;
+  return k;
+}
+
+constexpr int KV8_SEL_THREADS = 1024, KV8_SEL_BINS = 2048, KV8_SEL_COPIES = 4;
+
+// One block per (head, sequence). The heavy-th largest key is found by a
+// radix select (11, 11 and 10 bits, histograms in shared memory: whole-number
+// counts, so the order of the atomics does not matter), then one ordered pass
+// writes the kept positions: keys above the threshold, and of those equal to
+// it the lowest positions. Reads the weights four times (from L2 after the
+// first); bound by that one SM's latency.
+__global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8EvictParams p) {
+  pdl_wait();
+  __shared__ int hist[KV8_SEL_COPIES][KV8_SEL_BINS];
+  __shared__ int wsum[32], pick[2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int h = blockIdx.x, b = blockIdx.y;
+  const Kv8Kept k = kv8_kept(p, b);
+  const float* w = p.weights + (static_cast<long long>(b) * p.c.heads + h) * p.cap;
+  const long long out0 = (static_cast<long long>(b) * p.c.heads + h) * (static_cast<long long>(p.new_width) << p.c.page_log2);
+  const long long out_cap = static_cast<long long>(p.new_width) << p.c.page_log2;
+  int* kept = p.kept + out0;
+  float* nw = p.new_weights + out0;
+  if (h == 0 && tid == 0) p.new_lens[b] = k.total;
+
+  uint32_t prefix = 0, mask = 0;   // key bits fixed so far
+  int need = k.heavy;              // places left among keys that match the prefix
+  const bool select = k.heavy < k.old && k.heavy > 0;
+  if (select) {
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+      const int bits = pass == 2 ? 10 : 11;
+      for (int i = tid; i < KV8_SEL_COPIES * KV8_SEL_BINS; i += KV8_SEL_THREADS) (&hist[0][0])[i] = 0;
+      __syncthreads();
+      for (int i = tid; i < k.old; i += KV8_SEL_THREADS) {
+        const uint32_t key = weight_key(w[i]);
+        if ((key & mask) == prefix) atomicAdd(&hist[warp & (KV8_SEL_COPIES - 1)][(key >> shift) & ((1u << bits) - 1)], 1);
+      }
+      __syncthreads();
+      // Each thread owns two bins, highest first: thread t has bins 2047 - 2t, 2046 - 2t.
+      int c[2], mine = 0;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int bin = KV8_SEL_BINS - 1 - 2 * tid - j;
+        c[j] = 0;
+#pragma unroll
+        for (int q = 0; q < KV8_SEL_COPIES; ++q) c[j] += hist[q][bin];
+        mine += c[j];
+      }
+      int inc = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      if (lane == 31) wsum[warp] = inc;
+      __syncthreads();
+      int above = inc - mine;
+      for (int q = 0; q < warp; ++q) above += wsum[q];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (above < need && need <= above + c[j]) {
+          pick[0] = KV8_SEL_BINS - 1 - 2 * tid - j;
+          pick[1] = need - above;
+        }
+        above += c[j];
+      }
+      __syncthreads();
+      prefix |= static_cast<uint32_t>(pick[0]) << shift;
+      mask |= ((1u << bits) - 1) << shift;
+      need = pick[1];
+      __syncthreads();
+    }
+  }
+  // Ordered compaction of [0, old): at most `need` keys equal to the threshold.
+  int done = 0, eq_done = 0;
+  if (k.heavy > 0) {
+    for (int i0 = 0; i0 < k.old; i0 += KV8_SEL_THREADS) {
+      const int i = i0 + tid;
+      const float v = i < k.old ? w[i] : 0.f;
+      const uint32_t key = weight_key(v);
+      const bool gt = i < k.old && (!select || key > prefix);
+      const bool eq = i < k.old && select && key == prefix;
+      const unsigned mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq);
+      if (lane == 0) wsum[warp] = __popc(mg) | (__popc(me) << 16);
+      __syncthreads();
+      const int mine = wsum[lane];
+      int inc = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += u;
+      }
+      const int before = __shfl_sync(0xffffffffu, inc - mine, warp);
+      const int all = __shfl_sync(0xffffffffu, inc, 31);
+      const unsigned below = (1u << lane) - 1;
+      // Equal keys before this one, and how many of them were taken.
+      const int eq_before = eq_done + (before >> 16) + __popc(me & below);
+      const int gt_before = done + (before & 0xffff) + __popc(mg & below);
+      if (gt || (eq && eq_before < need)) {
+        const int at = gt_before + min(eq_before, select ? need : 0);
+        kept[at] = i;
+        nw[at] = v;
+      }
+      done += all & 0xffff;
+      eq_done += all >> 16;
+      __syncthreads();   // wsum is rewritten
+    }
+  }
+  for (long long j = k.heavy + tid; j < out_cap; j += KV8_SEL_THREADS) {
+    const bool live = j < k.total;
+    const int pos = k.old + static_cast<int>(j - k.heavy);
+    kept[j] = live ? pos : -1;
+    nw[j] = live ? w[pos] : 0.f;
+  }
+}
+
+// One block per (new page, head, sequence, K or V): gathers the kept rows
+// into registers, takes the new scale from their values and rounds them once.
+template <int PAGE>
+__global__ void __launch_bounds__(256) kv8_gather_kernel(const Kv8EvictParams p) {
+  pdl_wait();
+  constexpr int PASSES = PAGE / 16;
+  __shared__ float red[8];
+  __shared__ int bad;
+  const int h = blockIdx.y, b = blockIdx.z >> 1, which = blockIdx.z & 1;
+  const int total = kv8_kept(p, b).total;
+  const int n = min(PAGE, total - static_cast<int>(blockIdx.x) * PAGE);
+  if (n <= 0) return;
+  const int dst = kv8_page(p.new_table, p.new_width, p.c, b, blockIdx.x);
+  if (dst < 0) return;
+  // A page of the old table cannot receive rows: others still read it.
+  if (threadIdx.x == 0) bad = 0;
+  __syncthreads();
+  const int old_pages = (__ldg(p.s.lens + b) + PAGE - 1) / PAGE;
+  for (int i = threadIdx.x; i < min(old_pages, p.s.width); i += 256)
+    if (__ldg(p.s.table + static_cast<long long>(b) * p.s.width + i) == dst) bad = 1;
+  __syncthreads();
+  if (bad) {
+    if (threadIdx.x == 0) record_error(KV8_DEV_ERROR);
+    return;
+  }
+  const int c8 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+  const int* kept = p.kept + ((static_cast<long long>(b) * p.c.heads + h) * p.new_width + blockIdx.x) * PAGE;
+  const uint8_t* codes = which ? p.c.v8 : p.c.k8;
+  float* scales = which ? p.c.v_scale : p.c.k_scale;
+  uint2 raw[PASSES];
+  float sc[PASSES];
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int r = r0 + 16 * i;
+    raw[i] = make_uint2(0, 0);
+    sc[i] = 0.f;
+    if (r < n) {
+      const int pos = kept[r];
+      const int pid = kv8_page(p.s.table, p.s.width, p.c, b, pos / PAGE);
+      if (pid >= 0) {
+        const long long blk = static_cast<long long>(pid) * p.c.heads + h;
+        sc[i] = __ldg(scales + blk);
+        raw[i] = *reinterpret_cast<const uint2*>(codes + (blk * PAGE + pos % PAGE) * 128 + c8 * 8);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    float f[8];
+    e4m3x8_to_float(raw[i], f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(f[k]) * sc[i]);
+  }
+  amax = block_max_256(amax, red);
+  const float s = pow2f_exact(kv8_scale_exp(amax));
+  const float inv = 1.f / s;
+  const long long blk = static_cast<long long>(dst) * p.c.heads + h;
+  uint8_t* to = (which ? p.c.v8 : p.c.k8) + blk * (PAGE * 128) + c8 * 8;
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) {
+    const int r = r0 + 16 * i;
+    if (r >= n) continue;
+    float f[8];
+    e4m3x8_to_float(raw[i], f);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[k] = f[k] * sc[i] * inv;
+    *reinterpret_cast<uint2*>(to + r * 128) = pack_e4m3x8(f);
+  }
+  if (threadIdx.x == 0) scales[blk] = s;
+}
+
+}  // namespace wamb

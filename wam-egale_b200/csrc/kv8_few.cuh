@@ -1,0 +1,672 @@
+// Attention and attention weights over the E4M3 cache (kv8.cuh) for few query
+// rows: the single-token form and small groups, where the cache's bytes bound
+// the call.
+//
+//   s_ij = scale q_i . (code_j ks_j),  o_i = sum_j softmax_j(s_ij) code'_j vs_j
+//   lse_i = ln sum_j exp(s_ij),        w_j = sum_i exp(s_ij - lse_i)
+//
+// The `group` query heads of one cached head are rows of one tile (row
+// r = token * group + head in group), so each cached byte is read once for
+// all of them. A warp takes 16 keys at a time: their K and V codes (2 KB each)
+// come by TMA into its own ring, become f16 in registers (E4M3 is a subset of
+// f16, so nothing is rounded) and meet the queries in m16n8k16 products with
+// fp32 sums: Q (16 rows) x K^T, then P x V. Queries are scaled per row by a
+// power of two into f16's range first, which keeps their eight bits.
+//
+// The scales of a block enter the exponent: with y_ij = s_ij log2(e) +
+// log2(vs_j) the kernel sums P_ij = 2^(y_ij - M_i) against the codes, M_i a
+// running maximum of y (moved only when it grows by more than 2^8), and
+// l_i = sum_j P_ij / vs_j. P goes to the product as f16 with an offset of 2^6:
+// 11 bits down to 2^-20 of the row's maximum and whole steps of 2^-30 below.
+#pragma once
+#include "kv8.cuh"
+
+namespace wamb {
+
+struct Kv8AttnParams {
+  Kv8Cache c;
+  Kv8Seqs s;
+  const __nv_bfloat16* q;
+  long long q_sb, q_st, q_sh;      // element strides of (batch, token, head)
+  int group, causal;
+  float scale_log2;                // softmax scale * log2(e)
+  __nv_bfloat16* out;
+  long long o_sb, o_st, o_sh;
+  float* lse;                      // [batch, tokens, heads * group] or null
+  // attention weights
+  const float* lse_in;             // like lse
+  const float* base;               // [batch, heads, w_cap] or null (zeros)
+  float* weights;                  // like base; may be base
+  long long w_cap;
+  // stream-K: query tiles per sequence, CTAs, smallest share, partials
+  int qts, ctas, min_units;
+  float* part;
+};
+
+// --------------------------------------------------------------- schedule
+// The work of a call is a line of units. Entry e = b * qts + qt (a query tile
+// of QR rows of sequence b) has n(e) units of TK keys for each cached head;
+// entries follow one another, heads within an entry, key tiles within a
+// head: an item is one (entry, head). The line is cut into equal shares, one
+// per CTA, whatever the lengths, which only the device knows. A CTA finishes
+// items that lie in its share and leaves partials (max, sum, O) for the one
+// it joins in the middle (slot 0) and the one it leaves unfinished (slot 1).
+template <int QR, int TK>
+struct Kv8Line {
+  WAMB_DEV static int rows(const Kv8AttnParams& p, int b) { return kv8_count(p.s, b) * p.group; }
+  // Keys that the last row of the tile sees (every row of it sees no more).
+  WAMB_DEV static int visible(const Kv8AttnParams& p, int e) {
+    const int b = e / p.qts, qt = e - b * p.qts;
+    const int len = kv8_len(p.s, p.c, b);
+    if (!p.causal) return len;
+    const int t = kv8_count(p.s, b);
+    const int last = (min(t * p.group, (qt + 1) * QR) - 1) / p.group;
+    return max(0, min(len, len - t + last + 1));
+  }
+  // Units per head; a tile with rows has one at least (it must be answered).
+  WAMB_DEV static int units(const Kv8AttnParams& p, int e) {
+    const int b = e / p.qts, qt = e - b * p.qts;
+    if (qt * QR >= rows(p, b)) return 0;
+    return max(1, (visible(p, e) + TK - 1) / TK);
+  }
+};
+
+struct Kv8Item {
+  int e, h, n;         // entry, head, units
+  long long start;     // first unit on the line
+};
+
+// Moves `it` forward to the item that holds unit u.
+template <int QR, int TK>
+WAMB_DEV void kv8_seek(const Kv8AttnParams& p, Kv8Item& it, long long u) {
+  long long left = it.start + static_cast<long long>(it.n) * (p.c.heads - it.h);   // end of the entry
+  while (u >= left) {
+    it.start = left;
+    it.h = 0;
+    do { ++it.e; it.n = Kv8Line<QR, TK>::units(p, it.e); } while (it.n == 0);
+    left = it.start + static_cast<long long>(it.n) * p.c.heads;
+  }
+  const int skip = static_cast<int>((u - it.start) / it.n);
+  it.h += skip;
+  it.start += static_cast<long long>(skip) * it.n;
+}
+
+struct Kv8SchedSmem {
+  long long warp[32];
+  long long start;
+  int e;
+};
+struct Kv8Share {
+  long long units;     // of the whole line
+  int ctas;            // shares
+  long long u0, u1;
+  WAMB_DEV long long first(int cta) const { return cta * units / ctas; }
+};
+
+// The share of `cta` and the item of its first unit; false without work.
+// Called by the whole block.
+template <int QR, int TK, int THREADS>
+WAMB_DEV bool kv8_share(const Kv8AttnParams& p, int cta, Kv8SchedSmem& sm, Kv8Share& sh, Kv8Item& it) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int entries = p.s.batch * p.qts;
+  long long sum = 0;
+  for (int e = tid; e < entries; e += THREADS) sum += Kv8Line<QR, TK>::units(p, e);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  if (lane == 0) sm.warp[warp] = sum;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int i = 0; i < THREADS / 32; ++i) total += sm.warp[i];
+  sh.units = total * p.c.heads;
+  sh.ctas = static_cast<int>(min(static_cast<long long>(p.ctas), max(1ll, sh.units / p.min_units)));
+  if (sh.units == 0 || cta >= sh.ctas) return false;
+  sh.u0 = sh.first(cta);
+  sh.u1 = sh.first(cta + 1);
+  __syncthreads();
+  // The entry of u0: scan the entries' units a block at a time.
+  long long run = 0;
+  for (int e0 = 0;; e0 += THREADS) {
+    const int e = e0 + tid;
+    const long long mine = e < entries ? static_cast<long long>(Kv8Line<QR, TK>::units(p, e)) * p.c.heads : 0;
+    long long inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += v;
+    }
+    if (lane == 31) sm.warp[warp] = inc;
+    __syncthreads();
+    long long before = run;
+    for (int i = 0; i < THREADS / 32; ++i) {
+      if (i < warp) before += sm.warp[i];
+      run += sm.warp[i];
+    }
+    const long long end = before + inc;
+    if (end - mine <= sh.u0 && sh.u0 < end) {
+      sm.e = e;
+      sm.start = end - mine;
+    }
+    __syncthreads();
+    if (sh.u0 < run) break;
+  }
+  it.e = sm.e;
+  it.h = 0;
+  it.start = sm.start;
+  it.n = Kv8Line<QR, TK>::units(p, it.e);
+  kv8_seek<QR, TK>(p, it, sh.u0);
+  return true;
+}
+
+// Floats of a partial: O [QR][128] relative to the row's M, then M, l.
+template <int QR>
+__host__ __device__ constexpr size_t kv8_part_floats() { return static_cast<size_t>(QR) * 130; }
+
+// Final values of a row from its merged (M, l): out = O / l, lse.
+WAMB_DEV float kv8_row_lse(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f; }
+
+// Joins the partials of items that several CTAs worked on, in CTA order: one
+// block per (CTA, eight rows), one warp per row. Block c acts for the item
+// that CTA c finished but did not begin.
+template <int QR, int TK>
+__global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
+  pdl_wait();
+  __shared__ Kv8SchedSmem sm;
+  Kv8Share sh;
+  Kv8Item it;
+  const int c = blockIdx.x;
+  if (!kv8_share<QR, TK, 256>(p, c, sm, sh, it)) return;
+  if (it.start == sh.u0 || it.start + it.n > sh.u1) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = blockIdx.y * 8 + warp;
+  const int b = it.e / p.qts, qt = it.e - b * p.qts;
+  const int rr = qt * QR + row;
+  if (row >= QR || rr >= Kv8Line<QR, TK>::rows(p, b)) return;
+  const int c0 = static_cast<int>(((it.start + 1) * sh.ctas - 1) / sh.units);   // the CTA that began it
+  constexpr size_t PF = kv8_part_floats<QR>();
+  auto slot = [&](int k) { return p.part + static_cast<size_t>(2 * k + (k == c0 ? 1 : 0)) * PF; };
+  float m = -INFINITY;
+  for (int k = c0 + lane; k <= c; k += 32) m = fmaxf(m, __ldcg(slot(k) + QR * 128 + row));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  float l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k0 = c0; k0 <= c; k0 += 32) {
+    const int k = k0 + lane;
+    float w = 0.f;
+    if (k <= c) {
+      const float mk = __ldcg(slot(k) + QR * 128 + row);
+      w = mk == -INFINITY ? 0.f : exp2f(mk - m);
+      l += w * __ldcg(slot(k) + QR * 129 + row);
+    }
+    const int cnt = min(32, c - k0 + 1);
+#pragma unroll 8
+    for (int i = 0; i < cnt; ++i) {
+      const float wi = __shfl_sync(0xffffffffu, w, i);
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(slot(k0 + i) + row * 128) + lane);
+      acc.x += wi * v.x;
+      acc.y += wi * v.y;
+      acc.z += wi * v.z;
+      acc.w += wi * v.w;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  const int t = rr / p.group, hq = it.h * p.group + rr % p.group;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  *reinterpret_cast<uint2*>(p.out + b * p.o_sb + t * p.o_st + hq * p.o_sh + lane * 4) =
+      make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+  if (p.lse != nullptr && lane == 0)
+    p.lse[(static_cast<long long>(b) * p.s.tokens + t) * (p.c.heads * p.group) + hq] = kv8_row_lse(m, l);
+}
+
+// --------------------------------------------------------------- few rows
+constexpr int FEW_QR = 16, FEW_TK = 64, FEW_THREADS = 128, FEW_WARPS = 4;
+constexpr float FEW_RESCALE = 8.f;    // log2 growth of the maximum that moves it
+constexpr float FEW_OFFSET = 6.f;     // P is 2^6 at the maximum
+
+template <bool WEIGHTS>
+struct FewSmem {
+  static constexpr int STAGES = WEIGHTS ? 8 : 4;
+  static constexpr uint32_t STAGE_BYTES = WEIGHTS ? 2048 : 4096;    // 16 keys: K codes, V codes
+  static constexpr uint32_t RING = FEW_WARPS * STAGES * STAGE_BYTES;
+  static constexpr uint32_t LD = 132;                               // merge rows, padded
+  static constexpr uint32_t MERGE_OFF = RING;
+  static constexpr uint32_t MERGE_BYTES = WEIGHTS ? 0 : FEW_WARPS * FEW_QR * LD * 4;
+  static constexpr uint32_t ML_OFF = MERGE_OFF + MERGE_BYTES;       // m, l [warps][16]
+  static constexpr uint32_t BAR_OFF = ML_OFF + 2 * FEW_WARPS * FEW_QR * 4;
+  static constexpr uint32_t SCHED_OFF = BAR_OFF + FEW_WARPS * STAGES * 8;
+  static constexpr uint32_t TOTAL = 1024 + SCHED_OFF + sizeof(Kv8SchedSmem) + 16;
+};
+
+WAMB_DEV void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+WAMB_DEV uint32_t pack_f16(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+WAMB_DEV uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
+// A warp's 16 keys of one unit, as lane i of a batch holds them for unit i.
+struct FewUnit {
+  int row;        // first row in the [pages * heads * page, 128] code matrix
+  int k0;         // first key position; the number of live keys in bits 27..31
+  float ks, vs;
+  int e, h;
+  int last;       // this unit ends its item or the CTA's share
+};
+
+// One Q fragment set: the 16 rows of (entry, head) as f16 A operands of eight
+// 16-wide steps. Step s < 4 holds dims 16 t + 4 s + 0..3 of thread t = lane & 3
+// (the two halves of the step's 16 columns are this order for Q and K alike),
+// step s >= 4 dims 64 + 16 t + 4 (s - 4) + 0..3.
+struct FewQ {
+  uint32_t a[8][4];
+  float rf[2];        // row factor: (power-of-two row scale) * scale * log2(e); rows g, g + 8
+  int seen[2];        // keys each row sees
+};
+
+template <int QR, int TK>
+WAMB_DEV void few_load_q(const Kv8AttnParams& p, int e, int h, int qt, FewQ& f) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  const int b = e / p.qts;
+  const int tokens = kv8_count(p.s, b), len = kv8_len(p.s, p.c, b);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int rr = qt * QR + g + 8 * half;
+    const bool ok = rr < tokens * p.group;
+    const int t = rr / p.group;
+    const __nv_bfloat16* src = p.q + b * p.q_sb + t * p.q_st + (h * p.group + rr - t * p.group) * p.q_sh + 16 * t4;
+    float x[32];
+    float amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 w = ok ? __ldg(reinterpret_cast<const uint4*>(src + (i >> 1) * 64 + (i & 1) * 8)) : make_uint4(0, 0, 0, 0);
+      const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 v = unpack_bf16(ws[k]);
+        x[8 * i + 2 * k] = v.x;
+        x[8 * i + 2 * k + 1] = v.y;
+        amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
+      }
+    }
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    // The row's largest magnitude goes to [2^13, 2^14).
+    const int ex = min(max(__float_as_int(amax) >> 23, 14), 254);
+    const float up = __int_as_float((267 - ex) << 23);
+#pragma unroll
+    for (int s = 0; s < 8; ++s) {
+      f.a[s][half] = pack_f16(x[4 * s] * up, x[4 * s + 1] * up);
+      f.a[s][2 + half] = pack_f16(x[4 * s + 2] * up, x[4 * s + 3] * up);
+    }
+    f.rf[half] = __int_as_float((ex - 13) << 23) * p.scale_log2;
+    f.seen[half] = p.causal ? max(0, min(len, len - tokens + t + 1)) : len;
+    if (!ok) f.seen[half] = 0;
+  }
+}
+
+// S [16 rows][16 keys] of a warp's keys at `stage` (swizzled rows of 128 codes).
+WAMB_DEV void few_scores(uint32_t stage, const FewQ& q, float (&s)[2][4]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    // The two 16-byte pieces of the row, in an order that alternates with the
+    // row so that eight lanes cover all banks.
+    const uint32_t row = stage + (8 * j + g) * 128;
+    const int o = (g & 1) * 4;
+    const uint4 x = lds128(row + (((t4 + o) ^ g) << 4));
+    const uint4 y = lds128(row + (((t4 + 4 - o) ^ g) << 4));
+    const bool sw = g & 1;
+    const uint32_t w[8] = {sw ? y.x : x.x, sw ? y.y : x.y, sw ? y.z : x.z, sw ? y.w : x.w,
+                           sw ? x.x : y.x, sw ? x.y : y.y, sw ? x.z : y.z, sw ? x.w : y.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[j][i] = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      mma_f16_16816(s[j], q.a[k], e4m3x2_to_f16x2(w[k] & 0xffffu), e4m3x2_to_f16x2(w[k] >> 16));
+  }
+}
+
+// WEIGHTS = false: attention; units of every query tile are on the line.
+// WEIGHTS = true: p.qts is 1 on the line; each unit loops over `row_tiles`
+// tiles of 16 rows and owns its keys' sums, so no sum has a racing order.
+template <bool WEIGHTS>
+__global__ void __launch_bounds__(FEW_THREADS)
+    kv8_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                   const Kv8AttnParams p, const int row_tiles) {
+  using L = FewSmem<WEIGHTS>;
+  // The line of the weights has one entry per sequence whatever its rows.
+  constexpr int QR = WEIGHTS ? (1 << 30) : FEW_QR;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  Kv8SchedSmem& sched = *reinterpret_cast<Kv8SchedSmem*>(smem + L::SCHED_OFF);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::SCHED_OFF + sizeof(Kv8SchedSmem));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  const uint32_t ring = smem_u32(smem) + warp * (L::STAGES * L::STAGE_BYTES);
+  const uint32_t bars = smem_u32(smem + L::BAR_OFF) + warp * (L::STAGES * 8);
+  if (lane == 0)
+    for (int i = 0; i < L::STAGES; ++i) mbar_init(bars + 8 * i, 1);
+  if (threadIdx.x == 0) *abort_flag = 0;
+  fence_barrier_init();
+  pdl_wait();
+  if constexpr (WEIGHTS) {
+    // Columns past a sequence's keys carry the base over.
+    if (p.weights != p.base)
+      for (int i = blockIdx.x; i < p.s.batch * p.c.heads; i += gridDim.x) {
+        const int b = i / p.c.heads;
+        const int seen = kv8_count(p.s, b) > 0 ? kv8_len(p.s, p.c, b) : 0;
+        for (long long j = seen + threadIdx.x; j < p.w_cap; j += FEW_THREADS)
+          p.weights[i * p.w_cap + j] = p.base != nullptr ? p.base[i * p.w_cap + j] : 0.f;
+      }
+  }
+  Kv8Share sh;
+  Kv8Item it;
+  if (!kv8_share<QR, FEW_TK, FEW_THREADS>(p, blockIdx.x, sched, sh, it)) return;
+  const int count = static_cast<int>(sh.u1 - sh.u0);
+  const long long first_start = it.start;   // the item the share begins in
+
+  // Batches of 32 units: lane i holds unit i's addresses and scales, loaded a
+  // whole batch ahead of their use. `cur` moves over the line with them.
+  Kv8Item cur = it;
+  auto load_batch = [&](int j0, FewUnit& u) {
+    u.row = 0; u.k0 = 0; u.ks = 1.f; u.vs = 1.f; u.e = 0; u.h = 0; u.last = 0;
+    Kv8Item mine = cur;
+    const int j = min(j0 + lane, count - 1);
+    kv8_seek<QR, FEW_TK>(p, mine, sh.u0 + j);
+    if (j0 + lane < count) {
+      const int tile = static_cast<int>(sh.u0 + j - mine.start);
+      const int k0 = tile * FEW_TK + warp * 16;
+      const int live = max(0, min(16, Kv8Line<QR, FEW_TK>::visible(p, mine.e) - k0));
+      u.e = mine.e;
+      u.h = mine.h;
+      u.k0 = k0;
+      u.last = tile == mine.n - 1 || j == count - 1;
+      if (live > 0) {
+        int pid = kv8_page(p.s.table, p.s.width, p.c, mine.e / p.qts, k0 >> p.c.page_log2);
+        if (pid < 0) pid = 0;   // reported
+        const long long blk = static_cast<long long>(pid) * p.c.heads + mine.h;
+        u.row = static_cast<int>((blk << p.c.page_log2) + (k0 & (p.c.page - 1)));
+        u.ks = __ldg(p.c.k_scale + blk);
+        if constexpr (!WEIGHTS) u.vs = __ldg(p.c.v_scale + blk);
+      }
+      u.last |= live << 8;
+    }
+    cur.e = __shfl_sync(0xffffffffu, mine.e, 31);
+    cur.h = __shfl_sync(0xffffffffu, mine.h, 31);
+    cur.n = __shfl_sync(0xffffffffu, mine.n, 31);
+    cur.start = __shfl_sync(0xffffffffu, mine.start, 31);
+  };
+  FewUnit now, next;
+  load_batch(0, now);
+  if (count > 32) load_batch(32, next);
+  else next = now;
+  int issued = 0, used = 0, ahead = 0;   // ring loads issued and consumed; next unit to issue
+  auto issue = [&](int base) {   // base: first unit of `now`
+    while (ahead < count && ahead < base + 64 && issued < used + L::STAGES) {
+      const bool nx = ahead >= base + 32;
+      const int l = ahead & 31;
+      const int meta = __shfl_sync(0xffffffffu, nx ? next.last : now.last, l);
+      const int row = __shfl_sync(0xffffffffu, nx ? next.row : now.row, l);
+      if ((meta >> 8) > 0) {
+        const int st = issued % L::STAGES;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bars + 8 * st, L::STAGE_BYTES);
+          tma_load_2d(ring + st * L::STAGE_BYTES, &tmK, bars + 8 * st, 0, row);
+          if constexpr (!WEIGHTS) tma_load_2d(ring + st * L::STAGE_BYTES + 2048, &tmV, bars + 8 * st, 0, row);
+        }
+        ++issued;
+      }
+      ++ahead;
+    }
+  };
+  issue(0);
+
+  FewQ q;
+  float o[16][4];
+  float m[2], l[2];
+  auto reset = [&]() {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
+  };
+  bool fresh = true;
+  bool began = it.start == sh.u0;      // the current item begins in this share
+  long long item_start = first_start;
+  (void)item_start;
+  bool ok = true;
+  for (int j = 0; j < count; ++j) {
+    if ((j & 31) == 0 && j > 0) {
+      now = next;
+      if (j + 32 < count) load_batch(j + 32, next);
+    }
+    const int base = j & ~31;
+    const int src = j & 31;
+    const int meta = __shfl_sync(0xffffffffu, now.last, src);
+    const int e = __shfl_sync(0xffffffffu, now.e, src);
+    const int h = __shfl_sync(0xffffffffu, now.h, src);
+    const int k0 = __shfl_sync(0xffffffffu, now.k0, src);
+    const float ks = __shfl_sync(0xffffffffu, now.ks, src);
+    const int live = meta >> 8;
+    const int b = e / p.qts;
+    if constexpr (!WEIGHTS) {
+      if (fresh) {
+        few_load_q<FEW_QR, FEW_TK>(p, e, h, e - b * p.qts, q);
+        reset();
+        fresh = false;
+      }
+    }
+    uint32_t stage = 0;
+    if (live > 0) {
+      const int st = used % L::STAGES;
+      stage = ring + st * L::STAGE_BYTES;
+      ok = ok && mbar_wait(bars + 8 * st, (used / L::STAGES) & 1, abort_flag);
+    }
+    if constexpr (WEIGHTS) {
+      if (live > 0) {
+        float w[4] = {0.f, 0.f, 0.f, 0.f};   // keys 2 t, 2 t + 1, 8 + 2 t, 9 + 2 t
+        for (int qt = 0; qt < row_tiles; ++qt) {
+          if (fresh || row_tiles > 1) {
+            few_load_q<FEW_QR, FEW_TK>(p, e, h, qt, q);
+            // The rows' log-sum-exp in log2 units; rows that see nothing add nothing.
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const int rr = qt * FEW_QR + g + 8 * half;
+              const int t = rr / p.group;
+              l[half] = INFINITY;
+              if (rr < kv8_count(p.s, b) * p.group) {
+                const float x = p.lse_in[(static_cast<long long>(b) * p.s.tokens + t) * (p.c.heads * p.group) +
+                                         h * p.group + rr - t * p.group];
+                if (x != -INFINITY) l[half] = x * 1.4426950408889634f;
+              }
+            }
+            fresh = false;
+          }
+          float s[2][4];
+          few_scores(stage, q, s);
+#pragma unroll
+          for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int half = c >> 1, key = k0 + 8 * jt + 2 * t4 + (c & 1);
+              const float x = ex2_mufu(fmaf(s[jt][c], q.rf[half] * ks, -l[half]));
+              if (key < q.seen[half]) w[2 * jt + (c & 1)] += x;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) w[i] += __shfl_xor_sync(0xffffffffu, w[i], x);
+        }
+        if (g == 0) {
+          const long long at = (static_cast<long long>(b) * p.c.heads + h) * p.w_cap + k0;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int key = (i >> 1) * 8 + 2 * t4 + (i & 1);
+            if (key < live) p.weights[at + key] = ok ? (p.base != nullptr ? p.base[at + key] : 0.f) + w[i] : 0.f;
+          }
+        }
+        __syncwarp();
+        ++used;
+        issue(base);
+      }
+      if (meta & 1) fresh = true;
+    } else {
+      if (live > 0) {
+        const float vs = __shfl_sync(0xffffffffu, now.vs, src);
+        const float lv = log2f(vs), iv = 1.f / vs;
+        float s[2][4];
+        few_scores(stage, q, s);
+        const float f[2] = {q.rf[0] * ks, q.rf[1] * ks};
+        float y[2][4];
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int jt = 0; jt < 2; ++jt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int half = c >> 1, key = k0 + 8 * jt + 2 * t4 + (c & 1);
+            y[jt][c] = key < q.seen[half] ? fmaf(s[jt][c], f[half], lv) : -INFINITY;
+            mx[half] = fmaxf(mx[half], y[jt][c]);
+          }
+        if (__any_sync(0xffffffffu, mx[0] > m[0] + FEW_RESCALE || mx[1] > m[1] + FEW_RESCALE)) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float v = mx[half];
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
+            v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+            const float nm = fmaxf(m[half], v);
+            const float a = m[half] == -INFINITY ? 0.f : exp2f(m[half] - nm);
+            m[half] = nm;
+            l[half] *= a;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              o[i][2 * half] *= a;
+              o[i][2 * half + 1] *= a;
+            }
+          }
+        }
+        const float z0 = (m[0] == -INFINITY ? 0.f : m[0]) - FEW_OFFSET, z1 = (m[1] == -INFINITY ? 0.f : m[1]) - FEW_OFFSET;
+#pragma unroll
+        for (int jt = 0; jt < 2; ++jt) {
+          y[jt][0] = ex2_mufu(y[jt][0] - z0);
+          y[jt][1] = ex2_mufu(y[jt][1] - z0);
+          y[jt][2] = ex2_mufu(y[jt][2] - z1);
+          y[jt][3] = ex2_mufu(y[jt][3] - z1);
+        }
+        l[0] += (y[0][0] + y[0][1] + y[1][0] + y[1][1]) * iv;
+        l[1] += (y[0][2] + y[0][3] + y[1][2] + y[1][3]) * iv;
+        const uint32_t a[4] = {pack_f16(y[0][0], y[0][1]), pack_f16(y[0][2], y[0][3]), pack_f16(y[1][0], y[1][1]),
+                               pack_f16(y[1][2], y[1][3])};
+        // V rows 2 t, 2 t + 1, 8 + 2 t, 9 + 2 t, dims [16 g, +16); output
+        // column n = g of product i is dim 16 g + i.
+        uint4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = (i >> 1) * 8 + 2 * t4 + (i & 1);
+          v[i] = lds128(stage + 2048 + r * 128 + ((g ^ (r & 7)) << 4));
+          if (r >= live) v[i] = make_uint4(0, 0, 0, 0);   // whatever lies there (NaN codes too) counts for nothing
+        }
+        __syncwarp();
+        ++used;
+        issue(base);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t v0 = w == 0 ? v[0].x : w == 1 ? v[0].y : w == 2 ? v[0].z : v[0].w;
+          const uint32_t v1 = w == 0 ? v[1].x : w == 1 ? v[1].y : w == 2 ? v[1].z : v[1].w;
+          const uint32_t v2 = w == 0 ? v[2].x : w == 1 ? v[2].y : w == 2 ? v[2].z : v[2].w;
+          const uint32_t v3 = w == 0 ? v[3].x : w == 1 ? v[3].y : w == 2 ? v[3].z : v[3].w;
+          const uint32_t lo0 = __byte_perm(v0, v1, 0x5140), hi0 = __byte_perm(v0, v1, 0x7362);
+          const uint32_t lo1 = __byte_perm(v2, v3, 0x5140), hi1 = __byte_perm(v2, v3, 0x7362);
+          mma_f16_16816(o[4 * w], a, e4m3x2_to_f16x2(lo0 & 0xffffu), e4m3x2_to_f16x2(lo1 & 0xffffu));
+          mma_f16_16816(o[4 * w + 1], a, e4m3x2_to_f16x2(lo0 >> 16), e4m3x2_to_f16x2(lo1 >> 16));
+          mma_f16_16816(o[4 * w + 2], a, e4m3x2_to_f16x2(hi0 & 0xffffu), e4m3x2_to_f16x2(hi1 & 0xffffu));
+          mma_f16_16816(o[4 * w + 3], a, e4m3x2_to_f16x2(hi0 >> 16), e4m3x2_to_f16x2(hi1 >> 16));
+        }
+      }
+      if (meta & 1) {
+        // The item, or the share, ends: the warps' results meet in shared memory.
+        float* wm = reinterpret_cast<float*>(smem + L::ML_OFF);
+        float* wl = wm + FEW_WARPS * FEW_QR;
+        float* buf = reinterpret_cast<float*>(smem + L::MERGE_OFF) + warp * FEW_QR * L::LD;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
+          l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
+          const int r = g + 8 * half;
+          if (t4 == 0) {
+            wm[warp * FEW_QR + r] = m[half];
+            wl[warp * FEW_QR + r] = l[half];
+          }
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+              *reinterpret_cast<float4*>(buf + r * L::LD + 32 * t4 + 16 * c + i) =
+                  make_float4(o[i][2 * half + c], o[i + 1][2 * half + c], o[i + 2][2 * half + c], o[i + 3][2 * half + c]);
+        }
+        __syncthreads();
+        const int qt = e - b * p.qts;
+        const int rows = min(FEW_QR, kv8_count(p.s, b) * p.group - qt * FEW_QR);
+        // Whole only when the share holds the item's first and last unit.
+        const int vis = Kv8Line<QR, FEW_TK>::visible(p, e);
+        const int n = max(1, (vis + FEW_TK - 1) / FEW_TK);
+        const bool ends = (k0 - warp * 16) / FEW_TK == n - 1;
+        const bool whole = began && ends;
+        float* part = p.part + static_cast<size_t>(2 * blockIdx.x + (began ? 1 : 0)) * kv8_part_floats<FEW_QR>();
+        const float* mbuf = reinterpret_cast<const float*>(smem + L::MERGE_OFF);
+        for (int i = threadIdx.x; i < rows * 32; i += FEW_THREADS) {
+          const int r = i >> 5, c4 = i & 31;
+          float M = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < FEW_WARPS; ++w) M = fmaxf(M, wm[w * FEW_QR + r]);
+          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+          float den = 0.f;
+#pragma unroll
+          for (int w = 0; w < FEW_WARPS; ++w) {
+            const float mw = wm[w * FEW_QR + r];
+            const float x = mw == -INFINITY ? 0.f : exp2f(mw - M);
+            const float4 v = *reinterpret_cast<const float4*>(mbuf + (w * FEW_QR + r) * L::LD + c4 * 4);
+            den += x * wl[w * FEW_QR + r];
+            acc.x += x * v.x;
+            acc.y += x * v.y;
+            acc.z += x * v.z;
+            acc.w += x * v.w;
+          }
+          const float mref = M == -INFINITY ? M : M - FEW_OFFSET;
+          if (!ok) den = 0.f;
+          if (whole) {
+            const int rr = qt * FEW_QR + r, t = rr / p.group, hq = h * p.group + rr - t * p.group;
+            const float inv = den == 0.f ? 0.f : 1.f / den;
+            *reinterpret_cast<uint2*>(p.out + b * p.o_sb + t * p.o_st + hq * p.o_sh + c4 * 4) =
+                make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+            if (p.lse != nullptr && c4 == 0)
+              p.lse[(static_cast<long long>(b) * p.s.tokens + t) * (p.c.heads * p.group) + hq] = kv8_row_lse(mref, den);
+          } else {
+            reinterpret_cast<float4*>(part + r * 128)[c4] = acc;
+            if (c4 == 0) {
+              part[FEW_QR * 128 + r] = mref;
+              part[FEW_QR * 129 + r] = den;
+            }
+          }
+        }
+        __syncthreads();
+        fresh = true;
+        began = true;
+      }
+    }
+  }
+}
+
+}  // namespace wamb

@@ -7,6 +7,7 @@
 #include "block.cuh"
 #include "model.cuh"
 #include "speculative.cuh"
+#include "kv8_host.cuh"
 
 #include <cmath>
 
@@ -42,7 +43,7 @@ extern "C" {
 
 const char* wamb_last_error(void) { return wamb::g_last_error.c_str(); }
 
-int wamb_abi_version(void) { return 107; }
+int wamb_abi_version(void) { return 108; }
 
 int wamb_device_status(void* stream, int* device_code) {
   cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -384,6 +385,29 @@ int wamb_cfg_combine(const void* cond, const void* uncond, int32_t io_is_f32, in
   return launch_kernel(cfg_combine_kernel, dim3(elem_grid(n, di.sms)), dim3(256), 0,
                        static_cast<cudaStream_t>(stream), cond, uncond, out, io_is_f32, static_cast<long long>(n),
                        scale);
+}
+
+// ------------------------------------------------------- E4M3 KV cache
+int wamb_kv8_write(const wamb_kv8_write_args* args, void* stream) {
+  return wamb::kv8_write_impl(args, static_cast<cudaStream_t>(stream));
+}
+
+size_t wamb_kv8_attention_workspace_bytes(const wamb_kv8_attention_args* args) {
+  wamb::DeviceInfo di;
+  if (args == nullptr || wamb::device_info(&di) != WAMB_OK) return 0;
+  return wamb::kv8_attn_workspace(args, di);
+}
+
+int wamb_kv8_attention(const wamb_kv8_attention_args* args, void* stream) {
+  return wamb::kv8_attention_impl(args, false, static_cast<cudaStream_t>(stream));
+}
+
+int wamb_kv8_weights(const wamb_kv8_attention_args* args, void* stream) {
+  return wamb::kv8_attention_impl(args, true, static_cast<cudaStream_t>(stream));
+}
+
+int wamb_kv8_evict(const wamb_kv8_evict_args* args, void* stream) {
+  return wamb::kv8_evict_impl(args, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

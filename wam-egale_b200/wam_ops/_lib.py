@@ -93,6 +93,50 @@ class BlockArgs(ctypes.Structure):
     ]
 
 
+class Kv8CacheArgs(ctypes.Structure):
+    """Mirror of `wamb_kv8_cache` (include/wamb.h)."""
+    _fields_ = [
+        ("k8", c_void_p), ("v8", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+        ("pages", c_int32), ("heads", c_int32), ("page", c_int32),
+    ]
+
+
+class Kv8SeqsArgs(ctypes.Structure):
+    """Mirror of `wamb_kv8_seqs` (include/wamb.h)."""
+    _fields_ = [
+        ("batch", c_int32), ("tokens", c_int32), ("table_width", c_int32),
+        ("table", c_void_p), ("lens", c_void_p), ("counts", c_void_p),
+    ]
+
+
+class Kv8WriteArgs(ctypes.Structure):
+    """Mirror of `wamb_kv8_write_args` (include/wamb.h)."""
+    _fields_ = [
+        ("cache", Kv8CacheArgs), ("seqs", Kv8SeqsArgs), ("k", c_void_p), ("v", c_void_p),
+        ("k_stride", c_int64 * 3), ("v_stride", c_int64 * 3), ("x_is_f32", c_int32),
+    ]
+
+
+class Kv8AttentionArgs(ctypes.Structure):
+    """Mirror of `wamb_kv8_attention_args` (include/wamb.h)."""
+    _fields_ = [
+        ("cache", Kv8CacheArgs), ("seqs", Kv8SeqsArgs), ("q", c_void_p), ("q_stride", c_int64 * 3),
+        ("q_heads", c_int32), ("causal", c_int32), ("scale", ctypes.c_float),
+        ("out", c_void_p), ("out_stride", c_int64 * 3), ("lse", c_void_p),
+        ("base", c_void_p), ("weights", c_void_p), ("weights_cap", c_int64),
+        ("workspace", c_void_p), ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+class Kv8EvictArgs(ctypes.Structure):
+    """Mirror of `wamb_kv8_evict_args` (include/wamb.h)."""
+    _fields_ = [
+        ("cache", Kv8CacheArgs), ("seqs", Kv8SeqsArgs), ("weights", c_void_p), ("weights_cap", c_int64),
+        ("max_len", c_int64), ("new_table", c_void_p), ("new_width", c_int32), ("heavy", c_int32),
+        ("recent", c_int32), ("kept", c_void_p), ("new_weights", c_void_p), ("new_lens", c_void_p),
+    ]
+
+
 # Workspace taps (enum wamb_tap).
 TAPS = ("modulated1", "qkv", "self_attention", "residual1", "norm2", "cross_q", "cross_k",
         "cross_v", "cross_attention", "residual2", "modulated3", "gelu", "kv_slots",
@@ -101,7 +145,7 @@ TAPS = ("modulated1", "qkv", "self_attention", "residual1", "norm2", "cross_q", 
 # Weight slots the FP8 path reads as E4M3 (self q/k/v/out, cross q/out, FFN).
 FP8_WEIGHTS = (3, 5, 7, 9, 13, 19, 23, 25)
 
-ABI_VERSION = 107
+ABI_VERSION = 108
 
 # Every symbol include/wamb.h declares; tests check the library exports them.
 EXPORTED = (
@@ -112,6 +156,8 @@ EXPORTED = (
     "wamb_flow_step", "wamb_repeat_rows", "wamb_flow_step_cl",
     "wamb_draft_forward", "wamb_spec_scores", "wamb_spec_route", "wamb_spec_expand", "wamb_spec_commit",
     "wamb_cfg_combine",
+    "wamb_kv8_write", "wamb_kv8_attention_workspace_bytes", "wamb_kv8_attention", "wamb_kv8_weights",
+    "wamb_kv8_evict",
 )
 
 # Size of the fixed scratch array behind wamb_block_forward_noalloc.
@@ -170,6 +216,12 @@ def load():
     lib.wamb_spec_commit.argtypes = [c_void_p, c_void_p, c_void_p, c_int32, c_int64, ctypes.c_float,
                                      ctypes.c_float, ctypes.c_float, c_void_p, c_void_p, c_void_p]
     lib.wamb_cfg_combine.argtypes = [c_void_p, c_void_p, c_int32, c_int64, ctypes.c_float, c_void_p, c_void_p]
+    lib.wamb_kv8_write.argtypes = [ctypes.POINTER(Kv8WriteArgs), c_void_p]
+    lib.wamb_kv8_attention_workspace_bytes.argtypes = [ctypes.POINTER(Kv8AttentionArgs)]
+    lib.wamb_kv8_attention_workspace_bytes.restype = ctypes.c_size_t
+    lib.wamb_kv8_attention.argtypes = [ctypes.POINTER(Kv8AttentionArgs), c_void_p]
+    lib.wamb_kv8_weights.argtypes = [ctypes.POINTER(Kv8AttentionArgs), c_void_p]
+    lib.wamb_kv8_evict.argtypes = [ctypes.POINTER(Kv8EvictArgs), c_void_p]
     if lib.wamb_abi_version() != ABI_VERSION:
         raise WambError(f"{LIB_PATH} has ABI {lib.wamb_abi_version()}, expected {ABI_VERSION}: rebuild")
     _lib = lib
