@@ -1,6 +1,6 @@
 // Argument checks and launches of the E4M3 cache operators.
 #pragma once
-#include "kv8_few.cuh"
+#include "kv8_tc.cuh"
 
 namespace wamb {
 
@@ -126,11 +126,22 @@ inline int kv8_evict_impl(const wamb_kv8_evict_args* a, cudaStream_t s) {
   }
 }
 
-// Two CTAs of the few-row kernel fit an SM.
+// Two CTAs of the few-row kernel fit an SM, one of the tensor-core kernel.
 inline int kv8_few_ctas(const DeviceInfo& di) { return 2 * di.sms; }
 
+// A tile of 16 rows is one m16n8k16 operand; more rows go to the tcgen05
+// kernel, which reads each key once for 256 of them.
+inline bool kv8_is_few(int64_t rows) { return rows <= FEW_QR; }
+
+// Query rows of a sequence and cached head.
+inline int64_t kv8_rows(const wamb_kv8_attention_args* a) {
+  return a->cache.heads > 0 ? static_cast<int64_t>(a->seqs.tokens) * (a->q_heads / a->cache.heads) : 0;
+}
+// Two partials for each CTA.
 inline size_t kv8_attn_workspace(const wamb_kv8_attention_args* a, const DeviceInfo& di) {
-  return static_cast<size_t>(2) * kv8_few_ctas(di) * kv8_part_floats<FEW_QR>() * sizeof(float);
+  const size_t floats = kv8_is_few(kv8_rows(a)) ? kv8_few_ctas(di) * kv8_part_floats<FEW_QR>()
+                                                : di.sms * kv8_part_floats<KTC_QR>();
+  return 2 * floats * sizeof(float);
 }
 
 template <typename K>
@@ -159,7 +170,8 @@ inline int kv8_attention_impl(const wamb_kv8_attention_args* a, bool weights, cu
   WAMB_REQUIRE(static_cast<int64_t>(p.s.tokens) * p.group <= (1 << 29), WAMB_ERR_SHAPE, "kv8: %d x %d query rows",
                p.s.tokens, p.group);
   const int rows = p.s.tokens * p.group;
-  p.qts = weights ? 1 : (rows + FEW_QR - 1) / FEW_QR;
+  const bool few = kv8_is_few(rows);
+  p.qts = weights || few ? 1 : (rows + KTC_QR - 1) / KTC_QR;
   WAMB_REQUIRE(static_cast<int64_t>(p.s.batch) * std::max(1, p.qts) <= (1 << 30), WAMB_ERR_SHAPE, "kv8: too many query tiles");
   if (p.s.batch == 0 || (p.s.tokens == 0 && !weights)) return WAMB_OK;
   WAMB_REQUIRE(p.s.tokens == 0 || a->q, WAMB_ERR_ARG, "kv8: null q");
@@ -202,10 +214,12 @@ inline int kv8_attention_impl(const wamb_kv8_attention_args* a, bool weights, cu
     p.part = static_cast<float*>(a->workspace);
   }
   const uint64_t code_rows = static_cast<uint64_t>(p.c.pages) * p.c.heads * p.c.page;
+  // Boxes of the TMA loads: the few-row kernel takes 16 keys, the other whole pages.
+  const uint32_t box = weights || few ? 16 : p.c.page;
   CUtensorMap tmK, tmV;
-  rc = make_tmap_2d(&tmK, p.c.k8, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, code_rows, 128, 128, 16, 128);
+  rc = make_tmap_2d(&tmK, p.c.k8, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, code_rows, 128, 128, box, 128);
   if (rc) return rc;
-  rc = make_tmap_2d(&tmV, p.c.v8, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, code_rows, 128, 128, 16, 128);
+  rc = make_tmap_2d(&tmV, p.c.v8, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, code_rows, 128, 128, box, 128);
   if (rc) return rc;
   p.ctas = kv8_few_ctas(di);
   p.min_units = 1;
@@ -216,13 +230,23 @@ inline int kv8_attention_impl(const wamb_kv8_attention_args* a, bool weights, cu
     return launch_kernel(kv8_few_kernel<true>, dim3(p.ctas), dim3(FEW_THREADS), FewSmem<true>::TOTAL, s, tmK, tmV, p,
                          (rows + FEW_QR - 1) / FEW_QR);
   }
+  if (few) {
+    static bool done[64] = {};
+    rc = kv8_smem_once(kv8_few_kernel<false>, FewSmem<false>::TOTAL, done);
+    if (rc) return rc;
+    rc = launch_kernel(kv8_few_kernel<false>, dim3(p.ctas), dim3(FEW_THREADS), FewSmem<false>::TOTAL, s, tmK, tmV, p, 1);
+    if (rc) return rc;
+    if (cap <= FEW_TK) return WAMB_OK;   // one unit per item: nothing is ever shared
+    return launch_kernel(kv8_merge_kernel<FEW_QR, FEW_TK>, dim3(p.ctas, (rows + 7) / 8), dim3(256), 0, s, p);
+  }
+  p.ctas = di.sms;
   static bool done[64] = {};
-  rc = kv8_smem_once(kv8_few_kernel<false>, FewSmem<false>::TOTAL, done);
+  rc = kv8_smem_once(kv8_tc_kernel, KtcSmem::TOTAL, done);
   if (rc) return rc;
-  rc = launch_kernel(kv8_few_kernel<false>, dim3(p.ctas), dim3(FEW_THREADS), FewSmem<false>::TOTAL, s, tmK, tmV, p, 1);
+  rc = launch_kernel(kv8_tc_kernel, dim3(p.ctas), dim3(KTC_THREADS), KtcSmem::TOTAL, s, tmK, tmV, p);
   if (rc) return rc;
-  if (cap <= FEW_TK) return WAMB_OK;   // one unit per item: nothing is ever shared
-  return launch_kernel(kv8_merge_kernel<FEW_QR, FEW_TK>, dim3(p.ctas, std::min(2, (rows + 7) / 8)), dim3(256), 0, s, p);
+  if (cap <= KTC_TK) return WAMB_OK;
+  return launch_kernel(kv8_merge_kernel<KTC_QR, KTC_TK>, dim3(p.ctas, (std::min(rows, KTC_QR) + 7) / 8), dim3(256), 0, s, p);
 }
 
 }  // namespace wamb

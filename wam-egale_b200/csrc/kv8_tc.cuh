@@ -1,0 +1,526 @@
+// Attention over the E4M3 cache for more than a few query rows, on the
+// tcgen05 tensor cores. The mathematics, the rows of a query tile and the
+// stream-K line of units are those of kv8_few.cuh, with tiles of 256 rows and
+// units of 128 keys.
+//
+// S = Q K^T reads K's codes as they lie in the cache (kind::f8f6f4, no
+// conversion): a bf16 query has eight significant bits, which are two E4M3
+// values of four, q 2^-n = hi + lo, so S = (hi K^T + lo K^T) 2^n costs what
+// one bf16 product does. n puts the row's largest magnitude in (224, 448]; a
+// value smaller than 2^-10 of it keeps an absolute error of at most 2^-10
+// (2^-18 of the largest). The E4M3 product sums in full fp32 here (measured:
+// 9e-9 relative error against 64 bits at K 128, bf16's is 1.2e-7).
+// O += P V needs more range than two E4M3 pieces of P hold (a long flat tail
+// beside a sharp maximum), so P is f16 as in kv8_few.cuh and V's codes become
+// f16 in shared memory, once for 256 rows, by two warps of their own.
+//
+// One CTA per SM, 384 threads:
+//   warps 0..7   softmax, one thread per query row: warps 0-3 on TMEM slot A,
+//                warps 4-7 on slot B. They also split the queries into smem.
+//   warp 8       producer: page ids and scales (read four tiles ahead), TMA
+//                of K and V codes, the scales of each 16 keys to a ring
+//   warp 9       its lane 0 issues the MMAs
+//   warps 10, 11 V codes -> f16
+// With more than 128 rows, slot A and slot B hold the tile's two halves and
+// meet every key tile; with fewer, both hold the same rows and take the key
+// tiles in turn (joined at the end), so that one slot's softmax always runs
+// beside the other's products. In both cases the work is a row of steps, step
+// s on slot s & 1: S(s + 2) is issued behind PV(s).
+// TMEM columns: S/P of A [0,128), of B [128,256), O_A [256,384), O_B [384,512).
+#pragma once
+#include "attention.cuh"
+#include "kv8_few.cuh"
+
+namespace wamb {
+
+constexpr int KTC_THREADS = 384, KTC_QR = 256, KTC_TK = 128;
+constexpr uint32_t KTC_TILE8 = 128 * 128;      // 128 rows of 128 codes
+constexpr int KTC_KS = 3, KTC_V8S = 2, KTC_V16S = 2, KTC_SCS = 8;
+
+struct KtcSmem {
+  static constexpr uint32_t Q_OFF = 0;                                       // slot A hi, lo, slot B hi, lo
+  static constexpr uint32_t K_OFF = Q_OFF + 4 * KTC_TILE8;
+  static constexpr uint32_t V8_OFF = K_OFF + KTC_KS * KTC_TILE8;
+  static constexpr uint32_t V16_OFF = V8_OFF + KTC_V8S * KTC_TILE8;
+  static constexpr uint32_t SC_OFF = V16_OFF + KTC_V16S * 2 * KTC_TILE8;     // [8 tiles][8 groups of 16 keys] float4
+  static constexpr uint32_t XCH_OFF = SC_OFF + KTC_SCS * 8 * 16;             // m, l of both slots
+  static constexpr uint32_t BAR_OFF = XCH_OFF + 2 * 2 * 128 * 4;
+  static constexpr uint32_t NBARS = 2 * KTC_KS + 2 * KTC_V8S + 2 * KTC_V16S + 2 + 2 + 3 + KTC_SCS;
+  static constexpr uint32_t SCHED_OFF = BAR_OFF + NBARS * 8;
+  static constexpr uint32_t TOTAL = 1024 + SCHED_OFF + sizeof(Kv8SchedSmem) + 16;
+  static_assert(TOTAL <= 232448, "shared memory exceeds 227 KB");
+};
+
+// kind::f16 instruction descriptor with f16 operands, B MN-major.
+__host__ __device__ constexpr uint32_t idesc_f16_mn(int M, int N) {
+  return (1u << 4) | (1u << 16) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+WAMB_DEV void sts128(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// Row `row` of a query tile into its two E4M3 pieces at hi / lo (swizzled
+// 128-byte rows, row r of the tile); returns 2^n. All 128 values by one thread.
+template <bool STORE>
+WAMB_DEV float ktc_split_q(const __nv_bfloat16* src, bool ok, uint32_t hi, uint32_t lo, int r) {
+  uint4 w[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) w[i] = ok ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 v = unpack_bf16(u[k]);
+      amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
+    }
+  }
+  // Scale exponent as for a cache block, over fp32's whole range.
+  const int bits = __float_as_int(fminf(amax, 3.402823466e38f));
+  const int n = max(-118, min(119, (bits >> 23) - 135 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0)));
+  if constexpr (STORE) {
+    // An infinite query makes its row NaN, as the formula does (a saturated one would not).
+    const float up = amax <= 3.402823466e38f ? pow2f_exact(-n) : __int_as_float(0x7fffffff);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {   // 16 values: one swizzled piece
+      uint32_t h[4], l[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint4 q = w[2 * i + (k >> 1)];
+        const float2 a = unpack_bf16((k & 1) ? q.z : q.x), b = unpack_bf16((k & 1) ? q.w : q.y);
+        const float x[4] = {a.x * up, a.y * up, b.x * up, b.y * up};
+        const uint32_t h0 = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t h1 = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
+        const float2 f0 = e4m3x2_to_float2(h0), f1 = e4m3x2_to_float2(h1);
+        const uint32_t l0 = __nv_cvt_float2_to_fp8x2(make_float2(x[0] - f0.x, x[1] - f0.y), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t l1 = __nv_cvt_float2_to_fp8x2(make_float2(x[2] - f1.x, x[3] - f1.y), __NV_SATFINITE, __NV_E4M3);
+        h[k] = h0 | (h1 << 16);
+        l[k] = l0 | (l1 << 16);
+      }
+      const uint32_t at = r * 128 + ((i ^ (r & 7)) << 4);
+      sts128(hi + at, make_uint4(h[0], h[1], h[2], h[3]));
+      sts128(lo + at, make_uint4(l[0], l[1], l[2], l[3]));
+    }
+  }
+  return pow2f_exact(n);
+}
+
+// One CTA's walk over the segments of its share.
+struct KtcWalk {
+  Kv8Item it;
+  long long u;
+  WAMB_DEV bool done(const Kv8Share& sh) const { return u >= sh.u1; }
+  WAMB_DEV void next(const Kv8AttnParams& p, const Kv8Share& sh) {
+    u = min(sh.u1, it.start + it.n);
+    if (u < sh.u1) kv8_seek<KTC_QR, KTC_TK>(p, it, u);
+  }
+};
+struct KtcSeg {
+  int b, qt, rows;     // sequence, query tile, its rows (1..256)
+  int j0, n;           // key tiles [j0, j0 + n)
+  int vis;             // keys that the tile's last row sees
+  bool two;            // two query halves (rows > 128)
+  bool begins, ends;
+  WAMB_DEV KtcSeg(const Kv8AttnParams& p, const Kv8Share& sh, const KtcWalk& w) {
+    b = w.it.e / p.qts;
+    qt = w.it.e - b * p.qts;
+    rows = min(KTC_QR, Kv8Line<KTC_QR, KTC_TK>::rows(p, b) - qt * KTC_QR);
+    j0 = static_cast<int>(w.u - w.it.start);
+    n = static_cast<int>(min(sh.u1, w.it.start + w.it.n) - w.u);
+    vis = Kv8Line<KTC_QR, KTC_TK>::visible(p, w.it.e);
+    two = rows > 128;
+    begins = j0 == 0;
+    ends = j0 + n == w.it.n;
+  }
+  WAMB_DEV int live(int j) const { return max(0, min(KTC_TK, vis - (j0 + j) * KTC_TK)); }
+};
+
+__global__ void __launch_bounds__(KTC_THREADS, 1)
+    kv8_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                  const Kv8AttnParams p) {
+  using L = KtcSmem;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const uint32_t base = smem_u32(smem);
+  const uint32_t sQ = base + L::Q_OFF, sK = base + L::K_OFF, sV8 = base + L::V8_OFF, sV16 = base + L::V16_OFF;
+  uint32_t bar = base + L::BAR_OFF;
+  auto bars = [&](int n) { const uint32_t b = bar; bar += 8 * n; return b; };
+  const uint32_t k_full = bars(KTC_KS), k_empty = bars(KTC_KS), v8_full = bars(KTC_V8S), v8_empty = bars(KTC_V8S),
+                 v16_full = bars(KTC_V16S), v16_empty = bars(KTC_V16S), s_full = bars(2), p_full = bars(2),
+                 q_full = bars(1), o_done = bars(1), drain = bars(1), sc_full = bars(KTC_SCS);
+  Kv8SchedSmem& sched = *reinterpret_cast<Kv8SchedSmem*>(smem + L::SCHED_OFF);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::SCHED_OFF + sizeof(Kv8SchedSmem));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  pdl_wait();
+  Kv8Share sh;
+  KtcWalk walk;
+  if (!kv8_share<KTC_QR, KTC_TK, KTC_THREADS>(p, blockIdx.x, sched, sh, walk.it)) return;
+  walk.u = sh.u0;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < KTC_KS; ++i) { mbar_init(k_full + 8 * i, 1); mbar_init(k_empty + 8 * i, 1); }
+    for (int i = 0; i < KTC_V8S; ++i) { mbar_init(v8_full + 8 * i, 1); mbar_init(v8_empty + 8 * i, 2); }
+    for (int i = 0; i < KTC_V16S; ++i) { mbar_init(v16_full + 8 * i, 2); mbar_init(v16_empty + 8 * i, 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(s_full + 8 * i, 1); mbar_init(p_full + 8 * i, 4); }
+    mbar_init(q_full, 8);
+    mbar_init(o_done, 1);
+    mbar_init(drain, 1);
+    for (int i = 0; i < KTC_SCS; ++i) mbar_init(sc_full + 8 * i, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 8) {
+    // ---------------------------------------------------------- producer
+    // Lane (to, gi) looks after keys [16 gi, +16) of tile `to` of a batch of four.
+    const int to = lane >> 3, gi = lane & 7;
+    const int box_groups = p.c.page >> 4;   // 16-key groups of one page
+    int tiles = 0;                          // key tiles so far
+    bool go = true;
+    for (; go && !walk.done(sh); walk.next(p, sh)) {
+      const KtcSeg sg(p, sh, walk);
+      const int h = walk.it.h;
+      struct Ahead { int row; float ks, lv, iv; bool live; };
+      auto load = [&](int j) {
+        Ahead a{0, 1.f, 0.f, 1.f, false};
+        const int key = (sg.j0 + j + to) * KTC_TK + gi * 16;
+        if (j + to < sg.n && key < sg.vis) {
+          int pid = kv8_page(p.s.table, p.s.width, p.c, sg.b, key >> p.c.page_log2);
+          if (pid < 0) pid = 0;   // reported
+          const long long blk = static_cast<long long>(pid) * p.c.heads + h;
+          a.row = static_cast<int>((blk << p.c.page_log2) + (key & (p.c.page - 1)));
+          a.ks = __ldg(p.c.k_scale + blk);
+          const float vs = __ldg(p.c.v_scale + blk);
+          a.lv = log2f(vs);
+          a.iv = 1.f / vs;
+          a.live = true;
+        }
+        return a;
+      };
+      Ahead now = load(0);
+      for (int jb = 0; go && jb < sg.n; jb += 4) {
+        const Ahead next = load(jb + 4);
+        for (int i = 0; i < 4 && jb + i < sg.n; ++i, ++tiles) {
+          const int sc = tiles % KTC_SCS;
+          if (to == i)
+            *reinterpret_cast<float4*>(smem + L::SC_OFF + (sc * 8 + gi) * 16) = make_float4(now.ks, now.lv, now.iv, 0.f);
+          const bool lead = to == i && now.live && gi % box_groups == 0;
+          const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, lead)) * (p.c.page * 128);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(sc_full + 8 * sc);
+          const int ks = tiles % KTC_KS, vs = tiles % KTC_V8S;
+          go = mbar_wait(k_empty + 8 * ks, ((tiles / KTC_KS) & 1) ^ 1, abort_flag);
+          go = __all_sync(0xffffffffu, go);
+          if (!go) break;
+          if (lane == 0) mbar_arrive_expect_tx(k_full + 8 * ks, bytes);
+          __syncwarp();
+          if (lead) tma_load_2d(sK + ks * KTC_TILE8 + gi * 2048, &tmK, k_full + 8 * ks, 0, now.row);
+          go = mbar_wait(v8_empty + 8 * vs, ((tiles / KTC_V8S) & 1) ^ 1, abort_flag);
+          go = __all_sync(0xffffffffu, go);
+          if (!go) break;
+          if (lane == 0) mbar_arrive_expect_tx(v8_full + 8 * vs, bytes);
+          __syncwarp();
+          if (lead) tma_load_2d(sV8 + vs * KTC_TILE8 + gi * 2048, &tmV, v8_full + 8 * vs, 0, now.row);
+        }
+        now = next;
+      }
+    }
+    // Loads still in flight must land before the CTA exits.
+    if (lane == 0 && go) {
+      for (int t = max(0, tiles - KTC_KS); t < tiles; ++t) mbar_wait_teardown(k_full + 8 * (t % KTC_KS), (t / KTC_KS) & 1);
+      for (int t = max(0, tiles - KTC_V8S); t < tiles; ++t) mbar_wait_teardown(v8_full + 8 * (t % KTC_V8S), (t / KTC_V8S) & 1);
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    if (lane == 0) {
+      // ------------------------------------------------------- MMA issuer
+      constexpr uint32_t IDESC_S = idesc_e4m3(128, 128);
+      constexpr uint32_t IDESC_O = idesc_f16_mn(128, 128);
+      int tile0 = 0;                       // key tiles of earlier segments
+      int pcount[2] = {0, 0};              // P tiles taken from each slot
+      bool ok = true;
+      for (int seg = 0; ok && !walk.done(sh); walk.next(p, sh), ++seg) {
+        const KtcSeg sg(p, sh, walk);
+        const int steps = sg.two ? 2 * sg.n : sg.n;
+        auto issue_s = [&](int s) {
+          const int t = s & 1, j = sg.two ? s >> 1 : s, k = tile0 + j;
+          const uint32_t kb = sK + (k % KTC_KS) * KTC_TILE8;
+          const uint32_t qb = sQ + (sg.two ? t * 2 * KTC_TILE8 : 0);
+          if (!mbar_wait(k_full + 8 * (k % KTC_KS), (k / KTC_KS) & 1, abort_flag)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk)   // hi piece, then lo piece: 4 x 32 dims each
+            umma_e4m3(tmem + t * 128, sw128_desc(qb + (kk >> 2) * KTC_TILE8 + (kk & 3) * 32, 16, 1024),
+                      sw128_desc(kb + (kk & 3) * 32, 16, 1024), IDESC_S, kk > 0);
+          umma_commit(s_full + 8 * t);
+          if (!sg.two || t == 1) umma_commit(k_empty + 8 * (k % KTC_KS));
+          return true;
+        };
+        ok = mbar_wait(q_full, seg & 1, abort_flag);
+        if (ok) tc_fence_after();
+        if (ok) ok = issue_s(0);
+        if (ok && steps > 1) ok = issue_s(1);
+        for (int s = 0; ok && s < steps; ++s) {
+          const int t = s & 1, j = sg.two ? s >> 1 : s, k = tile0 + j;
+          const uint32_t vb = sV16 + (k % KTC_V16S) * 2 * KTC_TILE8;
+          ok = mbar_wait(v16_full + 8 * (k % KTC_V16S), (k / KTC_V16S) & 1, abort_flag) &&
+               mbar_wait(p_full + 8 * t, pcount[t] & 1, abort_flag);
+          if (!ok) break;
+          ++pcount[t];
+          tc_fence_after();
+          const int ksteps = max(1, (sg.live(j) + 15) >> 4);
+          const bool first = s < 2;
+          for (int kk = 0; kk < ksteps; ++kk)
+            umma_bf16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, sw128_desc(vb + kk * 2048, KTC_TILE8, 1024),
+                         IDESC_O, !first || kk > 0);
+          if (!sg.two || t == 1) umma_commit(v16_empty + 8 * (k % KTC_V16S));
+          if (s + 2 < steps) ok = issue_s(s + 2);
+        }
+        umma_commit(o_done);
+        tile0 += sg.n;
+      }
+      umma_commit(drain);
+      mbar_wait_teardown(drain, 0);
+    }
+    __syncwarp();
+  } else if (warp >= 10) {
+    // --------------------------------------------- V codes -> f16 tiles
+    const int ct = threadIdx.x - 320;    // 0..63
+    int tiles = 0;
+    bool ok = true;
+    for (; ok && !walk.done(sh); walk.next(p, sh)) {
+      const KtcSeg sg(p, sh, walk);
+      for (int j = 0; ok && j < sg.n; ++j, ++tiles) {
+        const int vs = tiles % KTC_V8S, vd = tiles % KTC_V16S;
+        ok = mbar_wait(v8_full + 8 * vs, (tiles / KTC_V8S) & 1, abort_flag) &&
+             mbar_wait(v16_empty + 8 * vd, ((tiles / KTC_V16S) & 1) ^ 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        const uint32_t src = sV8 + vs * KTC_TILE8, dst = sV16 + vd * 2 * KTC_TILE8;
+        const int live = sg.live(j);
+#pragma unroll 4
+        for (int i = 0; i < 16; ++i) {
+          // 16 codes (piece c of row r) -> two pieces of 8 f16 in column half c / 4.
+          const int id = i * 64 + ct, r = id >> 3, c = id & 7;
+          uint4 w = lds128(src + r * 128 + ((c ^ (r & 7)) << 4));
+          if (r >= live) w = make_uint4(0, 0, 0, 0);   // whatever lies there (NaN codes too) counts for nothing
+          const uint4 lo = make_uint4(e4m3x2_to_f16x2(w.x & 0xffffu), e4m3x2_to_f16x2(w.x >> 16),
+                                      e4m3x2_to_f16x2(w.y & 0xffffu), e4m3x2_to_f16x2(w.y >> 16));
+          const uint4 hi = make_uint4(e4m3x2_to_f16x2(w.z & 0xffffu), e4m3x2_to_f16x2(w.z >> 16),
+                                      e4m3x2_to_f16x2(w.w & 0xffffu), e4m3x2_to_f16x2(w.w >> 16));
+          // The lanes of the two halves store their pieces in opposite order: no bank twice.
+          const uint32_t at = dst + (c >> 2) * KTC_TILE8 + r * 128;
+          const int k0 = (c & 3) * 2, first = c >> 2;
+          sts128(at + (((k0 + first) ^ (r & 7)) << 4), first ? hi : lo);
+          sts128(at + (((k0 + 1 - first) ^ (r & 7)) << 4), first ? lo : hi);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(v16_full + 8 * vd);
+          mbar_arrive(v8_empty + 8 * vs);
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------ softmax / epilogue
+    const int t = warp >> 2;          // TMEM slot
+    const int r = (warp & 3) * 32 + lane;
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tS = tmem + lane_base + t * 128, tO = tmem + lane_base + 256 + t * 128;
+    int tile0 = 0, scount = 0;
+    bool ok = true;
+    for (int seg = 0; !walk.done(sh); walk.next(p, sh), ++seg) {
+      const KtcSeg sg(p, sh, walk);
+      const int h = walk.it.h;
+      const int rr = sg.qt * KTC_QR + (sg.two ? t * 128 : 0) + r;     // row of the (sequence, head)
+      const bool valid = rr < sg.qt * KTC_QR + sg.rows;
+      const int tok = rr / p.group;
+      const __nv_bfloat16* qrow = p.q + sg.b * p.q_sb + tok * p.q_st + (h * p.group + rr - tok * p.group) * p.q_sh;
+      float rf;
+      if (sg.two || t == 0) {
+        const uint32_t qs = sQ + t * 2 * KTC_TILE8;
+        rf = ktc_split_q<true>(qrow, valid, qs, qs + KTC_TILE8, r);
+        fence_proxy_async();
+      } else {
+        rf = ktc_split_q<false>(qrow, valid, 0, 0, r);
+      }
+      rf *= p.scale_log2;
+      tc_fence_before();   // the last segment's reads of TMEM
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+      const int len = kv8_len(p.s, p.c, sg.b);
+      const int seen = p.causal ? max(0, min(len, len - kv8_count(p.s, sg.b) + tok + 1)) : len;
+      float m = -INFINITY, l = 0.f;
+      const int mine = sg.two ? sg.n : (sg.n + 1 - t) >> 1;   // key tiles of this slot
+      for (int i = 0; ok && i < mine; ++i, ++scount) {
+        const int j = sg.two ? i : 2 * i + t;
+        const int sc = (tile0 + j) % KTC_SCS;
+        ok = mbar_wait(sc_full + 8 * sc, ((tile0 + j) / KTC_SCS) & 1, abort_flag) &&
+             mbar_wait(s_full + 8 * t, scount & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const float4* scale = reinterpret_cast<const float4*>(smem + L::SC_OFF) + sc * 8;
+        const int lim = seen - (sg.j0 + j) * KTC_TK;    // keys of this tile that the row sees
+        const bool part = __any_sync(0xffffffffu, lim < KTC_TK);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float s[32];
+          tmem_ld32(tS + c * 32, s);
+          tmem_wait_ld();
+          if (part) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (c * 32 + k >= lim) s[k] = -INFINITY;
+          }
+#pragma unroll
+          for (int gq = 0; gq < 2; ++gq) {
+            const float4 f = scale[2 * c + gq];
+            float a = fmax3(s[16 * gq], s[16 * gq + 1], s[16 * gq + 2]);
+#pragma unroll
+            for (int k = 3; k < 15; k += 2) a = fmax3(a, s[16 * gq + k], s[16 * gq + k + 1]);
+            a = fmaxf(a, s[16 * gq + 15]);
+            mx = fmaxf(mx, fmaf(a, fmaxf(rf * f.x, 1.17549435e-38f), f.y));
+          }
+        }
+        const bool grow = mx > m + FEW_RESCALE;
+        const float m_new = grow ? mx : m;
+        const float z = (m_new == -INFINITY ? 0.f : m_new) - FEW_OFFSET;
+        const float alpha = grow ? (m == -INFINITY ? 0.f : exp2f(m - m_new)) : 1.f;
+        float sum = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float s[32];
+          tmem_ld32(tS + c * 32, s);
+          tmem_wait_ld();
+          if (part) {
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (c * 32 + k >= lim) s[k] = -INFINITY;
+          }
+          uint32_t pk[16];
+#pragma unroll
+          for (int gq = 0; gq < 2; ++gq) {
+            const float4 f = scale[2 * c + gq];
+            const float fs = fmaxf(rf * f.x, 1.17549435e-38f), cs = f.y - z;
+            const uint64_t f2s = f2(fs, fs), c2s = f2(cs, cs);
+            uint64_t sum2 = f2(0.f, 0.f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float2 x = f2_split(ffma2(f2(s[16 * gq + 2 * k], s[16 * gq + 2 * k + 1]), f2s, c2s));
+              const float e0 = ex2_mufu(x.x), e1 = ex2_mufu(x.y);
+              sum2 = fadd2(sum2, f2(e0, e1));
+              pk[8 * gq + k] = pack_f16(e0, e1);
+            }
+            const float2 sv = f2_split(sum2);
+            sum = fmaf(sv.x + sv.y, f.z, sum);
+          }
+          tmem_st16u(tS + c * 16, pk);
+        }
+        if (i > 0 && __any_sync(0xffffffffu, grow)) {
+          // O is stable: this S was issued behind the slot's last PV and is complete.
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            float o[32];
+            tmem_ld32(tO + c * 32, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] *= alpha;
+            tmem_st32(tO + c * 32, o);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full + 8 * t);
+        l = l * alpha + sum;
+        m = m_new;
+      }
+      tile0 += sg.n;
+      if (ok) ok = mbar_wait(o_done, seg & 1, abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      tc_fence_after();
+      if (!ok) l = 0.f;
+      const bool whole = sg.begins && sg.ends;
+      float* part = p.part + static_cast<size_t>(2 * blockIdx.x + (sg.begins ? 1 : 0)) * kv8_part_floats<KTC_QR>();
+      const int prow = (sg.two ? t * 128 : 0) + r;
+      const int hq = h * p.group + rr - tok * p.group;
+      __nv_bfloat16* orow = p.out + sg.b * p.o_sb + tok * p.o_st + hq * p.o_sh;
+      float wA = 1.f, wB = 0.f, den = l, M = m;
+      if (!sg.two) {
+        // Both slots hold the same rows: slot t finishes columns [64 t, +64).
+        float* xm = reinterpret_cast<float*>(smem + L::XCH_OFF);
+        xm[t * 256 + r] = m;
+        xm[t * 256 + 128 + r] = l;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const float m0 = xm[r], l0 = xm[128 + r], m1 = xm[256 + r], l1 = xm[384 + r];
+        M = fmaxf(m0, m1);
+        wA = m0 == -INFINITY ? 0.f : exp2f(m0 - M);
+        wB = m1 == -INFINITY ? 0.f : exp2f(m1 - M);
+        den = wA * l0 + wB * l1;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
+      const float mref = M == -INFINITY ? M : M - FEW_OFFSET;
+      const float inv = den == 0.f ? 0.f : 1.f / den;
+      const int chunks = sg.two ? 4 : 2;
+      const uint32_t src = sg.two ? tO : tmem + lane_base + 256 + t * 64;
+      const int col0 = sg.two ? 0 : t * 64;
+#pragma unroll 1
+      for (int c = 0; ok && c < chunks; ++c) {
+        float o[32];
+        tmem_ld32(src + c * 32, o);
+        tmem_wait_ld();
+        if (!sg.two) {
+          const bool has_b = sg.n > 1;      // slot B met a key tile
+          float o1[32];
+          if (has_b) {
+            tmem_ld32(src + 128 + c * 32, o1);
+            tmem_wait_ld();
+          }
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = has_b ? o[k] * wA + o1[k] * wB : o[k] * wA;
+        }
+        if (valid && whole) {
+          uint4* dst = reinterpret_cast<uint4*>(orow + col0 + c * 32);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            dst[k] = make_uint4(pack_bf16(o[8 * k] * inv, o[8 * k + 1] * inv), pack_bf16(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
+                                pack_bf16(o[8 * k + 4] * inv, o[8 * k + 5] * inv), pack_bf16(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
+        } else if (valid) {
+          float4* dst = reinterpret_cast<float4*>(part + prow * 128 + col0 + c * 32);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+        }
+      }
+      if (valid && (sg.two || t == 0)) {
+        if (!whole) {
+          part[KTC_QR * 128 + prow] = mref;
+          part[KTC_QR * 129 + prow] = den;
+        } else if (p.lse != nullptr) {
+          p.lse[(static_cast<long long>(sg.b) * p.s.tokens + tok) * (p.c.heads * p.group) + hq] = kv8_row_lse(mref, den);
+        }
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace wamb
