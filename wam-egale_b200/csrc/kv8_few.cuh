@@ -165,59 +165,112 @@ __host__ __device__ constexpr size_t kv8_part_floats() { return static_cast<size
 // Final values of a row from its merged (M, l): out = O / l, lse.
 WAMB_DEV float kv8_row_lse(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f; }
 
-// Joins the partials of items that several CTAs worked on, in CTA order: one
-// block per (CTA, eight rows), one warp per row. Block c acts for the item
-// that CTA c finished but did not begin.
-template <int QR, int TK>
+// What CTA c leaves for the merge: the item that it finished but did not
+// begin (first < 0: none), and the CTA that began it.
+struct Kv8Join {
+  int first, e, h, pad;
+};
+constexpr size_t KV8_JOIN_BYTES = 1024 * sizeof(Kv8Join);   // in front of the partials
+WAMB_DEV Kv8Join* kv8_joins(const Kv8AttnParams& p) { return reinterpret_cast<Kv8Join*>(p.part) - 1024; }
+// Called by one thread of every CTA, with the first item of its share.
+WAMB_DEV void kv8_leave_join(const Kv8AttnParams& p, const Kv8Share& sh, bool work, const Kv8Item& it) {
+  Kv8Join j{-1, 0, 0, 0};
+  if (work && it.start < sh.u0 && it.start + it.n <= sh.u1) {
+    j.first = static_cast<int>(((it.start + 1) * sh.ctas - 1) / sh.units);
+    j.e = it.e;
+    j.h = it.h;
+  }
+  kv8_joins(p)[blockIdx.x] = j;
+}
+
+// Joins the partials of items that several CTAs worked on, in CTA order:
+// block (c, y) takes rows [y RB, +RB) of the item that CTA c finished. The
+// eight warps share a row's partials (every eighth each, so that a hundred of
+// them are read in a few round trips) and add their sums in warp order.
+template <int QR, int RB>
 __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
+  __shared__ float4 sum[RB][8][32];
+  __shared__ float den[RB][8], row_max[RB];
   pdl_wait();
-  __shared__ Kv8SchedSmem sm;
-  Kv8Share sh;
-  Kv8Item it;
   const int c = blockIdx.x;
-  if (!kv8_share<QR, TK, 256>(p, c, sm, sh, it)) return;
-  if (it.start == sh.u0 || it.start + it.n > sh.u1) return;
+  const Kv8Join j = kv8_joins(p)[c];
+  if (j.first < 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = blockIdx.y * 8 + warp;
-  const int b = it.e / p.qts, qt = it.e - b * p.qts;
-  const int rr = qt * QR + row;
-  if (row >= QR || rr >= Kv8Line<QR, TK>::rows(p, b)) return;
-  const int c0 = static_cast<int>(((it.start + 1) * sh.ctas - 1) / sh.units);   // the CTA that began it
+  const int b = j.e / p.qts, qt = j.e - b * p.qts;
+  const int rows = min(QR, kv8_count(p.s, b) * p.group - qt * QR);
+  const int row0 = blockIdx.y * RB;
+  if (row0 >= rows) return;
   constexpr size_t PF = kv8_part_floats<QR>();
-  auto slot = [&](int k) { return p.part + static_cast<size_t>(2 * k + (k == c0 ? 1 : 0)) * PF; };
-  float m = -INFINITY;
-  for (int k = c0 + lane; k <= c; k += 32) m = fmaxf(m, __ldcg(slot(k) + QR * 128 + row));
+  const int cnt = c - j.first + 1;
+  auto slot = [&](int i) { return p.part + static_cast<size_t>(2 * (j.first + i) + (i == 0 ? 1 : 0)) * PF; };
+  // Few partials: a warp per row. Many: all warps on each row.
+  const int step = cnt > 8 || RB == 1 ? 8 : 1, from = step == 8 ? warp : 0;
+  for (int q = step == 8 ? 0 : warp; q < RB; q += step == 8 ? 1 : 8) {
+    const int row = row0 + q;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+    if (row < rows) {
+      float m = -INFINITY;
+      for (int i = lane; i < cnt; i += 32) m = fmaxf(m, __ldcg(slot(i) + QR * 128 + row));
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  float l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k0 = c0; k0 <= c; k0 += 32) {
-    const int k = k0 + lane;
-    float w = 0.f;
-    if (k <= c) {
-      const float mk = __ldcg(slot(k) + QR * 128 + row);
-      w = mk == -INFINITY ? 0.f : exp2f(mk - m);
-      l += w * __ldcg(slot(k) + QR * 129 + row);
-    }
-    const int cnt = min(32, c - k0 + 1);
-#pragma unroll 8
-    for (int i = 0; i < cnt; ++i) {
-      const float wi = __shfl_sync(0xffffffffu, w, i);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(slot(k0 + i) + row * 128) + lane);
-      acc.x += wi * v.x;
-      acc.y += wi * v.y;
-      acc.z += wi * v.z;
-      acc.w += wi * v.w;
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      for (int i0 = from; i0 < cnt; i0 += 8 * step) {
+        float4 v[8];
+        float mk[8], lk[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int i = i0 + u * step;
+          lk[u] = 0.f;
+          if (i < cnt) {
+            v[u] = __ldcg(reinterpret_cast<const float4*>(slot(i) + row * 128) + lane);
+            mk[u] = __ldcg(slot(i) + QR * 128 + row);
+            lk[u] = __ldcg(slot(i) + QR * 129 + row);
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          if (lk[u] == 0.f) continue;   // no key seen there
+          const float w = exp2f(mk[u] - m);
+          l += w * lk[u];
+          acc.x += w * v[u].x;
+          acc.y += w * v[u].y;
+          acc.z += w * v[u].z;
+          acc.w += w * v[u].w;
+        }
+      }
+      if (step == 1) {
+        sum[q][0][lane] = acc;
+        if (lane == 0) den[q][0] = l;
+      } else {
+        sum[q][warp][lane] = acc;
+        if (lane == 0) den[q][warp] = l;
+      }
+      // The row's maximum is the same for all its warps; the first keeps it.
+      if (lane == 0 && (step == 1 || warp == 0)) row_max[q] = m;
     }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  const int t = rr / p.group, hq = it.h * p.group + rr % p.group;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(p.out + b * p.o_sb + t * p.o_st + hq * p.o_sh + lane * 4) =
-      make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-  if (p.lse != nullptr && lane == 0)
-    p.lse[(static_cast<long long>(b) * p.s.tokens + t) * (p.c.heads * p.group) + hq] = kv8_row_lse(m, l);
+  __syncthreads();
+  const int parts = step == 8 ? 8 : 1;
+  for (int q = warp; q < RB; q += 8) {
+    const int rr = qt * QR + row0 + q;
+    if (row0 + q >= rows) continue;
+    float4 acc = sum[q][0][lane];
+    float l = den[q][0];
+    for (int i = 1; i < parts; ++i) {
+      const float4 v = sum[q][i][lane];
+      acc.x += v.x;
+      acc.y += v.y;
+      acc.z += v.z;
+      acc.w += v.w;
+      l += den[q][i];
+    }
+    const int t = rr / p.group, hq = j.h * p.group + rr - t * p.group;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<uint2*>(p.out + b * p.o_sb + t * p.o_st + hq * p.o_sh + lane * 4) =
+        make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+    if (p.lse != nullptr && lane == 0)
+      p.lse[(static_cast<long long>(b) * p.s.tokens + t) * (p.c.heads * p.group) + hq] = kv8_row_lse(row_max[q], l);
+  }
 }
 
 // --------------------------------------------------------------- few rows
@@ -371,7 +424,11 @@ __global__ void __launch_bounds__(FEW_THREADS)
   }
   Kv8Share sh;
   Kv8Item it;
-  if (!kv8_share<QR, FEW_TK, FEW_THREADS>(p, blockIdx.x, sched, sh, it)) return;
+  const bool work = kv8_share<QR, FEW_TK, FEW_THREADS>(p, blockIdx.x, sched, sh, it);
+  if constexpr (!WEIGHTS) {
+    if (threadIdx.x == 0) kv8_leave_join(p, sh, work, it);
+  }
+  if (!work) return;
   const int count = static_cast<int>(sh.u1 - sh.u0);
   const long long first_start = it.start;   // the item the share begins in
 

@@ -141,7 +141,7 @@ inline int64_t kv8_rows(const wamb_kv8_attention_args* a) {
 inline size_t kv8_attn_workspace(const wamb_kv8_attention_args* a, const DeviceInfo& di) {
   const size_t floats = kv8_is_few(kv8_rows(a)) ? kv8_few_ctas(di) * kv8_part_floats<FEW_QR>()
                                                 : di.sms * kv8_part_floats<KTC_QR>();
-  return 2 * floats * sizeof(float);
+  return KV8_JOIN_BYTES + 2 * floats * sizeof(float);
 }
 
 template <typename K>
@@ -207,11 +207,13 @@ inline int kv8_attention_impl(const wamb_kv8_attention_args* a, bool weights, cu
   DeviceInfo di;
   rc = device_info(&di);
   if (rc) return rc;
+  WAMB_REQUIRE(kv8_few_ctas(di) <= static_cast<int>(KV8_JOIN_BYTES / sizeof(Kv8Join)), WAMB_ERR_DEVICE, "kv8: %d SMs",
+               di.sms);
   if (!weights) {
     WAMB_REQUIRE(a->workspace && a->workspace_bytes >= kv8_attn_workspace(a, di), WAMB_ERR_WORKSPACE,
                  "kv8 attention: workspace of %zu bytes, needs %zu", a->workspace_bytes, kv8_attn_workspace(a, di));
     WAMB_REQUIRE(aligned16(a->workspace), WAMB_ERR_ALIGN, "kv8 attention: workspace must be 16-byte aligned");
-    p.part = static_cast<float*>(a->workspace);
+    p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + KV8_JOIN_BYTES);
   }
   const uint64_t code_rows = static_cast<uint64_t>(p.c.pages) * p.c.heads * p.c.page;
   // Boxes of the TMA loads: the few-row kernel takes 16 keys, the other whole pages.
@@ -237,7 +239,7 @@ inline int kv8_attention_impl(const wamb_kv8_attention_args* a, bool weights, cu
     rc = launch_kernel(kv8_few_kernel<false>, dim3(p.ctas), dim3(FEW_THREADS), FewSmem<false>::TOTAL, s, tmK, tmV, p, 1);
     if (rc) return rc;
     if (cap <= FEW_TK) return WAMB_OK;   // one unit per item: nothing is ever shared
-    return launch_kernel(kv8_merge_kernel<FEW_QR, FEW_TK>, dim3(p.ctas, (rows + 7) / 8), dim3(256), 0, s, p);
+    return launch_kernel(kv8_merge_kernel<FEW_QR, 1>, dim3(p.ctas, rows), dim3(256), 0, s, p);
   }
   p.ctas = di.sms;
   static bool done[64] = {};
@@ -246,7 +248,7 @@ inline int kv8_attention_impl(const wamb_kv8_attention_args* a, bool weights, cu
   rc = launch_kernel(kv8_tc_kernel, dim3(p.ctas), dim3(KTC_THREADS), KtcSmem::TOTAL, s, tmK, tmV, p);
   if (rc) return rc;
   if (cap <= KTC_TK) return WAMB_OK;
-  return launch_kernel(kv8_merge_kernel<KTC_QR, KTC_TK>, dim3(p.ctas, (std::min(rows, KTC_QR) + 7) / 8), dim3(256), 0, s, p);
+  return launch_kernel(kv8_merge_kernel<KTC_QR, 8>, dim3(p.ctas, (std::min(rows, KTC_QR) + 7) / 8), dim3(256), 0, s, p);
 }
 
 }  // namespace wamb

@@ -60,6 +60,42 @@ WAMB_DEV void sts128(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 
+WAMB_DEV float max3_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// Pairs of every eight whose 2^x runs on the FMA pipe: the MUFU's 16 a cycle
+// alone would take 2048 cycles for 256 x 128 scores, as long as the products.
+constexpr int KTC_POLY = 2;
+
+// 2^x for a pair: x clamped to >= -125, x = n + f with |f| <= 1/2 by the
+// 1.5 * 2^23 shifter, 2^f by the polynomial of degree 5 with the smallest
+// largest relative error (Remez exchange; 1.6e-7 with fp32 coefficients,
+// recomputed by tests/test_host_exp2_poly5.py), n added to the exponent field.
+constexpr float KTC_C0 = 1.0000001192092896f;
+constexpr float KTC_C1 = 0.6931469440460205f;
+constexpr float KTC_C2 = 0.24022120237350464f;
+constexpr float KTC_C3 = 0.05550713092088699f;
+constexpr float KTC_C4 = 0.009675540961325169f;
+constexpr float KTC_C5 = 0.0013276472454890609f;
+WAMB_DEV uint64_t ex2_poly5(uint64_t x2) {
+  const float2 xv = f2_split(x2);
+  const uint64_t x = f2(fmaxf(xv.x, -125.f), fmaxf(xv.y, -125.f));
+  const uint64_t shifter = f2(12582912.f, 12582912.f);
+  const uint64_t t = fadd2(x, shifter);
+  const uint64_t f = fsub2(x, fsub2(t, shifter));
+  uint64_t p = ffma2(f, f2(KTC_C5, KTC_C5), f2(KTC_C4, KTC_C4));
+  p = ffma2(p, f, f2(KTC_C3, KTC_C3));
+  p = ffma2(p, f, f2(KTC_C2, KTC_C2));
+  p = ffma2(p, f, f2(KTC_C1, KTC_C1));
+  p = ffma2(p, f, f2(KTC_C0, KTC_C0));
+  const float2 pv = f2_split(p), tv = f2_split(t);
+  return f2(__int_as_float(__float_as_int(pv.x) + (__float_as_int(tv.x) << 23)),
+            __int_as_float(__float_as_int(pv.y) + (__float_as_int(tv.y) << 23)));
+}
+
 // Row `row` of a query tile into its two E4M3 pieces at hi / lo (swizzled
 // 128-byte rows, row r of the tile); returns 2^n. All 128 values by one thread.
 template <bool STORE>
@@ -158,7 +194,9 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
   pdl_wait();
   Kv8Share sh;
   KtcWalk walk;
-  if (!kv8_share<KTC_QR, KTC_TK, KTC_THREADS>(p, blockIdx.x, sched, sh, walk.it)) return;
+  const bool work = kv8_share<KTC_QR, KTC_TK, KTC_THREADS>(p, blockIdx.x, sched, sh, walk.it);
+  if (threadIdx.x == 0) kv8_leave_join(p, sh, work, walk.it);
+  if (!work) return;
   walk.u = sh.u0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < KTC_KS; ++i) { mbar_init(k_full + 8 * i, 1); mbar_init(k_empty + 8 * i, 1); }
@@ -180,7 +218,10 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-
+  // The softmax warps hold a whole row of 128 scores: 256 threads x 208 and
+  // 128 x 80 registers, within the launch's 384 x 168.
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
   if (warp == 8) {
     // ---------------------------------------------------------- producer
     // Lane (to, gi) looks after keys [16 gi, +16) of tile `to` of a batch of four.
@@ -191,31 +232,35 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
     for (; go && !walk.done(sh); walk.next(p, sh)) {
       const KtcSeg sg(p, sh, walk);
       const int h = walk.it.h;
-      struct Ahead { int row; float ks, lv, iv; bool live; };
-      auto load = [&](int j) {
-        Ahead a{0, 1.f, 0.f, 1.f, false};
+      // Page ids are read two batches ahead, scales one, so that no load is
+      // waited for.
+      struct Ahead { int row; float ks, vs; };   // row < 0: no keys
+      auto page_of = [&](int j) {
         const int key = (sg.j0 + j + to) * KTC_TK + gi * 16;
-        if (j + to < sg.n && key < sg.vis) {
-          int pid = kv8_page(p.s.table, p.s.width, p.c, sg.b, key >> p.c.page_log2);
-          if (pid < 0) pid = 0;   // reported
+        if (j + to >= sg.n || key >= sg.vis) return -1;
+        return max(0, kv8_page(p.s.table, p.s.width, p.c, sg.b, key >> p.c.page_log2));   // a bad id is reported
+      };
+      auto load = [&](int j, int pid) {
+        Ahead a{-1, 1.f, 1.f};
+        if (pid >= 0) {
+          const int key = (sg.j0 + j + to) * KTC_TK + gi * 16;
           const long long blk = static_cast<long long>(pid) * p.c.heads + h;
           a.row = static_cast<int>((blk << p.c.page_log2) + (key & (p.c.page - 1)));
           a.ks = __ldg(p.c.k_scale + blk);
-          const float vs = __ldg(p.c.v_scale + blk);
-          a.lv = log2f(vs);
-          a.iv = 1.f / vs;
-          a.live = true;
+          a.vs = __ldg(p.c.v_scale + blk);
         }
         return a;
       };
-      Ahead now = load(0);
+      Ahead now = load(0, page_of(0));
+      int pid = page_of(4);
       for (int jb = 0; go && jb < sg.n; jb += 4) {
-        const Ahead next = load(jb + 4);
+        const Ahead next = load(jb + 4, pid);
+        pid = page_of(jb + 8);
         for (int i = 0; i < 4 && jb + i < sg.n; ++i, ++tiles) {
           const int sc = tiles % KTC_SCS;
           if (to == i)
-            *reinterpret_cast<float4*>(smem + L::SC_OFF + (sc * 8 + gi) * 16) = make_float4(now.ks, now.lv, now.iv, 0.f);
-          const bool lead = to == i && now.live && gi % box_groups == 0;
+            *reinterpret_cast<float4*>(smem + L::SC_OFF + (sc * 8 + gi) * 16) = make_float4(now.ks, log2f(now.vs), 1.f / now.vs, 0.f);
+          const bool lead = to == i && now.row >= 0 && gi % box_groups == 0;
           const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, lead)) * (p.c.page * 128);
           __syncwarp();
           if (lane == 0) mbar_arrive(sc_full + 8 * sc);
@@ -294,7 +339,7 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
       mbar_wait_teardown(drain, 0);
     }
     __syncwarp();
-  } else if (warp >= 10) {
+  } else {
     // --------------------------------------------- V codes -> f16 tiles
     const int ct = threadIdx.x - 320;    // 0..63
     int tiles = 0;
@@ -333,8 +378,10 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
         }
       }
     }
+  }
   } else {
     // ------------------------------------------------ softmax / epilogue
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     const int t = warp >> 2;          // TMEM slot
     const int r = (warp & 3) * 32 + lane;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -375,42 +422,43 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
         const float4* scale = reinterpret_cast<const float4*>(smem + L::SC_OFF) + sc * 8;
         const int lim = seen - (sg.j0 + j) * KTC_TK;    // keys of this tile that the row sees
         const bool part = __any_sync(0xffffffffu, lim < KTC_TK);
-        float mx = -INFINITY;
+        float s[128];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          float s[32];
-          tmem_ld32(tS + c * 32, s);
-          tmem_wait_ld();
-          if (part) {
+          float x[32];
+          tmem_ld32(tS + c * 32, x);
 #pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (c * 32 + k >= lim) s[k] = -INFINITY;
-          }
-#pragma unroll
-          for (int gq = 0; gq < 2; ++gq) {
-            const float4 f = scale[2 * c + gq];
-            float a = fmax3(s[16 * gq], s[16 * gq + 1], s[16 * gq + 2]);
-#pragma unroll
-            for (int k = 3; k < 15; k += 2) a = fmax3(a, s[16 * gq + k], s[16 * gq + k + 1]);
-            a = fmaxf(a, s[16 * gq + 15]);
-            mx = fmaxf(mx, fmaf(a, fmaxf(rf * f.x, 1.17549435e-38f), f.y));
-          }
+          for (int k = 0; k < 32; ++k) s[c * 32 + k] = x[k];
         }
-        const bool grow = mx > m + FEW_RESCALE;
+        tmem_wait_ld();
+        if (part) {
+#pragma unroll
+          for (int k = 0; k < 128; ++k)
+            if (k >= lim) s[k] = -INFINITY;
+        }
+        // Maximum of y over the 8 groups of 16 keys; NaN wins (it makes the row NaN).
+        float mx = -INFINITY;
+#pragma unroll
+        for (int g8 = 0; g8 < 8; ++g8) {
+          const float4 f = scale[g8];
+          const float* sg8 = s + 16 * g8;
+          float a = max3_nan(sg8[0], sg8[1], sg8[2]), b = max3_nan(sg8[3], sg8[4], sg8[5]);
+          a = max3_nan(a, sg8[6], sg8[7]);
+          b = max3_nan(b, sg8[8], sg8[9]);
+          a = max3_nan(a, sg8[10], sg8[11]);
+          b = max3_nan(b, sg8[12], sg8[13]);
+          a = max3_nan(a, sg8[14], sg8[15]);
+          a = max3_nan(a, b, b);
+          a = fmaf(a, fmaxf(rf * f.x, 1.17549435e-38f), f.y);
+          mx = max3_nan(mx, a, a);
+        }
+        const bool grow = !(mx <= m + FEW_RESCALE);
         const float m_new = grow ? mx : m;
         const float z = (m_new == -INFINITY ? 0.f : m_new) - FEW_OFFSET;
         const float alpha = grow ? (m == -INFINITY ? 0.f : exp2f(m - m_new)) : 1.f;
         float sum = 0.f;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          float s[32];
-          tmem_ld32(tS + c * 32, s);
-          tmem_wait_ld();
-          if (part) {
-#pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (c * 32 + k >= lim) s[k] = -INFINITY;
-          }
           uint32_t pk[16];
 #pragma unroll
           for (int gq = 0; gq < 2; ++gq) {
@@ -420,16 +468,25 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
             uint64_t sum2 = f2(0.f, 0.f);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-              const float2 x = f2_split(ffma2(f2(s[16 * gq + 2 * k], s[16 * gq + 2 * k + 1]), f2s, c2s));
-              const float e0 = ex2_mufu(x.x), e1 = ex2_mufu(x.y);
-              sum2 = fadd2(sum2, f2(e0, e1));
-              pk[8 * gq + k] = pack_f16(e0, e1);
+              const uint64_t x2 = ffma2(f2(s[32 * c + 16 * gq + 2 * k], s[32 * c + 16 * gq + 2 * k + 1]), f2s, c2s);
+              float2 e;
+              if (k < 8 - KTC_POLY) {
+                const float2 x = f2_split(x2);
+                e = make_float2(ex2_mufu(x.x), ex2_mufu(x.y));
+                sum2 = fadd2(sum2, f2(e.x, e.y));
+              } else {
+                const uint64_t e2 = ex2_poly5(x2);
+                sum2 = fadd2(sum2, e2);
+                e = f2_split(e2);
+              }
+              pk[8 * gq + k] = pack_f16(e.x, e.y);
             }
             const float2 sv = f2_split(sum2);
             sum = fmaf(sv.x + sv.y, f.z, sum);
           }
           tmem_st16u(tS + c * 16, pk);
         }
+        if (m_new == -INFINITY) sum = 0.f;   // no key seen yet (the polynomial's 2^-125 are no weights)
         if (i > 0 && __any_sync(0xffffffffu, grow)) {
           // O is stable: this S was issued behind the slot's last PV and is complete.
 #pragma unroll 1
