@@ -532,7 +532,7 @@ WAMB_API int wamb_kv8_write(const wamb_kv8_write_args* args, void* stream);
  * left as they were. What lies past lens[b] in a page counts for nothing,
  * but a NaN that was written as V reaches every row of the call that is
  * computed beside its key. workspace: wamb_kv8_attention_workspace_bytes()
- * bytes of scratch, any contents, not shared with a call that may run at the
+ * bytes of scratch (256-byte aligned, any contents), not shared with a call that may run at the
  * same time. Results do not depend on timing. */
 typedef struct wamb_kv8_attention_args {
   wamb_kv8_cache cache;

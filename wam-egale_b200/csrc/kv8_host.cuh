@@ -137,11 +137,39 @@ inline bool kv8_is_few(int64_t rows) { return rows <= FEW_QR; }
 inline int64_t kv8_rows(const wamb_kv8_attention_args* a) {
   return a->cache.heads > 0 ? static_cast<int64_t>(a->seqs.tokens) * (a->q_heads / a->cache.heads) : 0;
 }
-// Two partials for each CTA.
+// The split queries of the tensor-core kernels: rows of 256 bytes, a factor
+// and (weights) a log-sum-exp each.
+struct Kv8SplitQ {
+  int rows_pad = 0;
+  long long total = 0;
+  size_t bytes(bool weights) const { return static_cast<size_t>(total) * (256 + (weights ? 8 : 4)); }
+};
+inline Kv8SplitQ kv8_split_q(int64_t batch, int64_t heads, int64_t rows) {
+  Kv8SplitQ q;
+  q.rows_pad = static_cast<int>((rows + 127) / 128 * 128);
+  q.total = batch * heads * q.rows_pad;
+  return q;
+}
+// Joins and two partials for each CTA, then the split queries.
+inline size_t kv8_part_bytes(bool few, const DeviceInfo& di) {
+  const size_t floats = few ? kv8_few_ctas(di) * kv8_part_floats<FEW_QR>() : di.sms * kv8_part_floats<KTC_QR>();
+  return (KV8_JOIN_BYTES + 2 * floats * sizeof(float) + 255) / 256 * 256;
+}
 inline size_t kv8_attn_workspace(const wamb_kv8_attention_args* a, const DeviceInfo& di) {
-  const size_t floats = kv8_is_few(kv8_rows(a)) ? kv8_few_ctas(di) * kv8_part_floats<FEW_QR>()
-                                                : di.sms * kv8_part_floats<KTC_QR>();
-  return KV8_JOIN_BYTES + 2 * floats * sizeof(float);
+  const int64_t rows = kv8_rows(a);
+  const bool few = kv8_is_few(rows);
+  return kv8_part_bytes(few, di) + (few ? 0 : kv8_split_q(a->seqs.batch, a->cache.heads, rows).bytes(false));
+}
+// Splits the queries into `at`; returns the map of its rows and the factors.
+inline int kv8_split_launch(const Kv8AttnParams& p, const Kv8SplitQ& sq, uint8_t* at, bool weights, CUtensorMap* map,
+                            float** factor, float** lse2, cudaStream_t s) {
+  WAMB_REQUIRE(sq.total <= INT32_MAX, WAMB_ERR_SHAPE, "kv8: %lld query rows", sq.total);
+  *factor = reinterpret_cast<float*>(at + sq.total * 256);
+  *lse2 = weights ? *factor + sq.total : nullptr;
+  int rc = make_tmap_2d(map, at, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, sq.total, 256, 256, 128, 128);
+  if (rc) return rc;
+  return launch_kernel(kv8_split_q_kernel, dim3(static_cast<unsigned>((sq.total + 31) / 32)), dim3(256), 0, s, p,
+                       sq.rows_pad, sq.total, at, *factor, *lse2);
 }
 
 template <typename K>
@@ -212,7 +240,8 @@ inline int kv8_attention_impl(const wamb_kv8_attention_args* a, bool weights, cu
   if (!weights) {
     WAMB_REQUIRE(a->workspace && a->workspace_bytes >= kv8_attn_workspace(a, di), WAMB_ERR_WORKSPACE,
                  "kv8 attention: workspace of %zu bytes, needs %zu", a->workspace_bytes, kv8_attn_workspace(a, di));
-    WAMB_REQUIRE(aligned16(a->workspace), WAMB_ERR_ALIGN, "kv8 attention: workspace must be 16-byte aligned");
+    WAMB_REQUIRE(reinterpret_cast<uintptr_t>(a->workspace) % 256 == 0, WAMB_ERR_ALIGN,
+                 "kv8 attention: workspace must be 256-byte aligned");
     p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + KV8_JOIN_BYTES);
   }
   const uint64_t code_rows = static_cast<uint64_t>(p.c.pages) * p.c.heads * p.c.page;
@@ -242,10 +271,17 @@ inline int kv8_attention_impl(const wamb_kv8_attention_args* a, bool weights, cu
     return launch_kernel(kv8_merge_kernel<FEW_QR, 1>, dim3(p.ctas, rows), dim3(256), 0, s, p);
   }
   p.ctas = di.sms;
+  CUtensorMap tmQ;
+  float *factor = nullptr, *unused = nullptr;
+  const Kv8SplitQ sq = kv8_split_q(p.s.batch, p.c.heads, rows);
+  rc = kv8_split_launch(p, sq, static_cast<uint8_t*>(a->workspace) + kv8_part_bytes(false, di), false, &tmQ, &factor,
+                        &unused, s);
+  if (rc) return rc;
   static bool done[64] = {};
   rc = kv8_smem_once(kv8_tc_kernel, KtcSmem::TOTAL, done);
   if (rc) return rc;
-  rc = launch_kernel(kv8_tc_kernel, dim3(p.ctas), dim3(KTC_THREADS), KtcSmem::TOTAL, s, tmK, tmV, p);
+  rc = launch_kernel(kv8_tc_kernel, dim3(p.ctas), dim3(KTC_THREADS), KtcSmem::TOTAL, s, tmK, tmV, tmQ,
+                     static_cast<const float*>(factor), sq.rows_pad, p);
   if (rc) return rc;
   if (cap <= KTC_TK) return WAMB_OK;
   return launch_kernel(kv8_merge_kernel<KTC_QR, 8>, dim3(p.ctas, (std::min(rows, KTC_QR) + 7) / 8), dim3(256), 0, s, p);

@@ -16,9 +16,10 @@
 //
 // One CTA per SM, 384 threads:
 //   warps 0..7   softmax, one thread per query row: warps 0-3 on TMEM slot A,
-//                warps 4-7 on slot B. They also split the queries into smem.
+//                warps 4-7 on slot B
 //   warp 8       producer: page ids and scales (read four tiles ahead), TMA
-//                of K and V codes, the scales of each 16 keys to a ring
+//                of the queries' pieces (split once by kv8_split_q_kernel)
+//                and of K and V codes, the scales of each 16 keys to a ring
 //   warp 9       its lane 0 issues the MMAs
 //   warps 10, 11 V codes -> f16
 // With more than 128 rows, slot A and slot B hold the tile's two halves and
@@ -30,6 +31,7 @@
 #pragma once
 #include "attention.cuh"
 #include "kv8_few.cuh"
+#include <type_traits>
 
 namespace wamb {
 
@@ -42,10 +44,10 @@ struct KtcSmem {
   static constexpr uint32_t K_OFF = Q_OFF + 4 * KTC_TILE8;
   static constexpr uint32_t V8_OFF = K_OFF + KTC_KS * KTC_TILE8;
   static constexpr uint32_t V16_OFF = V8_OFF + KTC_V8S * KTC_TILE8;
-  static constexpr uint32_t SC_OFF = V16_OFF + KTC_V16S * 2 * KTC_TILE8;     // [8 tiles][8 groups of 16 keys] float4
+  static constexpr uint32_t SC_OFF = V16_OFF + KTC_V16S * 2 * KTC_TILE8;     // [8 tiles] ks, log2 vs, 1 / vs of 8 groups of 16 keys
   static constexpr uint32_t XCH_OFF = SC_OFF + KTC_SCS * 8 * 16;             // m, l of both slots
   static constexpr uint32_t BAR_OFF = XCH_OFF + 2 * 2 * 128 * 4;
-  static constexpr uint32_t NBARS = 2 * KTC_KS + 2 * KTC_V8S + 2 * KTC_V16S + 2 + 2 + 3 + KTC_SCS;
+  static constexpr uint32_t NBARS = 2 * KTC_KS + 2 * KTC_V8S + 2 * KTC_V16S + 2 + 2 + 4 + KTC_SCS;
   static constexpr uint32_t SCHED_OFF = BAR_OFF + NBARS * 8;
   static constexpr uint32_t TOTAL = 1024 + SCHED_OFF + sizeof(Kv8SchedSmem) + 16;
   static_assert(TOTAL <= 232448, "shared memory exceeds 227 KB");
@@ -54,6 +56,48 @@ struct KtcSmem {
 // kind::f16 instruction descriptor with f16 operands, B MN-major.
 __host__ __device__ constexpr uint32_t idesc_f16_mn(int M, int N) {
   return (1u << 4) | (1u << 16) | (static_cast<uint32_t>(N >> 3) << 17) | (static_cast<uint32_t>(M >> 4) << 24);
+}
+
+// Low and high words of the swizzled operand descriptors (sw128_desc): the low
+// one moves with the address, the high one is a constant, so that an MMA costs
+// its issuing thread one addition.
+constexpr uint32_t KTC_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
+WAMB_DEV uint32_t ktc_desc_lo(uint32_t addr, uint32_t lbo) { return (addr >> 4) | ((lbo >> 4) << 16); }
+
+// S [128 rows][128 keys] = (hi + lo) K^T: 4 x 32 dims of each piece.
+WAMB_DEV void ktc_issue_s(uint32_t d, uint32_t q, uint32_t k) {
+  constexpr uint32_t IDESC = idesc_e4m3(128, 128);
+  const uint32_t qd = ktc_desc_lo(q, 16), kd = ktc_desc_lo(k, 16);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+        "r"(qd + (i >> 2) * (KTC_TILE8 >> 4) + (i & 3) * 2), "r"(kd + (i & 3) * 2), "n"(KTC_DESC_HI), "n"(IDESC),
+        "r"(i > 0 ? 1u : 0u)
+        : "memory");
+}
+// O [128 rows][128 dims] (+)= P V: P in TMEM, 8 x 16 keys (rows of V past the
+// live keys are zero, and so is P).
+WAMB_DEV void ktc_issue_pv(uint32_t d, uint32_t pt, uint32_t v, bool accumulate) {
+  constexpr uint32_t IDESC = idesc_f16_mn(128, 128);
+  const uint32_t vd = ktc_desc_lo(v, KTC_TILE8), acc = accumulate;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+        "mov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d),
+        "r"(pt + 8 * i), "r"(vd + i * (2048 >> 4)), "n"(KTC_DESC_HI), "n"(IDESC), "r"(i > 0 ? 1u : acc)
+        : "memory");
+}
+
+// One lane of the converged warp, always the same.
+WAMB_DEV bool elect_one() {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+  return ok != 0;
 }
 
 WAMB_DEV void sts128(uint32_t a, uint4 v) {
@@ -68,7 +112,7 @@ WAMB_DEV float max3_nan(float a, float b, float c) {
 
 // Pairs of every eight whose 2^x runs on the FMA pipe: the MUFU's 16 a cycle
 // alone would take 2048 cycles for 256 x 128 scores, as long as the products.
-constexpr int KTC_POLY = 2;
+constexpr int KTC_POLY = 0;
 
 // 2^x for a pair: x clamped to >= -125, x = n + f with |f| <= 1/2 by the
 // 1.5 * 2^23 shifter, 2^f by the polynomial of degree 5 with the smallest
@@ -96,51 +140,66 @@ WAMB_DEV uint64_t ex2_poly5(uint64_t x2) {
             __int_as_float(__float_as_int(pv.y) + (__float_as_int(tv.y) << 23)));
 }
 
-// Row `row` of a query tile into its two E4M3 pieces at hi / lo (swizzled
-// 128-byte rows, row r of the tile); returns 2^n. All 128 values by one thread.
-template <bool STORE>
-WAMB_DEV float ktc_split_q(const __nv_bfloat16* src, bool ok, uint32_t hi, uint32_t lo, int r) {
-  uint4 w[16];
+// The queries in two E4M3 pieces, for the tensor-core kernels: row
+// (b * heads + h) * rows_pad + r of q8 [., 256] holds hi (128 codes) and lo of
+// row r of (sequence b, cached head h), rf its factor 2^n * scale * log2(e);
+// rows past the sequence's are zeros. With lse2 (weights): lse2 = lse *
+// log2(e), +inf for rows that add nothing. A warp per row, four rows at once;
+// bound by memory (512 B a row) or by the launch.
+__global__ void __launch_bounds__(256) kv8_split_q_kernel(const Kv8AttnParams p, const int rows_pad, const long long total,
+                                                          uint8_t* q8, float* rf, float* lse2) {
+  pdl_wait();
+  constexpr int AT_ONCE = 4;
+  const int lane = threadIdx.x & 31;
+  const long long first = (static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5)) * AT_ONCE;
+  uint2 w[AT_ONCE];
+  bool ok[AT_ONCE];
+  float z[AT_ONCE];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) w[i] = ok ? __ldg(reinterpret_cast<const uint4*>(src) + i) : make_uint4(0, 0, 0, 0);
-  float amax = 0.f;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 v = unpack_bf16(u[k]);
-      amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
+  for (int i = 0; i < AT_ONCE; ++i) {
+    const long long row = first + i;
+    w[i] = make_uint2(0, 0);
+    z[i] = -INFINITY;
+    ok[i] = false;
+    if (row < total) {
+      const int bh = static_cast<int>(row / rows_pad), r = static_cast<int>(row - static_cast<long long>(bh) * rows_pad);
+      const int b = bh / p.c.heads, h = bh - b * p.c.heads;
+      const int t = r / p.group, hq = h * p.group + r - t * p.group;
+      ok[i] = t < kv8_count(p.s, b);
+      if (ok[i]) {
+        w[i] = __ldg(reinterpret_cast<const uint2*>(p.q + b * p.q_sb + t * p.q_st + hq * p.q_sh) + lane);
+        if (lse2 != nullptr)
+          z[i] = __ldg(p.lse_in + (static_cast<long long>(b) * p.s.tokens + t) * (p.c.heads * p.group) + hq);
+      }
     }
   }
-  // Scale exponent as for a cache block, over fp32's whole range.
-  const int bits = __float_as_int(fminf(amax, 3.402823466e38f));
-  const int n = max(-118, min(119, (bits >> 23) - 135 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0)));
-  if constexpr (STORE) {
+#pragma unroll
+  for (int i = 0; i < AT_ONCE; ++i) {
+    const long long row = first + i;
+    if (row >= total) continue;   // the same for the whole warp
+    const float2 a = unpack_bf16(w[i].x), b = unpack_bf16(w[i].y);
+    float amax = fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y)));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    // Scale exponent as for a cache block, over fp32's whole range.
+    const int bits = __float_as_int(fminf(amax, 3.402823466e38f));
+    const int n = max(-118, min(119, (bits >> 23) - 135 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0)));
     // An infinite query makes its row NaN, as the formula does (a saturated one would not).
     const float up = amax <= 3.402823466e38f ? pow2f_exact(-n) : __int_as_float(0x7fffffff);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {   // 16 values: one swizzled piece
-      uint32_t h[4], l[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint4 q = w[2 * i + (k >> 1)];
-        const float2 a = unpack_bf16((k & 1) ? q.z : q.x), b = unpack_bf16((k & 1) ? q.w : q.y);
-        const float x[4] = {a.x * up, a.y * up, b.x * up, b.y * up};
-        const uint32_t h0 = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t h1 = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
-        const float2 f0 = e4m3x2_to_float2(h0), f1 = e4m3x2_to_float2(h1);
-        const uint32_t l0 = __nv_cvt_float2_to_fp8x2(make_float2(x[0] - f0.x, x[1] - f0.y), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t l1 = __nv_cvt_float2_to_fp8x2(make_float2(x[2] - f1.x, x[3] - f1.y), __NV_SATFINITE, __NV_E4M3);
-        h[k] = h0 | (h1 << 16);
-        l[k] = l0 | (l1 << 16);
-      }
-      const uint32_t at = r * 128 + ((i ^ (r & 7)) << 4);
-      sts128(hi + at, make_uint4(h[0], h[1], h[2], h[3]));
-      sts128(lo + at, make_uint4(l[0], l[1], l[2], l[3]));
+    const float x[4] = {a.x * up, a.y * up, b.x * up, b.y * up};
+    const uint32_t h0 = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t h1 = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
+    const float2 f0 = e4m3x2_to_float2(h0), f1 = e4m3x2_to_float2(h1);
+    const uint32_t l0 = __nv_cvt_float2_to_fp8x2(make_float2(x[0] - f0.x, x[1] - f0.y), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t l1 = __nv_cvt_float2_to_fp8x2(make_float2(x[2] - f1.x, x[3] - f1.y), __NV_SATFINITE, __NV_E4M3);
+    uint32_t* dst = reinterpret_cast<uint32_t*>(q8 + row * 256) + lane;
+    dst[0] = h0 | (h1 << 16);
+    dst[32] = l0 | (l1 << 16);
+    if (lane == 0) {
+      rf[row] = pow2f_exact(n) * p.scale_log2;
+      if (lse2 != nullptr) lse2[row] = !ok[i] || z[i] == -INFINITY ? INFINITY : z[i] * 1.4426950408889634f;
     }
   }
-  return pow2f_exact(n);
 }
 
 // One CTA's walk over the segments of its share.
@@ -175,7 +234,7 @@ struct KtcSeg {
 
 __global__ void __launch_bounds__(KTC_THREADS, 1)
     kv8_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                  const Kv8AttnParams p) {
+                  const __grid_constant__ CUtensorMap tmQ, const float* q_factor, const int rows_pad, const Kv8AttnParams p) {
   using L = KtcSmem;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -185,11 +244,11 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
   auto bars = [&](int n) { const uint32_t b = bar; bar += 8 * n; return b; };
   const uint32_t k_full = bars(KTC_KS), k_empty = bars(KTC_KS), v8_full = bars(KTC_V8S), v8_empty = bars(KTC_V8S),
                  v16_full = bars(KTC_V16S), v16_empty = bars(KTC_V16S), s_full = bars(2), p_full = bars(2),
-                 q_full = bars(1), o_done = bars(1), drain = bars(1), sc_full = bars(KTC_SCS);
+                 q_full = bars(1), o_done = bars(1), o_free = bars(1), drain = bars(1), sc_full = bars(KTC_SCS);
   Kv8SchedSmem& sched = *reinterpret_cast<Kv8SchedSmem*>(smem + L::SCHED_OFF);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::SCHED_OFF + sizeof(Kv8SchedSmem));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // warp: uniform
 
   pdl_wait();
   Kv8Share sh;
@@ -203,7 +262,8 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
     for (int i = 0; i < KTC_V8S; ++i) { mbar_init(v8_full + 8 * i, 1); mbar_init(v8_empty + 8 * i, 2); }
     for (int i = 0; i < KTC_V16S; ++i) { mbar_init(v16_full + 8 * i, 2); mbar_init(v16_empty + 8 * i, 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(s_full + 8 * i, 1); mbar_init(p_full + 8 * i, 4); }
-    mbar_init(q_full, 8);
+    mbar_init(q_full, 1);
+    mbar_init(o_free, 8);
     mbar_init(o_done, 1);
     mbar_init(drain, 1);
     for (int i = 0; i < KTC_SCS; ++i) mbar_init(sc_full + 8 * i, 1);
@@ -227,11 +287,25 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
     // Lane (to, gi) looks after keys [16 gi, +16) of tile `to` of a batch of four.
     const int to = lane >> 3, gi = lane & 7;
     const int box_groups = p.c.page >> 4;   // 16-key groups of one page
-    int tiles = 0;                          // key tiles so far
+    int tiles = 0, queries = 0;             // key tiles and query tiles so far
     bool go = true;
-    for (; go && !walk.done(sh); walk.next(p, sh)) {
+    for (int seg = 0; go && !walk.done(sh); walk.next(p, sh), ++seg) {
       const KtcSeg sg(p, sh, walk);
       const int h = walk.it.h;
+      // The queries' pieces, once the last segment's products have read theirs.
+      if (seg > 0) go = __all_sync(0xffffffffu, mbar_wait(o_done, (seg - 1) & 1, abort_flag));
+      if (!go) break;
+      if (lane == 0) {
+        const int row = (sg.b * p.c.heads + h) * rows_pad + sg.qt * KTC_QR;
+        mbar_arrive_expect_tx(q_full, (sg.two ? 4 : 2) * KTC_TILE8);
+        tma_load_2d(sQ, &tmQ, q_full, 0, row);
+        tma_load_2d(sQ + KTC_TILE8, &tmQ, q_full, 128, row);
+        if (sg.two) {
+          tma_load_2d(sQ + 2 * KTC_TILE8, &tmQ, q_full, 0, row + 128);
+          tma_load_2d(sQ + 3 * KTC_TILE8, &tmQ, q_full, 128, row + 128);
+        }
+      }
+      ++queries;
       // Page ids are read two batches ahead, scales one, so that no load is
       // waited for.
       struct Ahead { int row; float ks, vs; };   // row < 0: no keys
@@ -258,8 +332,12 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
         pid = page_of(jb + 8);
         for (int i = 0; i < 4 && jb + i < sg.n; ++i, ++tiles) {
           const int sc = tiles % KTC_SCS;
-          if (to == i)
-            *reinterpret_cast<float4*>(smem + L::SC_OFF + (sc * 8 + gi) * 16) = make_float4(now.ks, log2f(now.vs), 1.f / now.vs, 0.f);
+          if (to == i) {
+            float* at = reinterpret_cast<float*>(smem + L::SC_OFF) + sc * 32 + gi;
+            at[0] = now.ks;
+            at[8] = log2f(now.vs);
+            at[16] = 1.f / now.vs;
+          }
           const bool lead = to == i && now.row >= 0 && gi % box_groups == 0;
           const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, lead)) * (p.c.page * 128);
           __syncwarp();
@@ -283,58 +361,66 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
     }
     // Loads still in flight must land before the CTA exits.
     if (lane == 0 && go) {
+      if (queries > 0) mbar_wait_teardown(q_full, (queries - 1) & 1);
       for (int t = max(0, tiles - KTC_KS); t < tiles; ++t) mbar_wait_teardown(k_full + 8 * (t % KTC_KS), (t / KTC_KS) & 1);
       for (int t = max(0, tiles - KTC_V8S); t < tiles; ++t) mbar_wait_teardown(v8_full + 8 * (t % KTC_V8S), (t / KTC_V8S) & 1);
     }
     __syncwarp();
   } else if (warp == 9) {
-    if (lane == 0) {
-      // ------------------------------------------------------- MMA issuer
-      constexpr uint32_t IDESC_S = idesc_e4m3(128, 128);
-      constexpr uint32_t IDESC_O = idesc_f16_mn(128, 128);
-      int tile0 = 0;                       // key tiles of earlier segments
-      int pcount[2] = {0, 0};              // P tiles taken from each slot
-      bool ok = true;
-      for (int seg = 0; ok && !walk.done(sh); walk.next(p, sh), ++seg) {
-        const KtcSeg sg(p, sh, walk);
-        const int steps = sg.two ? 2 * sg.n : sg.n;
-        auto issue_s = [&](int s) {
-          const int t = s & 1, j = sg.two ? s >> 1 : s, k = tile0 + j;
-          const uint32_t kb = sK + (k % KTC_KS) * KTC_TILE8;
-          const uint32_t qb = sQ + (sg.two ? t * 2 * KTC_TILE8 : 0);
-          if (!mbar_wait(k_full + 8 * (k % KTC_KS), (k / KTC_KS) & 1, abort_flag)) return false;
+    // --------------------------------------------------------- MMA issuer
+    // The whole warp walks the loop on values that are the same in every lane
+    // (so that descriptors are computed in uniform registers) and one lane
+    // issues: a lane alone in a divergent branch took ~110 cycles an MMA.
+    const bool issuer = elect_one();
+    uint32_t kq = 0, kpar = 0;      // K ring: slot and phase of the next score tile
+    uint32_t vq = 0, vpar = 0;      // f16 V ring, likewise
+    uint32_t ppar = 0;              // bit t: phase of slot t's next P tile
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    bool ok = true;
+    for (uint32_t seg = 0; ok && !walk.done(sh); walk.next(p, sh), ++seg) {
+      const KtcSeg sg(p, sh, walk);
+      const bool two = __shfl_sync(0xffffffffu, sg.two, 0);
+      const int tiles = __shfl_sync(0xffffffffu, sg.n, 0);
+      const int steps = two ? 2 * tiles : tiles;
+      auto wait = [&](uint32_t b, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag)) != 0; };
+      ok = wait(q_full, seg & 1);
+      // Step s: PV of its tile, then the scores of step s + 2 (slot `t` = s & 1).
+      auto step = [&](auto slot, int s) {
+        constexpr uint32_t t = decltype(slot)::value;
+        const bool last = t == 1 || !two;     // of the key tile
+        const bool first = t == 0 || !two;
+        if (s >= 0) {
+          if (s == 0 && seg > 0) ok = wait(o_free, (seg - 1) & 1);   // the last segment's output has left TMEM
+          if (first) ok = ok && wait(v16_full + 8 * vq, vpar);
+          ok = ok && wait(p_full + 8 * t, (ppar >> t) & 1);
+          if (!ok) return;
+          ppar ^= 1u << t;
           tc_fence_after();
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk)   // hi piece, then lo piece: 4 x 32 dims each
-            umma_e4m3(tmem + t * 128, sw128_desc(qb + (kk >> 2) * KTC_TILE8 + (kk & 3) * 32, 16, 1024),
-                      sw128_desc(kb + (kk & 3) * 32, 16, 1024), IDESC_S, kk > 0);
-          umma_commit(s_full + 8 * t);
-          if (!sg.two || t == 1) umma_commit(k_empty + 8 * (k % KTC_KS));
-          return true;
-        };
-        ok = mbar_wait(q_full, seg & 1, abort_flag);
-        if (ok) tc_fence_after();
-        if (ok) ok = issue_s(0);
-        if (ok && steps > 1) ok = issue_s(1);
-        for (int s = 0; ok && s < steps; ++s) {
-          const int t = s & 1, j = sg.two ? s >> 1 : s, k = tile0 + j;
-          const uint32_t vb = sV16 + (k % KTC_V16S) * 2 * KTC_TILE8;
-          ok = mbar_wait(v16_full + 8 * (k % KTC_V16S), (k / KTC_V16S) & 1, abort_flag) &&
-               mbar_wait(p_full + 8 * t, pcount[t] & 1, abort_flag);
-          if (!ok) break;
-          ++pcount[t];
-          tc_fence_after();
-          const int ksteps = max(1, (sg.live(j) + 15) >> 4);
-          const bool first = s < 2;
-          for (int kk = 0; kk < ksteps; ++kk)
-            umma_bf16_ts(tmem + 256 + t * 128, tmem + t * 128 + kk * 8, sw128_desc(vb + kk * 2048, KTC_TILE8, 1024),
-                         IDESC_O, !first || kk > 0);
-          if (!sg.two || t == 1) umma_commit(v16_empty + 8 * (k % KTC_V16S));
-          if (s + 2 < steps) ok = issue_s(s + 2);
+          if (issuer) {
+            ktc_issue_pv(tm + 256 + t * 128, tm + t * 128, sV16 + vq * (2 * KTC_TILE8), s >= 2);
+            if (last) umma_commit(v16_empty + 8 * vq);
+          }
+          if (last && ++vq == KTC_V16S) { vq = 0; vpar ^= 1; }
         }
-        umma_commit(o_done);
-        tile0 += sg.n;
+        if (s + 2 < steps) {
+          if (first) ok = wait(k_full + 8 * kq, kpar);
+          if (!ok) return;
+          tc_fence_after();
+          if (issuer) {
+            ktc_issue_s(tm + t * 128, two ? sQ + t * (2 * KTC_TILE8) : sQ, sK + kq * KTC_TILE8);
+            umma_commit(s_full + 8 * t);
+            if (last) umma_commit(k_empty + 8 * kq);
+          }
+          if (last && ++kq == KTC_KS) { kq = 0; kpar ^= 1; }
+        }
+      };
+      for (int s = -2; ok && s < steps; s += 2) {
+        step(std::integral_constant<uint32_t, 0>{}, s);
+        if (ok && s + 1 < steps) step(std::integral_constant<uint32_t, 1>{}, s + 1);
       }
+      if (issuer) umma_commit(o_done);
+    }
+    if (issuer) {
       umma_commit(drain);
       mbar_wait_teardown(drain, 0);
     }
@@ -394,19 +480,7 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
       const int rr = sg.qt * KTC_QR + (sg.two ? t * 128 : 0) + r;     // row of the (sequence, head)
       const bool valid = rr < sg.qt * KTC_QR + sg.rows;
       const int tok = rr / p.group;
-      const __nv_bfloat16* qrow = p.q + sg.b * p.q_sb + tok * p.q_st + (h * p.group + rr - tok * p.group) * p.q_sh;
-      float rf;
-      if (sg.two || t == 0) {
-        const uint32_t qs = sQ + t * 2 * KTC_TILE8;
-        rf = ktc_split_q<true>(qrow, valid, qs, qs + KTC_TILE8, r);
-        fence_proxy_async();
-      } else {
-        rf = ktc_split_q<false>(qrow, valid, 0, 0, r);
-      }
-      rf *= p.scale_log2;
-      tc_fence_before();   // the last segment's reads of TMEM
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
+      const float rf = valid ? __ldg(q_factor + (static_cast<long long>(sg.b) * p.c.heads + h) * rows_pad + rr) : 0.f;
       const int len = kv8_len(p.s, p.c, sg.b);
       const int seen = p.causal ? max(0, min(len, len - kv8_count(p.s, sg.b) + tok + 1)) : len;
       float m = -INFINITY, l = 0.f;
@@ -414,14 +488,41 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
       for (int i = 0; ok && i < mine; ++i, ++scount) {
         const int j = sg.two ? i : 2 * i + t;
         const int sc = (tile0 + j) % KTC_SCS;
-        ok = mbar_wait(sc_full + 8 * sc, ((tile0 + j) / KTC_SCS) & 1, abort_flag) &&
-             mbar_wait(s_full + 8 * t, scount & 1, abort_flag);
+        // The tile's scales come to registers before its scores are there:
+        // shared memory answers slowly while the MMAs read their operands.
+        ok = mbar_wait(sc_full + 8 * sc, ((tile0 + j) / KTC_SCS) & 1, abort_flag);
+        const float4* scale = reinterpret_cast<const float4*>(smem + L::SC_OFF) + sc * 8;
+        float fs[8], lv[8];
+        {
+          const float4 a = scale[0], b = scale[1], c = scale[2], d = scale[3];
+          const float ks[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+          for (int g8 = 0; g8 < 8; ++g8) fs[g8] = fmaxf(rf * ks[g8], 1.17549435e-38f);   // > 0: hidden scores stay -inf
+          lv[0] = c.x; lv[1] = c.y; lv[2] = c.z; lv[3] = c.w;
+          lv[4] = d.x; lv[5] = d.y; lv[6] = d.z; lv[7] = d.w;
+        }
+        ok = ok && mbar_wait(s_full + 8 * t, scount & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        const float4* scale = reinterpret_cast<const float4*>(smem + L::SC_OFF) + sc * 8;
         const int lim = seen - (sg.j0 + j) * KTC_TK;    // keys of this tile that the row sees
         const bool part = __any_sync(0xffffffffu, lim < KTC_TK);
+        if (part) {
+          // Hidden scores become -inf where they lie, in a rolled loop: 128
+          // selects inside the common path cost it 4% (its code no longer
+          // stays in the instruction cache).
+#pragma unroll 1
+          for (int c = 0; c < 4; ++c) {
+            float x[32];
+            tmem_ld32(tS + c * 32, x);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 32; ++k)
+              if (c * 32 + k >= lim) x[k] = -INFINITY;
+            tmem_st32(tS + c * 32, x);
+          }
+          tmem_wait_st();
+        }
         float s[128];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -431,16 +532,10 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
           for (int k = 0; k < 32; ++k) s[c * 32 + k] = x[k];
         }
         tmem_wait_ld();
-        if (part) {
-#pragma unroll
-          for (int k = 0; k < 128; ++k)
-            if (k >= lim) s[k] = -INFINITY;
-        }
         // Maximum of y over the 8 groups of 16 keys; NaN wins (it makes the row NaN).
         float mx = -INFINITY;
 #pragma unroll
         for (int g8 = 0; g8 < 8; ++g8) {
-          const float4 f = scale[g8];
           const float* sg8 = s + 16 * g8;
           float a = max3_nan(sg8[0], sg8[1], sg8[2]), b = max3_nan(sg8[3], sg8[4], sg8[5]);
           a = max3_nan(a, sg8[6], sg8[7]);
@@ -449,22 +544,21 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
           b = max3_nan(b, sg8[12], sg8[13]);
           a = max3_nan(a, sg8[14], sg8[15]);
           a = max3_nan(a, b, b);
-          a = fmaf(a, fmaxf(rf * f.x, 1.17549435e-38f), f.y);
+          a = fmaf(a, fs[g8], lv[g8]);
           mx = max3_nan(mx, a, a);
         }
         const bool grow = !(mx <= m + FEW_RESCALE);
         const float m_new = grow ? mx : m;
         const float z = (m_new == -INFINITY ? 0.f : m_new) - FEW_OFFSET;
         const float alpha = grow ? (m == -INFINITY ? 0.f : exp2f(m - m_new)) : 1.f;
-        float sum = 0.f;
+        float sums[8];
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t pk[16];
 #pragma unroll
           for (int gq = 0; gq < 2; ++gq) {
-            const float4 f = scale[2 * c + gq];
-            const float fs = fmaxf(rf * f.x, 1.17549435e-38f), cs = f.y - z;
-            const uint64_t f2s = f2(fs, fs), c2s = f2(cs, cs);
+            const float cs = lv[2 * c + gq] - z;
+            const uint64_t f2s = f2(fs[2 * c + gq], fs[2 * c + gq]), c2s = f2(cs, cs);
             uint64_t sum2 = f2(0.f, 0.f);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
@@ -482,11 +576,10 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
               pk[8 * gq + k] = pack_f16(e.x, e.y);
             }
             const float2 sv = f2_split(sum2);
-            sum = fmaf(sv.x + sv.y, f.z, sum);
+            sums[2 * c + gq] = sv.x + sv.y;
           }
           tmem_st16u(tS + c * 16, pk);
         }
-        if (m_new == -INFINITY) sum = 0.f;   // no key seen yet (the polynomial's 2^-125 are no weights)
         if (i > 0 && __any_sync(0xffffffffu, grow)) {
           // O is stable: this S was issued behind the slot's last PV and is complete.
 #pragma unroll 1
@@ -503,7 +596,19 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full + 8 * t);
-        l = l * alpha + sum;
+        {
+          const float4 a = scale[4], b = scale[5];
+          float sum = sums[0] * a.x;
+          sum = fmaf(sums[1], a.y, sum);
+          sum = fmaf(sums[2], a.z, sum);
+          sum = fmaf(sums[3], a.w, sum);
+          sum = fmaf(sums[4], b.x, sum);
+          sum = fmaf(sums[5], b.y, sum);
+          sum = fmaf(sums[6], b.z, sum);
+          sum = fmaf(sums[7], b.w, sum);
+          if (m_new == -INFINITY) sum = 0.f;   // no key seen yet (the polynomial's 2^-125 are no weights)
+          l = fmaf(l, alpha, sum);
+        }
         m = m_new;
       }
       tile0 += sg.n;
@@ -562,6 +667,9 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
           for (int k = 0; k < 8; ++k) dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
         }
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_free);
       if (valid && (sg.two || t == 0)) {
         if (!whole) {
           part[KTC_QR * 128 + prow] = mref;
