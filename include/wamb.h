@@ -558,7 +558,9 @@ WAMB_API int wamb_kv8_attention(const wamb_kv8_attention_args* args, void* strea
  * head h that see j of exp(scale q k_j - lse), lse as wamb_kv8_attention gave
  * it for the same q, lens, counts, causal and scale (rows with lse -inf add
  * nothing). Columns that no row sees carry the base over. out, out_stride and
- * v8 are not read. */
+ * v8 are not read. workspace: wamb_kv8_weights_workspace_bytes() bytes (0
+ * for few rows), as for wamb_kv8_attention. */
+WAMB_API size_t wamb_kv8_weights_workspace_bytes(const wamb_kv8_attention_args* args);
 WAMB_API int wamb_kv8_weights(const wamb_kv8_attention_args* args, void* stream);
 
 /* Eviction by accumulated weight, for each cached head on its own: of sequence

@@ -489,3 +489,13 @@ def test_bad_pages_and_lengths_are_reported(cuda_device):
     bad(lambda: c.evict(table, n, w, table[:, :1].contiguous(), heavy=4, recent=4))   # onto itself
     c.attention(q, table, n)
     assert _lib.device_status() == 0
+
+
+# ------------------------------------------- many tiles behind one another
+@pytest.mark.parametrize("B,H,G,T,L,causal", [(1, 2, 1, 880, 4400, False), (2, 1, 2, 700, 3000, True), (3, 2, 1, 100, 2500, False)])
+def test_weights_many_tiles(cuda_device, B, H, G, T, L, causal):
+    """Units of one to eleven query tiles in one CTA's share (the
+    exponentials fall behind the loads by several tiles)."""
+    c, table, _, n, g = _setup(B, H, 64, [L - 300 * b for b in range(B)], T, poison=False)
+    counts = _i32([T - 256 * b if T > 600 else T for b in range(B)])
+    _check_weights(c, _q(g, B, T, H * G, 128), table, n, table.shape[1] * 64, counts=counts, causal=causal)

@@ -7,11 +7,14 @@
 //
 // The `group` query heads of one cached head are rows of one tile (row
 // r = token * group + head in group), so each cached byte is read once for
-// all of them. A warp takes 16 keys at a time: their K and V codes (2 KB each)
-// come by TMA into its own ring, become f16 in registers (E4M3 is a subset of
-// f16, so nothing is rounded) and meet the queries in m16n8k16 products with
-// fp32 sums: Q (16 rows) x K^T, then P x V. Queries are scaled per row by a
-// power of two into f16's range first, which keeps their eight bits.
+// all of them. A warp takes 32 keys at a time, K and V codes (4 KB each) by
+// TMA into its own ring, with no barrier between warps until an item ends.
+// S = Q K^T takes the codes as they are (m16n8k32): a bf16 query has eight
+// significant bits, which are two E4M3 values of four, q 2^-n = hi + lo, so
+// S = (hi K^T + lo K^T) 2^n. n puts the row's largest magnitude into (224,
+// 448]; a value below 2^-10 of that keeps an absolute error of at most 2^-10
+// (2^-17 of the largest). For P V the codes become f16 in registers (E4M3 is a
+// subset of f16, nothing is rounded).
 //
 // The scales of a block enter the exponent: with y_ij = s_ij log2(e) +
 // log2(vs_j) the kernel sums P_ij = 2^(y_ij - M_i) against the codes, M_i a
@@ -19,6 +22,7 @@
 // l_i = sum_j P_ij / vs_j. P goes to the product as f16 with an offset of 2^6:
 // 11 bits down to 2^-20 of the row's maximum and whole steps of 2^-30 below.
 #pragma once
+#include "attention.cuh"
 #include "kv8.cuh"
 
 namespace wamb {
@@ -274,27 +278,47 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
 }
 
 // --------------------------------------------------------------- few rows
-constexpr int FEW_QR = 16, FEW_TK = 64, FEW_THREADS = 128, FEW_WARPS = 4;
+constexpr int FEW_QR = 16, FEW_TK = 128, FEW_THREADS = 128, FEW_WARPS = 4;
+constexpr int FEW_KEYS = 32;          // of a warp in one unit: two halves of 16, each inside one page
 constexpr float FEW_RESCALE = 8.f;    // log2 growth of the maximum that moves it
 constexpr float FEW_OFFSET = 6.f;     // P is 2^6 at the maximum
 
+// A warp's keys of one unit: where their codes lie and what they are scaled by.
+struct FewUnit {
+  int row[2];      // first row of each half in the [pages * heads * page, 128] code matrix
+  int k0, live;    // first key position, live keys
+  float ks[2], vs[2];
+  int e, h, last;  // last: the unit ends its item or the CTA's share
+  int pad;
+};
+
 template <bool WEIGHTS>
 struct FewSmem {
-  static constexpr int STAGES = WEIGHTS ? 8 : 4;
-  static constexpr uint32_t STAGE_BYTES = WEIGHTS ? 2048 : 4096;    // 16 keys: K codes, V codes
+  static constexpr int STAGES = WEIGHTS ? 4 : 2;
+  static constexpr uint32_t K_BYTES = FEW_KEYS * 128;
+  static constexpr uint32_t STAGE_BYTES = WEIGHTS ? K_BYTES : 2 * K_BYTES;    // K codes, V codes
   static constexpr uint32_t RING = FEW_WARPS * STAGES * STAGE_BYTES;
   static constexpr uint32_t LD = 132;                               // merge rows, padded
   static constexpr uint32_t MERGE_OFF = RING;
   static constexpr uint32_t MERGE_BYTES = WEIGHTS ? 0 : FEW_WARPS * FEW_QR * LD * 4;
   static constexpr uint32_t ML_OFF = MERGE_OFF + MERGE_BYTES;       // m, l [warps][16]
-  static constexpr uint32_t BAR_OFF = ML_OFF + 2 * FEW_WARPS * FEW_QR * 4;
+  static constexpr uint32_t UNIT_OFF = ML_OFF + 2 * FEW_WARPS * FEW_QR * 4;   // [warps][2 batches][32]
+  static constexpr uint32_t BAR_OFF = UNIT_OFF + FEW_WARPS * 64 * sizeof(FewUnit);
   static constexpr uint32_t SCHED_OFF = BAR_OFF + FEW_WARPS * STAGES * 8;
   static constexpr uint32_t TOTAL = 1024 + SCHED_OFF + sizeof(Kv8SchedSmem) + 16;
+  static_assert(sizeof(FewUnit) == 48 && 2 * (TOTAL + 1024) <= 233472, "two CTAs must fit an SM");
 };
 
+// fp32 += f16 x f16: 16 rows x 16 x 8; and E4M3 x E4M3: 16 rows x 32 x 8.
 WAMB_DEV void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+WAMB_DEV void mma_e4m3_16832(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -308,37 +332,47 @@ WAMB_DEV uint4 lds128(uint32_t a) {
   return v;
 }
 
-// A warp's 16 keys of one unit, as lane i of a batch holds them for unit i.
-struct FewUnit {
-  int row;        // first row in the [pages * heads * page, 128] code matrix
-  int k0;         // first key position; the number of live keys in bits 27..31
-  float ks, vs;
-  int e, h;
-  int last;       // this unit ends its item or the CTA's share
-};
+// Four values into their E4M3 code word `h` and the word of what it leaves.
+// A bf16 value has eight significant bits: two codes of four hold it.
+WAMB_DEV void split_e4m3x4(const float (&x)[4], uint32_t& h, uint32_t& l) {
+  const uint32_t h0 = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t h1 = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
+  const float2 f0 = e4m3x2_to_float2(h0), f1 = e4m3x2_to_float2(h1);
+  const uint32_t l0 = __nv_cvt_float2_to_fp8x2(make_float2(x[0] - f0.x, x[1] - f0.y), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t l1 = __nv_cvt_float2_to_fp8x2(make_float2(x[2] - f1.x, x[3] - f1.y), __NV_SATFINITE, __NV_E4M3);
+  h = h0 | (h1 << 16);
+  l = l0 | (l1 << 16);
+}
+// Exponent n and factor 2^-n that bring a query row's largest magnitude into
+// (224, 448]. An infinite query makes its row NaN, as the formula does (a
+// saturated one would not).
+WAMB_DEV float query_scale(float amax, int& n) {
+  const int bits = __float_as_int(fminf(amax, 3.402823466e38f));
+  n = max(-118, min(119, (bits >> 23) - 135 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0)));
+  return amax <= 3.402823466e38f ? pow2f_exact(-n) : __int_as_float(0x7fffffff);
+}
 
-// One Q fragment set: the 16 rows of (entry, head) as f16 A operands of eight
-// 16-wide steps. Step s < 4 holds dims 16 t + 4 s + 0..3 of thread t = lane & 3
-// (the two halves of the step's 16 columns are this order for Q and K alike),
-// step s >= 4 dims 64 + 16 t + 4 (s - 4) + 0..3.
+// The 16 rows of an (entry, head) as E4M3 A operands of four 32-wide steps,
+// in two pieces. Thread t = lane & 3 holds dims 16 t .. 16 t + 15 in words 0-3
+// of a row and 64 + 16 t .. in words 4-7; step s takes words 2 s, 2 s + 1 (the
+// same order for queries and keys, so the sum over dims is the same).
 struct FewQ {
-  uint32_t a[8][4];
-  float rf[2];        // row factor: (power-of-two row scale) * scale * log2(e); rows g, g + 8
+  uint32_t hi[4][4], lo[4][4];
+  float rf[2];        // row factor: 2^n * scale * log2(e); rows g, g + 8
   int seen[2];        // keys each row sees
 };
 
-template <int QR, int TK>
-WAMB_DEV void few_load_q(const Kv8AttnParams& p, int e, int h, int qt, FewQ& f) {
+WAMB_DEV void few_load_q(const Kv8AttnParams& p, int e, int h, FewQ& f) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  const int b = e / p.qts;
+  const int b = e;   // one query tile per sequence
   const int tokens = kv8_count(p.s, b), len = kv8_len(p.s, p.c, b);
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    const int rr = qt * QR + g + 8 * half;
+    const int rr = g + 8 * half;
     const bool ok = rr < tokens * p.group;
     const int t = rr / p.group;
     const __nv_bfloat16* src = p.q + b * p.q_sb + t * p.q_st + (h * p.group + rr - t * p.group) * p.q_sh + 16 * t4;
-    float x[32];
+    float x[8][4];
     float amax = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -347,59 +381,59 @@ WAMB_DEV void few_load_q(const Kv8AttnParams& p, int e, int h, int qt, FewQ& f) 
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float2 v = unpack_bf16(ws[k]);
-        x[8 * i + 2 * k] = v.x;
-        x[8 * i + 2 * k + 1] = v.y;
+        x[2 * i + (k >> 1)][2 * (k & 1)] = v.x;
+        x[2 * i + (k >> 1)][2 * (k & 1) + 1] = v.y;
         amax = fmaxf(amax, fmaxf(fabsf(v.x), fabsf(v.y)));
       }
     }
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    // The row's largest magnitude goes to [2^13, 2^14).
-    const int ex = min(max(__float_as_int(amax) >> 23, 14), 254);
-    const float up = __int_as_float((267 - ex) << 23);
+    int n;
+    const float up = query_scale(amax, n);
 #pragma unroll
-    for (int s = 0; s < 8; ++s) {
-      f.a[s][half] = pack_f16(x[4 * s] * up, x[4 * s + 1] * up);
-      f.a[s][2 + half] = pack_f16(x[4 * s + 2] * up, x[4 * s + 3] * up);
+    for (int w = 0; w < 8; ++w) {
+      const float y[4] = {x[w][0] * up, x[w][1] * up, x[w][2] * up, x[w][3] * up};
+      split_e4m3x4(y, f.hi[w >> 1][half + 2 * (w & 1)], f.lo[w >> 1][half + 2 * (w & 1)]);
     }
-    f.rf[half] = __int_as_float((ex - 13) << 23) * p.scale_log2;
-    f.seen[half] = p.causal ? max(0, min(len, len - tokens + t + 1)) : len;
-    if (!ok) f.seen[half] = 0;
+    f.rf[half] = pow2f_exact(n) * p.scale_log2;
+    f.seen[half] = !ok ? 0 : p.causal ? max(0, min(len, len - tokens + t + 1)) : len;
   }
 }
 
-// S [16 rows][16 keys] of a warp's keys at `stage` (swizzled rows of 128 codes).
-WAMB_DEV void few_scores(uint32_t stage, const FewQ& q, float (&s)[2][4]) {
+// S [16 rows][32 keys] of a warp's keys at `stage` (swizzled rows of 128 codes).
+WAMB_DEV void few_scores(uint32_t stage, const FewQ& q, float (&s)[4][4]) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+  // The two 16-byte pieces of a row, in an order that alternates with the row
+  // so that eight lanes cover all banks.
+  const int o = (g & 1) * 4;
+  const bool sw = g & 1;
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    // The two 16-byte pieces of the row, in an order that alternates with the
-    // row so that eight lanes cover all banks.
+  for (int j = 0; j < 4; ++j) {
     const uint32_t row = stage + (8 * j + g) * 128;
-    const int o = (g & 1) * 4;
     const uint4 x = lds128(row + (((t4 + o) ^ g) << 4));
     const uint4 y = lds128(row + (((t4 + 4 - o) ^ g) << 4));
-    const bool sw = g & 1;
     const uint32_t w[8] = {sw ? y.x : x.x, sw ? y.y : x.y, sw ? y.z : x.z, sw ? y.w : x.w,
                            sw ? x.x : y.x, sw ? x.y : y.y, sw ? x.z : y.z, sw ? x.w : y.w};
+    float r[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[j][i] = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      mma_f16_16816(s[j], q.a[k], e4m3x2_to_f16x2(w[k] & 0xffffu), e4m3x2_to_f16x2(w[k] >> 16));
+    for (int k = 0; k < 4; ++k) {   // two chains of sums, half as long
+      mma_e4m3_16832(s[j], q.hi[k], w[2 * k], w[2 * k + 1]);
+      mma_e4m3_16832(r, q.lo[k], w[2 * k], w[2 * k + 1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[j][i] += r[i];
   }
 }
 
-// WEIGHTS = false: attention; units of every query tile are on the line.
-// WEIGHTS = true: p.qts is 1 on the line; each unit loops over `row_tiles`
-// tiles of 16 rows and owns its keys' sums, so no sum has a racing order.
+// Attention (WEIGHTS = false) and attention weights (true; each unit owns its
+// keys' sums, so no sum has a racing order).
 template <bool WEIGHTS>
 __global__ void __launch_bounds__(FEW_THREADS)
     kv8_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                   const Kv8AttnParams p, const int row_tiles) {
+                   const Kv8AttnParams p) {
   using L = FewSmem<WEIGHTS>;
-  // The line of the weights has one entry per sequence whatever its rows.
-  constexpr int QR = WEIGHTS ? (1 << 30) : FEW_QR;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
   Kv8SchedSmem& sched = *reinterpret_cast<Kv8SchedSmem*>(smem + L::SCHED_OFF);
@@ -407,6 +441,7 @@ __global__ void __launch_bounds__(FEW_THREADS)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const uint32_t ring = smem_u32(smem) + warp * (L::STAGES * L::STAGE_BYTES);
   const uint32_t bars = smem_u32(smem + L::BAR_OFF) + warp * (L::STAGES * 8);
+  FewUnit* units = reinterpret_cast<FewUnit*>(smem + L::UNIT_OFF) + warp * 64;
   if (lane == 0)
     for (int i = 0; i < L::STAGES; ++i) mbar_init(bars + 8 * i, 1);
   if (threadIdx.x == 0) *abort_flag = 0;
@@ -424,69 +459,73 @@ __global__ void __launch_bounds__(FEW_THREADS)
   }
   Kv8Share sh;
   Kv8Item it;
-  const bool work = kv8_share<QR, FEW_TK, FEW_THREADS>(p, blockIdx.x, sched, sh, it);
+  const bool work = kv8_share<FEW_QR, FEW_TK, FEW_THREADS>(p, blockIdx.x, sched, sh, it);
   if constexpr (!WEIGHTS) {
     if (threadIdx.x == 0) kv8_leave_join(p, sh, work, it);
   }
   if (!work) return;
   const int count = static_cast<int>(sh.u1 - sh.u0);
-  const long long first_start = it.start;   // the item the share begins in
+  bool began = it.start == sh.u0;      // the current item begins in this share
 
-  // Batches of 32 units: lane i holds unit i's addresses and scales, loaded a
-  // whole batch ahead of their use. `cur` moves over the line with them.
-  Kv8Item cur = it;
-  auto load_batch = [&](int j0, FewUnit& u) {
-    u.row = 0; u.k0 = 0; u.ks = 1.f; u.vs = 1.f; u.e = 0; u.h = 0; u.last = 0;
-    Kv8Item mine = cur;
+  // Batches of 32 units: lane i looks up unit i's addresses and scales, a
+  // whole batch ahead of their use. `it` moves over the line with them.
+  auto load_batch = [&](int j0) {
     const int j = min(j0 + lane, count - 1);
-    kv8_seek<QR, FEW_TK>(p, mine, sh.u0 + j);
-    if (j0 + lane < count) {
-      const int tile = static_cast<int>(sh.u0 + j - mine.start);
-      const int k0 = tile * FEW_TK + warp * 16;
-      const int live = max(0, min(16, Kv8Line<QR, FEW_TK>::visible(p, mine.e) - k0));
-      u.e = mine.e;
-      u.h = mine.h;
-      u.k0 = k0;
-      u.last = tile == mine.n - 1 || j == count - 1;
-      if (live > 0) {
-        int pid = kv8_page(p.s.table, p.s.width, p.c, mine.e / p.qts, k0 >> p.c.page_log2);
+    kv8_seek<FEW_QR, FEW_TK>(p, it, sh.u0 + j);
+    const int tile = static_cast<int>(sh.u0 + j - it.start);
+    FewUnit u;
+    u.k0 = tile * FEW_TK + warp * FEW_KEYS;
+    u.live = max(0, min(FEW_KEYS, Kv8Line<FEW_QR, FEW_TK>::visible(p, it.e) - u.k0));
+    u.e = it.e;
+    u.h = it.h;
+    u.last = tile == it.n - 1 || j == count - 1;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      u.row[i] = 0;
+      u.ks[i] = u.vs[i] = 1.f;
+      if (u.live > 16 * i) {
+        const int k = u.k0 + 16 * i;
+        int pid = kv8_page(p.s.table, p.s.width, p.c, it.e / p.qts, k >> p.c.page_log2);
         if (pid < 0) pid = 0;   // reported
-        const long long blk = static_cast<long long>(pid) * p.c.heads + mine.h;
-        u.row = static_cast<int>((blk << p.c.page_log2) + (k0 & (p.c.page - 1)));
-        u.ks = __ldg(p.c.k_scale + blk);
-        if constexpr (!WEIGHTS) u.vs = __ldg(p.c.v_scale + blk);
+        const long long blk = static_cast<long long>(pid) * p.c.heads + it.h;
+        u.row[i] = static_cast<int>((blk << p.c.page_log2) + (k & (p.c.page - 1)));
+        u.ks[i] = __ldg(p.c.k_scale + blk);
+        if constexpr (!WEIGHTS) u.vs[i] = __ldg(p.c.v_scale + blk);
       }
-      u.last |= live << 8;
     }
-    cur.e = __shfl_sync(0xffffffffu, mine.e, 31);
-    cur.h = __shfl_sync(0xffffffffu, mine.h, 31);
-    cur.n = __shfl_sync(0xffffffffu, mine.n, 31);
-    cur.start = __shfl_sync(0xffffffffu, mine.start, 31);
+    u.pad = 0;
+    units[(j0 & 32) + lane] = u;
+    it.e = __shfl_sync(0xffffffffu, it.e, 31);
+    it.h = __shfl_sync(0xffffffffu, it.h, 31);
+    it.n = __shfl_sync(0xffffffffu, it.n, 31);
+    it.start = __shfl_sync(0xffffffffu, it.start, 31);
+    __syncwarp();
   };
-  FewUnit now, next;
-  load_batch(0, now);
-  if (count > 32) load_batch(32, next);
-  else next = now;
-  int issued = 0, used = 0, ahead = 0;   // ring loads issued and consumed; next unit to issue
-  auto issue = [&](int base) {   // base: first unit of `now`
-    while (ahead < count && ahead < base + 64 && issued < used + L::STAGES) {
-      const bool nx = ahead >= base + 32;
-      const int l = ahead & 31;
-      const int meta = __shfl_sync(0xffffffffu, nx ? next.last : now.last, l);
-      const int row = __shfl_sync(0xffffffffu, nx ? next.row : now.row, l);
-      if ((meta >> 8) > 0) {
-        const int st = issued % L::STAGES;
+  int issued = 0, used = 0, ahead = 0, known = 0;   // ring loads issued and consumed; next unit to issue; units looked up
+  auto issue = [&]() {
+    while (ahead < known && issued < used + L::STAGES) {
+      const FewUnit& u = units[ahead & 63];
+      const int live = u.live;
+      if (live > 0) {
+        const uint32_t st = issued % L::STAGES, at = ring + st * L::STAGE_BYTES, bar = bars + 8 * st;
         if (lane == 0) {
-          mbar_arrive_expect_tx(bars + 8 * st, L::STAGE_BYTES);
-          tma_load_2d(ring + st * L::STAGE_BYTES, &tmK, bars + 8 * st, 0, row);
-          if constexpr (!WEIGHTS) tma_load_2d(ring + st * L::STAGE_BYTES + 2048, &tmV, bars + 8 * st, 0, row);
+          const int r0 = u.row[0], r1 = u.row[1];
+          mbar_arrive_expect_tx(bar, (live > 16 ? 2 : 1) * (WEIGHTS ? 2048 : 4096));
+          tma_load_2d(at, &tmK, bar, 0, r0);
+          if (live > 16) tma_load_2d(at + 2048, &tmK, bar, 0, r1);
+          if constexpr (!WEIGHTS) {
+            tma_load_2d(at + L::K_BYTES, &tmV, bar, 0, r0);
+            if (live > 16) tma_load_2d(at + L::K_BYTES + 2048, &tmV, bar, 0, r1);
+          }
         }
         ++issued;
       }
       ++ahead;
     }
   };
-  issue(0);
+  load_batch(0);
+  known = min(32, count);
+  issue();
 
   FewQ q;
   float o[16][4];
@@ -500,103 +539,83 @@ __global__ void __launch_bounds__(FEW_THREADS)
     l[0] = l[1] = 0.f;
   };
   bool fresh = true;
-  bool began = it.start == sh.u0;      // the current item begins in this share
-  long long item_start = first_start;
-  (void)item_start;
   bool ok = true;
   for (int j = 0; j < count; ++j) {
-    if ((j & 31) == 0 && j > 0) {
-      now = next;
-      if (j + 32 < count) load_batch(j + 32, next);
+    if ((j & 31) == 8 && known < count) {   // the batch before this one is used up: its places take the next
+      load_batch(known);
+      known = min(known + 32, count);
+      issue();
     }
-    const int base = j & ~31;
-    const int src = j & 31;
-    const int meta = __shfl_sync(0xffffffffu, now.last, src);
-    const int e = __shfl_sync(0xffffffffu, now.e, src);
-    const int h = __shfl_sync(0xffffffffu, now.h, src);
-    const int k0 = __shfl_sync(0xffffffffu, now.k0, src);
-    const float ks = __shfl_sync(0xffffffffu, now.ks, src);
-    const int live = meta >> 8;
-    const int b = e / p.qts;
-    if constexpr (!WEIGHTS) {
-      if (fresh) {
-        few_load_q<FEW_QR, FEW_TK>(p, e, h, e - b * p.qts, q);
+    const FewUnit& u = units[j & 63];
+    const int live = u.live, k0 = u.k0, last = u.last;
+    if (fresh) {
+      few_load_q(p, u.e, u.h, q);
+      if constexpr (WEIGHTS) {
+        // The rows' log-sum-exp in log2 units; rows that see nothing add nothing.
+        const int tokens = kv8_count(p.s, u.e);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int rr = g + 8 * half, t = rr / p.group;
+          l[half] = INFINITY;
+          if (rr < tokens * p.group) {
+            const float x = p.lse_in[(static_cast<long long>(u.e) * p.s.tokens + t) * (p.c.heads * p.group) + u.h * p.group +
+                                     rr - t * p.group];
+            if (x != -INFINITY) l[half] = x * 1.4426950408889634f;
+          }
+        }
+      } else {
         reset();
-        fresh = false;
       }
+      fresh = false;
     }
-    uint32_t stage = 0;
     if (live > 0) {
+      const float ks[2] = {u.ks[0], u.ks[1]};
+      [[maybe_unused]] const float vs[2] = {u.vs[0], u.vs[1]};
       const int st = used % L::STAGES;
-      stage = ring + st * L::STAGE_BYTES;
-      ok = ok && mbar_wait(bars + 8 * st, (used / L::STAGES) & 1, abort_flag);
-    }
-    if constexpr (WEIGHTS) {
-      if (live > 0) {
-        float w[4] = {0.f, 0.f, 0.f, 0.f};   // keys 2 t, 2 t + 1, 8 + 2 t, 9 + 2 t
-        for (int qt = 0; qt < row_tiles; ++qt) {
-          if (fresh || row_tiles > 1) {
-            few_load_q<FEW_QR, FEW_TK>(p, e, h, qt, q);
-            // The rows' log-sum-exp in log2 units; rows that see nothing add nothing.
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const int rr = qt * FEW_QR + g + 8 * half;
-              const int t = rr / p.group;
-              l[half] = INFINITY;
-              if (rr < kv8_count(p.s, b) * p.group) {
-                const float x = p.lse_in[(static_cast<long long>(b) * p.s.tokens + t) * (p.c.heads * p.group) +
-                                         h * p.group + rr - t * p.group];
-                if (x != -INFINITY) l[half] = x * 1.4426950408889634f;
-              }
-            }
-            fresh = false;
-          }
-          float s[2][4];
-          few_scores(stage, q, s);
-#pragma unroll
-          for (int jt = 0; jt < 2; ++jt)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              const int half = c >> 1, key = k0 + 8 * jt + 2 * t4 + (c & 1);
-              const float x = ex2_mufu(fmaf(s[jt][c], q.rf[half] * ks, -l[half]));
-              if (key < q.seen[half]) w[2 * jt + (c & 1)] += x;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) w[i] += __shfl_xor_sync(0xffffffffu, w[i], x);
-        }
-        if (g == 0) {
-          const long long at = (static_cast<long long>(b) * p.c.heads + h) * p.w_cap + k0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int key = (i >> 1) * 8 + 2 * t4 + (i & 1);
-            if (key < live) p.weights[at + key] = ok ? (p.base != nullptr ? p.base[at + key] : 0.f) + w[i] : 0.f;
-          }
-        }
+      const uint32_t stage = ring + st * L::STAGE_BYTES;
+      if constexpr (WEIGHTS) {
+        // Lane (g, t) finishes key 8 (g / 2) + 2 t + g % 2.
+        const int key = 8 * (g >> 1) + 2 * t4 + (g & 1);
+        const long long at = (static_cast<long long>(u.e) * p.c.heads + u.h) * p.w_cap + k0 + key;
+        const float base = p.base != nullptr && key < live ? __ldcg(p.base + at) : 0.f;
+        ok = mbar_wait(bars + 8 * st, (used / L::STAGES) & 1, abort_flag) && ok;
+        float s[4][4];
+        few_scores(stage, q, s);
         __syncwarp();
         ++used;
-        issue(base);
-      }
-      if (meta & 1) fresh = true;
-    } else {
-      if (live > 0) {
-        const float vs = __shfl_sync(0xffffffffu, now.vs, src);
-        const float lv = log2f(vs), iv = 1.f / vs;
-        float s[2][4];
+        issue();
+        float mine = 0.f;
+#pragma unroll
+        for (int jt = 0; jt < 4; ++jt) {
+          const float f0 = q.rf[0] * ks[jt >> 1], f1 = q.rf[1] * ks[jt >> 1];
+          const int kk = k0 + 8 * jt + 2 * t4;
+          float w[2];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const float a = ex2_mufu(fmaf(s[jt][c], f0, -l[0])), d = ex2_mufu(fmaf(s[jt][2 + c], f1, -l[1]));
+            w[c] = (kk + c < q.seen[0] ? a : 0.f) + (kk + c < q.seen[1] ? d : 0.f);
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) w[c] += __shfl_xor_sync(0xffffffffu, w[c], x);
+          }
+          if (jt == g >> 1) mine = (g & 1) ? w[1] : w[0];
+        }
+        if (key < live) p.weights[at] = ok ? base + mine : 0.f;
+      } else {
+        ok = mbar_wait(bars + 8 * st, (used / L::STAGES) & 1, abort_flag) && ok;
+        float s[4][4];
         few_scores(stage, q, s);
-        const float f[2] = {q.rf[0] * ks, q.rf[1] * ks};
-        float y[2][4];
+        const float lv[2] = {log2f(vs[0]), log2f(vs[1])}, iv[2] = {1.f / vs[0], 1.f / vs[1]};
         float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int jt = 0; jt < 2; ++jt)
+        for (int jt = 0; jt < 4; ++jt) {
+          const float f[2] = {q.rf[0] * ks[jt >> 1], q.rf[1] * ks[jt >> 1]};
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const int half = c >> 1, key = k0 + 8 * jt + 2 * t4 + (c & 1);
-            y[jt][c] = key < q.seen[half] ? fmaf(s[jt][c], f[half], lv) : -INFINITY;
-            mx[half] = fmaxf(mx[half], y[jt][c]);
+            s[jt][c] = key < q.seen[half] ? fmaf(s[jt][c], f[half], lv[jt >> 1]) : -INFINITY;
+            mx[half] = fmaxf(mx[half], s[jt][c]);
           }
+        }
         if (__any_sync(0xffffffffu, mx[0] > m[0] + FEW_RESCALE || mx[1] > m[1] + FEW_RESCALE)) {
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
@@ -616,112 +635,116 @@ __global__ void __launch_bounds__(FEW_THREADS)
         }
         const float z0 = (m[0] == -INFINITY ? 0.f : m[0]) - FEW_OFFSET, z1 = (m[1] == -INFINITY ? 0.f : m[1]) - FEW_OFFSET;
 #pragma unroll
-        for (int jt = 0; jt < 2; ++jt) {
-          y[jt][0] = ex2_mufu(y[jt][0] - z0);
-          y[jt][1] = ex2_mufu(y[jt][1] - z0);
-          y[jt][2] = ex2_mufu(y[jt][2] - z1);
-          y[jt][3] = ex2_mufu(y[jt][3] - z1);
+        for (int jt = 0; jt < 4; ++jt) {
+          s[jt][0] = ex2_mufu(s[jt][0] - z0);
+          s[jt][1] = ex2_mufu(s[jt][1] - z0);
+          s[jt][2] = ex2_mufu(s[jt][2] - z1);
+          s[jt][3] = ex2_mufu(s[jt][3] - z1);
+          l[0] = fmaf(s[jt][0] + s[jt][1], iv[jt >> 1], l[0]);
+          l[1] = fmaf(s[jt][2] + s[jt][3], iv[jt >> 1], l[1]);
         }
-        l[0] += (y[0][0] + y[0][1] + y[1][0] + y[1][1]) * iv;
-        l[1] += (y[0][2] + y[0][3] + y[1][2] + y[1][3]) * iv;
-        const uint32_t a[4] = {pack_f16(y[0][0], y[0][1]), pack_f16(y[0][2], y[0][3]), pack_f16(y[1][0], y[1][1]),
-                               pack_f16(y[1][2], y[1][3])};
-        // V rows 2 t, 2 t + 1, 8 + 2 t, 9 + 2 t, dims [16 g, +16); output
-        // column n = g of product i is dim 16 g + i.
-        uint4 v[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = (i >> 1) * 8 + 2 * t4 + (i & 1);
-          v[i] = lds128(stage + 2048 + r * 128 + ((g ^ (r & 7)) << 4));
-          if (r >= live) v[i] = make_uint4(0, 0, 0, 0);   // whatever lies there (NaN codes too) counts for nothing
-        }
-        __syncwarp();
-        ++used;
-        issue(base);
+        for (int kk = 0; kk < 2; ++kk) {
+          // V rows 2 t, 2 t + 1, 8 + 2 t, 9 + 2 t of the half, dims [16 g, +16);
+          // output column n = g of product i is dim 16 g + i.
+          const uint32_t a[4] = {pack_f16(s[2 * kk][0], s[2 * kk][1]), pack_f16(s[2 * kk][2], s[2 * kk][3]),
+                                 pack_f16(s[2 * kk + 1][0], s[2 * kk + 1][1]), pack_f16(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+          uint4 v[4];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t v0 = w == 0 ? v[0].x : w == 1 ? v[0].y : w == 2 ? v[0].z : v[0].w;
-          const uint32_t v1 = w == 0 ? v[1].x : w == 1 ? v[1].y : w == 2 ? v[1].z : v[1].w;
-          const uint32_t v2 = w == 0 ? v[2].x : w == 1 ? v[2].y : w == 2 ? v[2].z : v[2].w;
-          const uint32_t v3 = w == 0 ? v[3].x : w == 1 ? v[3].y : w == 2 ? v[3].z : v[3].w;
-          const uint32_t lo0 = __byte_perm(v0, v1, 0x5140), hi0 = __byte_perm(v0, v1, 0x7362);
-          const uint32_t lo1 = __byte_perm(v2, v3, 0x5140), hi1 = __byte_perm(v2, v3, 0x7362);
-          mma_f16_16816(o[4 * w], a, e4m3x2_to_f16x2(lo0 & 0xffffu), e4m3x2_to_f16x2(lo1 & 0xffffu));
-          mma_f16_16816(o[4 * w + 1], a, e4m3x2_to_f16x2(lo0 >> 16), e4m3x2_to_f16x2(lo1 >> 16));
-          mma_f16_16816(o[4 * w + 2], a, e4m3x2_to_f16x2(hi0 & 0xffffu), e4m3x2_to_f16x2(hi1 & 0xffffu));
-          mma_f16_16816(o[4 * w + 3], a, e4m3x2_to_f16x2(hi0 >> 16), e4m3x2_to_f16x2(hi1 >> 16));
+          for (int i = 0; i < 4; ++i) {
+            const int r = (i >> 1) * 8 + 2 * t4 + (i & 1);
+            v[i] = lds128(stage + L::K_BYTES + (16 * kk + r) * 128 + ((g ^ (r & 7)) << 4));
+            if (16 * kk + r >= live) v[i] = make_uint4(0, 0, 0, 0);   // whatever lies there (NaN codes too) counts for nothing
+          }
+          if (kk == 1) {
+            __syncwarp();
+            ++used;
+            issue();
+          }
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t v0 = w == 0 ? v[0].x : w == 1 ? v[0].y : w == 2 ? v[0].z : v[0].w;
+            const uint32_t v1 = w == 0 ? v[1].x : w == 1 ? v[1].y : w == 2 ? v[1].z : v[1].w;
+            const uint32_t v2 = w == 0 ? v[2].x : w == 1 ? v[2].y : w == 2 ? v[2].z : v[2].w;
+            const uint32_t v3 = w == 0 ? v[3].x : w == 1 ? v[3].y : w == 2 ? v[3].z : v[3].w;
+            const uint32_t lo0 = __byte_perm(v0, v1, 0x5140), hi0 = __byte_perm(v0, v1, 0x7362);
+            const uint32_t lo1 = __byte_perm(v2, v3, 0x5140), hi1 = __byte_perm(v2, v3, 0x7362);
+            mma_f16_16816(o[4 * w], a, e4m3x2_to_f16x2(lo0), e4m3x2_to_f16x2(lo1));
+            mma_f16_16816(o[4 * w + 1], a, e4m3x2_to_f16x2(lo0 >> 16), e4m3x2_to_f16x2(lo1 >> 16));
+            mma_f16_16816(o[4 * w + 2], a, e4m3x2_to_f16x2(hi0), e4m3x2_to_f16x2(hi1));
+            mma_f16_16816(o[4 * w + 3], a, e4m3x2_to_f16x2(hi0 >> 16), e4m3x2_to_f16x2(hi1 >> 16));
+          }
         }
       }
-      if (meta & 1) {
-        // The item, or the share, ends: the warps' results meet in shared memory.
-        float* wm = reinterpret_cast<float*>(smem + L::ML_OFF);
-        float* wl = wm + FEW_WARPS * FEW_QR;
-        float* buf = reinterpret_cast<float*>(smem + L::MERGE_OFF) + warp * FEW_QR * L::LD;
+    }
+    if (!last) continue;
+    fresh = true;
+    if constexpr (!WEIGHTS) {
+      // The item, or the share, ends: the warps' results meet in shared memory.
+      float* wm = reinterpret_cast<float*>(smem + L::ML_OFF);
+      float* wl = wm + FEW_WARPS * FEW_QR;
+      float* buf = reinterpret_cast<float*>(smem + L::MERGE_OFF) + warp * FEW_QR * L::LD;
+      const int b = u.e, h = u.h;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
-          l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-          const int r = g + 8 * half;
-          if (t4 == 0) {
-            wm[warp * FEW_QR + r] = m[half];
-            wl[warp * FEW_QR + r] = l[half];
-          }
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-              *reinterpret_cast<float4*>(buf + r * L::LD + 32 * t4 + 16 * c + i) =
-                  make_float4(o[i][2 * half + c], o[i + 1][2 * half + c], o[i + 2][2 * half + c], o[i + 3][2 * half + c]);
+      for (int half = 0; half < 2; ++half) {
+        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
+        l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
+        const int r = g + 8 * half;
+        if (t4 == 0) {
+          wm[warp * FEW_QR + r] = m[half];
+          wl[warp * FEW_QR + r] = l[half];
         }
-        __syncthreads();
-        const int qt = e - b * p.qts;
-        const int rows = min(FEW_QR, kv8_count(p.s, b) * p.group - qt * FEW_QR);
-        // Whole only when the share holds the item's first and last unit.
-        const int vis = Kv8Line<QR, FEW_TK>::visible(p, e);
-        const int n = max(1, (vis + FEW_TK - 1) / FEW_TK);
-        const bool ends = (k0 - warp * 16) / FEW_TK == n - 1;
-        const bool whole = began && ends;
-        float* part = p.part + static_cast<size_t>(2 * blockIdx.x + (began ? 1 : 0)) * kv8_part_floats<FEW_QR>();
-        const float* mbuf = reinterpret_cast<const float*>(smem + L::MERGE_OFF);
-        for (int i = threadIdx.x; i < rows * 32; i += FEW_THREADS) {
-          const int r = i >> 5, c4 = i & 31;
-          float M = -INFINITY;
 #pragma unroll
-          for (int w = 0; w < FEW_WARPS; ++w) M = fmaxf(M, wm[w * FEW_QR + r]);
-          float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-          float den = 0.f;
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int w = 0; w < FEW_WARPS; ++w) {
-            const float mw = wm[w * FEW_QR + r];
-            const float x = mw == -INFINITY ? 0.f : exp2f(mw - M);
-            const float4 v = *reinterpret_cast<const float4*>(mbuf + (w * FEW_QR + r) * L::LD + c4 * 4);
-            den += x * wl[w * FEW_QR + r];
-            acc.x += x * v.x;
-            acc.y += x * v.y;
-            acc.z += x * v.z;
-            acc.w += x * v.w;
-          }
-          const float mref = M == -INFINITY ? M : M - FEW_OFFSET;
-          if (!ok) den = 0.f;
-          if (whole) {
-            const int rr = qt * FEW_QR + r, t = rr / p.group, hq = h * p.group + rr - t * p.group;
-            const float inv = den == 0.f ? 0.f : 1.f / den;
-            *reinterpret_cast<uint2*>(p.out + b * p.o_sb + t * p.o_st + hq * p.o_sh + c4 * 4) =
-                make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-            if (p.lse != nullptr && c4 == 0)
-              p.lse[(static_cast<long long>(b) * p.s.tokens + t) * (p.c.heads * p.group) + hq] = kv8_row_lse(mref, den);
-          } else {
-            reinterpret_cast<float4*>(part + r * 128)[c4] = acc;
-            if (c4 == 0) {
-              part[FEW_QR * 128 + r] = mref;
-              part[FEW_QR * 129 + r] = den;
-            }
-          }
-        }
-        __syncthreads();
-        fresh = true;
-        began = true;
+          for (int i = 0; i < 16; i += 4)
+            *reinterpret_cast<float4*>(buf + r * L::LD + 32 * t4 + 16 * c + i) =
+                make_float4(o[i][2 * half + c], o[i + 1][2 * half + c], o[i + 2][2 * half + c], o[i + 3][2 * half + c]);
       }
+      __syncthreads();
+      const int rows = min(FEW_QR, kv8_count(p.s, b) * p.group);
+      // Whole only when the share holds the item's first and last unit.
+      const int n = max(1, (Kv8Line<FEW_QR, FEW_TK>::visible(p, b) + FEW_TK - 1) / FEW_TK);
+      const bool whole = began && (k0 - warp * FEW_KEYS) / FEW_TK == n - 1;
+      float* part = p.part + static_cast<size_t>(2 * blockIdx.x + (began ? 1 : 0)) * kv8_part_floats<FEW_QR>();
+      const float* mbuf = reinterpret_cast<const float*>(smem + L::MERGE_OFF);
+      for (int i = threadIdx.x; i < rows * 32; i += FEW_THREADS) {
+        const int r = i >> 5, c4 = i & 31;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < FEW_WARPS; ++w) M = fmaxf(M, wm[w * FEW_QR + r]);
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float den = 0.f;
+#pragma unroll
+        for (int w = 0; w < FEW_WARPS; ++w) {
+          const float mw = wm[w * FEW_QR + r];
+          const float x = mw == -INFINITY ? 0.f : exp2f(mw - M);
+          const float4 v = *reinterpret_cast<const float4*>(mbuf + (w * FEW_QR + r) * L::LD + c4 * 4);
+          den += x * wl[w * FEW_QR + r];
+          acc.x += x * v.x;
+          acc.y += x * v.y;
+          acc.z += x * v.z;
+          acc.w += x * v.w;
+        }
+        const float mref = M == -INFINITY ? M : M - FEW_OFFSET;
+        if (!ok) den = 0.f;
+        if (whole) {
+          const int t = r / p.group, hq = h * p.group + r - t * p.group;
+          const float inv = den == 0.f ? 0.f : 1.f / den;
+          *reinterpret_cast<uint2*>(p.out + b * p.o_sb + t * p.o_st + hq * p.o_sh + c4 * 4) =
+              make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+          if (p.lse != nullptr && c4 == 0)
+            p.lse[(static_cast<long long>(b) * p.s.tokens + t) * (p.c.heads * p.group) + hq] = kv8_row_lse(mref, den);
+        } else {
+          reinterpret_cast<float4*>(part + r * 128)[c4] = acc;
+          if (c4 == 0) {
+            part[FEW_QR * 128 + r] = mref;
+            part[FEW_QR * 129 + r] = den;
+          }
+        }
+      }
+      __syncthreads();
+      began = true;
     }
   }
 }

@@ -155,21 +155,22 @@ inline size_t kv8_part_bytes(bool few, const DeviceInfo& di) {
   const size_t floats = few ? kv8_few_ctas(di) * kv8_part_floats<FEW_QR>() : di.sms * kv8_part_floats<KTC_QR>();
   return (KV8_JOIN_BYTES + 2 * floats * sizeof(float) + 255) / 256 * 256;
 }
-inline size_t kv8_attn_workspace(const wamb_kv8_attention_args* a, const DeviceInfo& di) {
+inline size_t kv8_workspace(const wamb_kv8_attention_args* a, bool weights, const DeviceInfo& di) {
   const int64_t rows = kv8_rows(a);
   const bool few = kv8_is_few(rows);
-  return kv8_part_bytes(few, di) + (few ? 0 : kv8_split_q(a->seqs.batch, a->cache.heads, rows).bytes(false));
+  return (weights ? 0 : kv8_part_bytes(few, di)) +
+         (few ? 0 : kv8_split_q(a->seqs.batch, a->cache.heads, rows).bytes(weights));
 }
 // Splits the queries into `at`; returns the map of its rows and the factors.
 inline int kv8_split_launch(const Kv8AttnParams& p, const Kv8SplitQ& sq, uint8_t* at, bool weights, CUtensorMap* map,
-                            float** factor, float** lse2, cudaStream_t s) {
+                            float** factor, float** neg_lse2, cudaStream_t s) {
   WAMB_REQUIRE(sq.total <= INT32_MAX, WAMB_ERR_SHAPE, "kv8: %lld query rows", sq.total);
   *factor = reinterpret_cast<float*>(at + sq.total * 256);
-  *lse2 = weights ? *factor + sq.total : nullptr;
+  *neg_lse2 = weights ? *factor + sq.total : nullptr;
   int rc = make_tmap_2d(map, at, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, sq.total, 256, 256, 128, 128);
   if (rc) return rc;
   return launch_kernel(kv8_split_q_kernel, dim3(static_cast<unsigned>((sq.total + 31) / 32)), dim3(256), 0, s, p,
-                       sq.rows_pad, sq.total, at, *factor, *lse2);
+                       sq.rows_pad, sq.total, at, *factor, *neg_lse2);
 }
 
 template <typename K>
@@ -237,16 +238,18 @@ inline int kv8_attention_impl(const wamb_kv8_attention_args* a, bool weights, cu
   if (rc) return rc;
   WAMB_REQUIRE(kv8_few_ctas(di) <= static_cast<int>(KV8_JOIN_BYTES / sizeof(Kv8Join)), WAMB_ERR_DEVICE, "kv8: %d SMs",
                di.sms);
-  if (!weights) {
-    WAMB_REQUIRE(a->workspace && a->workspace_bytes >= kv8_attn_workspace(a, di), WAMB_ERR_WORKSPACE,
-                 "kv8 attention: workspace of %zu bytes, needs %zu", a->workspace_bytes, kv8_attn_workspace(a, di));
+  const size_t need = kv8_workspace(a, weights, di);
+  if (need > 0) {
+    WAMB_REQUIRE(a->workspace && a->workspace_bytes >= need, WAMB_ERR_WORKSPACE, "kv8: workspace of %zu bytes, needs %zu",
+                 a->workspace ? a->workspace_bytes : size_t{0}, need);
     WAMB_REQUIRE(reinterpret_cast<uintptr_t>(a->workspace) % 256 == 0, WAMB_ERR_ALIGN,
-                 "kv8 attention: workspace must be 256-byte aligned");
-    p.part = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + KV8_JOIN_BYTES);
+                 "kv8: workspace must be 256-byte aligned");
   }
+  uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  if (!weights) p.part = reinterpret_cast<float*>(ws + KV8_JOIN_BYTES);
   const uint64_t code_rows = static_cast<uint64_t>(p.c.pages) * p.c.heads * p.c.page;
   // Boxes of the TMA loads: the few-row kernel takes 16 keys, the other whole pages.
-  const uint32_t box = weights || few ? 16 : p.c.page;
+  const uint32_t box = few ? 16 : p.c.page;
   CUtensorMap tmK, tmV;
   rc = make_tmap_2d(&tmK, p.c.k8, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, code_rows, 128, 128, box, 128);
   if (rc) return rc;
@@ -254,29 +257,34 @@ inline int kv8_attention_impl(const wamb_kv8_attention_args* a, bool weights, cu
   if (rc) return rc;
   p.ctas = kv8_few_ctas(di);
   p.min_units = 1;
-  if (weights) {
+  if (weights && few) {
     static bool done[64] = {};
     rc = kv8_smem_once(kv8_few_kernel<true>, FewSmem<true>::TOTAL, done);
     if (rc) return rc;
-    return launch_kernel(kv8_few_kernel<true>, dim3(p.ctas), dim3(FEW_THREADS), FewSmem<true>::TOTAL, s, tmK, tmV, p,
-                         (rows + FEW_QR - 1) / FEW_QR);
+    return launch_kernel(kv8_few_kernel<true>, dim3(p.ctas), dim3(FEW_THREADS), FewSmem<true>::TOTAL, s, tmK, tmV, p);
   }
   if (few) {
     static bool done[64] = {};
     rc = kv8_smem_once(kv8_few_kernel<false>, FewSmem<false>::TOTAL, done);
     if (rc) return rc;
-    rc = launch_kernel(kv8_few_kernel<false>, dim3(p.ctas), dim3(FEW_THREADS), FewSmem<false>::TOTAL, s, tmK, tmV, p, 1);
+    rc = launch_kernel(kv8_few_kernel<false>, dim3(p.ctas), dim3(FEW_THREADS), FewSmem<false>::TOTAL, s, tmK, tmV, p);
     if (rc) return rc;
     if (cap <= FEW_TK) return WAMB_OK;   // one unit per item: nothing is ever shared
     return launch_kernel(kv8_merge_kernel<FEW_QR, 1>, dim3(p.ctas, rows), dim3(256), 0, s, p);
   }
   p.ctas = di.sms;
   CUtensorMap tmQ;
-  float *factor = nullptr, *unused = nullptr;
+  float *factor = nullptr, *neg_lse2 = nullptr;
   const Kv8SplitQ sq = kv8_split_q(p.s.batch, p.c.heads, rows);
-  rc = kv8_split_launch(p, sq, static_cast<uint8_t*>(a->workspace) + kv8_part_bytes(false, di), false, &tmQ, &factor,
-                        &unused, s);
+  rc = kv8_split_launch(p, sq, weights ? ws : ws + kv8_part_bytes(false, di), weights, &tmQ, &factor, &neg_lse2, s);
   if (rc) return rc;
+  if (weights) {
+    static bool done[64] = {};
+    rc = kv8_smem_once(kv8_weights_tc_kernel, KwtSmem::TOTAL, done);
+    if (rc) return rc;
+    return launch_kernel(kv8_weights_tc_kernel, dim3(p.ctas), dim3(KWT_THREADS), KwtSmem::TOTAL, s, tmK, tmQ,
+                         static_cast<const float*>(factor), static_cast<const float*>(neg_lse2), sq.rows_pad, p);
+  }
   static bool done[64] = {};
   rc = kv8_smem_once(kv8_tc_kernel, KtcSmem::TOTAL, done);
   if (rc) return rc;

@@ -30,6 +30,7 @@
 // TMEM columns: S/P of A [0,128), of B [128,256), O_A [256,384), O_B [384,512).
 #pragma once
 #include "attention.cuh"
+#include "glue.cuh"
 #include "kv8_few.cuh"
 #include <type_traits>
 
@@ -75,6 +76,20 @@ WAMB_DEV void ktc_issue_s(uint32_t d, uint32_t q, uint32_t k) {
         "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %4, p;\n\t}" ::"r"(d),
         "r"(qd + (i >> 2) * (KTC_TILE8 >> 4) + (i & 3) * 2), "r"(kd + (i & 3) * 2), "n"(KTC_DESC_HI), "n"(IDESC),
+        "r"(i > 0 ? 1u : 0u)
+        : "memory");
+}
+// S^T [128 keys][128 rows] = K (hi + lo)^T.
+WAMB_DEV void ktc_issue_st(uint32_t d, uint32_t k, uint32_t q) {
+  constexpr uint32_t IDESC = idesc_e4m3(128, 128);
+  const uint32_t qd = ktc_desc_lo(q, 16), kd = ktc_desc_lo(k, 16);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %4, p;\n\t}" ::"r"(d),
+        "r"(kd + (i & 3) * 2), "r"(qd + (i >> 2) * (KTC_TILE8 >> 4) + (i & 3) * 2), "n"(KTC_DESC_HI), "n"(IDESC),
         "r"(i > 0 ? 1u : 0u)
         : "memory");
 }
@@ -143,11 +158,11 @@ WAMB_DEV uint64_t ex2_poly5(uint64_t x2) {
 // The queries in two E4M3 pieces, for the tensor-core kernels: row
 // (b * heads + h) * rows_pad + r of q8 [., 256] holds hi (128 codes) and lo of
 // row r of (sequence b, cached head h), rf its factor 2^n * scale * log2(e);
-// rows past the sequence's are zeros. With lse2 (weights): lse2 = lse *
-// log2(e), +inf for rows that add nothing. A warp per row, four rows at once;
+// rows past the sequence's are zeros. With neg_lse2 (weights): -lse * log2(e),
+// -inf for rows that add nothing. A warp per row, four rows at once;
 // bound by memory (512 B a row) or by the launch.
 __global__ void __launch_bounds__(256) kv8_split_q_kernel(const Kv8AttnParams p, const int rows_pad, const long long total,
-                                                          uint8_t* q8, float* rf, float* lse2) {
+                                                          uint8_t* q8, float* rf, float* neg_lse2) {
   pdl_wait();
   constexpr int AT_ONCE = 4;
   const int lane = threadIdx.x & 31;
@@ -168,7 +183,7 @@ __global__ void __launch_bounds__(256) kv8_split_q_kernel(const Kv8AttnParams p,
       ok[i] = t < kv8_count(p.s, b);
       if (ok[i]) {
         w[i] = __ldg(reinterpret_cast<const uint2*>(p.q + b * p.q_sb + t * p.q_st + hq * p.q_sh) + lane);
-        if (lse2 != nullptr)
+        if (neg_lse2 != nullptr)
           z[i] = __ldg(p.lse_in + (static_cast<long long>(b) * p.s.tokens + t) * (p.c.heads * p.group) + hq);
       }
     }
@@ -181,35 +196,30 @@ __global__ void __launch_bounds__(256) kv8_split_q_kernel(const Kv8AttnParams p,
     float amax = fmaxf(fmaxf(fabsf(a.x), fabsf(a.y)), fmaxf(fabsf(b.x), fabsf(b.y)));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    // Scale exponent as for a cache block, over fp32's whole range.
-    const int bits = __float_as_int(fminf(amax, 3.402823466e38f));
-    const int n = max(-118, min(119, (bits >> 23) - 135 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0)));
-    // An infinite query makes its row NaN, as the formula does (a saturated one would not).
-    const float up = amax <= 3.402823466e38f ? pow2f_exact(-n) : __int_as_float(0x7fffffff);
+    int n;
+    const float up = query_scale(amax, n);
     const float x[4] = {a.x * up, a.y * up, b.x * up, b.y * up};
-    const uint32_t h0 = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t h1 = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
-    const float2 f0 = e4m3x2_to_float2(h0), f1 = e4m3x2_to_float2(h1);
-    const uint32_t l0 = __nv_cvt_float2_to_fp8x2(make_float2(x[0] - f0.x, x[1] - f0.y), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t l1 = __nv_cvt_float2_to_fp8x2(make_float2(x[2] - f1.x, x[3] - f1.y), __NV_SATFINITE, __NV_E4M3);
+    uint32_t hi, lo;
+    split_e4m3x4(x, hi, lo);
     uint32_t* dst = reinterpret_cast<uint32_t*>(q8 + row * 256) + lane;
-    dst[0] = h0 | (h1 << 16);
-    dst[32] = l0 | (l1 << 16);
+    dst[0] = hi;
+    dst[32] = lo;
     if (lane == 0) {
       rf[row] = pow2f_exact(n) * p.scale_log2;
-      if (lse2 != nullptr) lse2[row] = !ok[i] || z[i] == -INFINITY ? INFINITY : z[i] * 1.4426950408889634f;
+      if (neg_lse2 != nullptr) neg_lse2[row] = !ok[i] || z[i] == -INFINITY ? -INFINITY : z[i] * -1.4426950408889634f;
     }
   }
 }
 
 // One CTA's walk over the segments of its share.
+template <int QR>
 struct KtcWalk {
   Kv8Item it;
   long long u;
   WAMB_DEV bool done(const Kv8Share& sh) const { return u >= sh.u1; }
   WAMB_DEV void next(const Kv8AttnParams& p, const Kv8Share& sh) {
     u = min(sh.u1, it.start + it.n);
-    if (u < sh.u1) kv8_seek<KTC_QR, KTC_TK>(p, it, u);
+    if (u < sh.u1) kv8_seek<QR, KTC_TK>(p, it, u);
   }
 };
 struct KtcSeg {
@@ -218,7 +228,7 @@ struct KtcSeg {
   int vis;             // keys that the tile's last row sees
   bool two;            // two query halves (rows > 128)
   bool begins, ends;
-  WAMB_DEV KtcSeg(const Kv8AttnParams& p, const Kv8Share& sh, const KtcWalk& w) {
+  WAMB_DEV KtcSeg(const Kv8AttnParams& p, const Kv8Share& sh, const KtcWalk<KTC_QR>& w) {
     b = w.it.e / p.qts;
     qt = w.it.e - b * p.qts;
     rows = min(KTC_QR, Kv8Line<KTC_QR, KTC_TK>::rows(p, b) - qt * KTC_QR);
@@ -252,7 +262,7 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
 
   pdl_wait();
   Kv8Share sh;
-  KtcWalk walk;
+  KtcWalk<KTC_QR> walk;
   const bool work = kv8_share<KTC_QR, KTC_TK, KTC_THREADS>(p, blockIdx.x, sched, sh, walk.it);
   if (threadIdx.x == 0) kv8_leave_join(p, sh, work, walk.it);
   if (!work) return;
@@ -678,6 +688,280 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
           p.lse[(static_cast<long long>(sg.b) * p.s.tokens + tok) * (p.c.heads * p.group) + hq] = kv8_row_lse(mref, den);
         }
       }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ----------------------------------------------------------------- weights
+// Attention weights for more than a few query rows: S^T = K Q^T with the keys
+// in the lanes (M 128 keys, N 128 query rows), so that a thread owns a key
+// and adds up its column of exp(s - lse) with no exchange between threads; the
+// rows' factors and log-sum-exps come from shared memory, the same address for
+// a whole warp. Units are key tiles (all query rows of the sequence), cut
+// evenly over the CTAs; a unit's sums are complete, so there are no partials.
+// Bound by the exponentials: 128 x 128 of them take the SM 1024 cycles, the
+// products of the two query pieces 512.
+// 320 threads: warps 0-3 and 4-7 take the query tiles in turn (four score
+// buffers in TMEM), warp 8 loads, warp 9 issues the MMAs.
+constexpr int KWT_THREADS = 320, KWT_QS = 4, KWT_FS = 8, KWT_QR = 1 << 30;
+
+struct KwtSmem {
+  static constexpr uint32_t K_OFF = 0;                                     // 2 tiles of codes
+  static constexpr uint32_t Q_OFF = K_OFF + 2 * KTC_TILE8;                 // [4] hi, lo
+  static constexpr uint32_t F_OFF = Q_OFF + KWT_QS * 2 * KTC_TILE8;        // [8] factors, -lse2 of 128 rows
+  static constexpr uint32_t SC_OFF = F_OFF + KWT_FS * 1024;                // [8 units] ks of 8 groups of 16 keys
+  static constexpr uint32_t XCH_OFF = SC_OFF + 8 * 32;                     // sums of warps 4-7, [2] x 128
+  static constexpr uint32_t BAR_OFF = XCH_OFF + 2 * 128 * 4;
+  static constexpr uint32_t NBARS = 4 + 2 * KWT_QS + 8 + 1 + KWT_FS + 8;
+  static constexpr uint32_t SCHED_OFF = BAR_OFF + NBARS * 8;
+  static constexpr uint32_t TOTAL = 1024 + SCHED_OFF + sizeof(Kv8SchedSmem) + 16;
+  static_assert(TOTAL <= 232448, "shared memory exceeds 227 KB");
+};
+
+// Query tiles of one unit: [q0, q1) of 128 rows each.
+struct KwtUnit {
+  int b, h, k0, len, q0, q1, shift;   // row r sees key j when r >= group * (j - shift)
+  WAMB_DEV KwtUnit(const Kv8AttnParams& p, const KtcWalk<KWT_QR>& w) {
+    b = w.it.e;
+    h = w.it.h;
+    k0 = static_cast<int>(w.u - w.it.start) * KTC_TK;
+    len = kv8_len(p.s, p.c, b);
+    const int tokens = kv8_count(p.s, b);
+    shift = len - tokens;
+    q1 = (tokens * p.group + 127) / 128;
+    q0 = p.causal && k0 > shift ? static_cast<int>(min(static_cast<long long>(q1 - 1), static_cast<long long>(k0 - shift) * p.group / 128)) : 0;
+  }
+};
+// The walk goes unit by unit.
+WAMB_DEV void kwt_next(const Kv8AttnParams& p, const Kv8Share& sh, KtcWalk<KWT_QR>& w) {
+  if (++w.u < sh.u1) kv8_seek<KWT_QR, KTC_TK>(p, w.it, w.u);
+}
+
+__global__ void __launch_bounds__(KWT_THREADS, 1)
+    kv8_weights_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmQ,
+                          const float* q_factor, const float* q_neg_lse2, const int rows_pad, const Kv8AttnParams p) {
+  using L = KwtSmem;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const uint32_t base = smem_u32(smem);
+  const uint32_t sK = base + L::K_OFF, sQ = base + L::Q_OFF, sF = base + L::F_OFF;
+  uint32_t bar = base + L::BAR_OFF;
+  auto bars = [&](int n) { const uint32_t b = bar; bar += 8 * n; return b; };
+  const uint32_t k_full = bars(2), k_empty = bars(2), q_full = bars(KWT_QS), q_empty = bars(KWT_QS), s_full = bars(4),
+                 s_free = bars(4), drain = bars(1), f_full = bars(KWT_FS), sc_full = bars(8);
+  Kv8SchedSmem& sched = *reinterpret_cast<Kv8SchedSmem*>(smem + L::SCHED_OFF);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::SCHED_OFF + sizeof(Kv8SchedSmem));
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // warp: uniform
+
+  pdl_wait();
+  // Columns past a sequence's keys carry the base over.
+  if (p.weights != p.base)
+    for (int i = blockIdx.x; i < p.s.batch * p.c.heads; i += gridDim.x) {
+      const int b = i / p.c.heads;
+      const int seen = kv8_count(p.s, b) > 0 ? kv8_len(p.s, p.c, b) : 0;
+      for (long long j = seen + threadIdx.x; j < p.w_cap; j += KWT_THREADS)
+        p.weights[i * p.w_cap + j] = p.base != nullptr ? p.base[i * p.w_cap + j] : 0.f;
+    }
+  Kv8Share sh;
+  KtcWalk<KWT_QR> walk;
+  if (!kv8_share<KWT_QR, KTC_TK, KWT_THREADS>(p, blockIdx.x, sched, sh, walk.it)) return;
+  walk.u = sh.u0;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) { mbar_init(k_full + 8 * i, 1); mbar_init(k_empty + 8 * i, 1); }
+    for (int i = 0; i < KWT_QS; ++i) { mbar_init(q_full + 8 * i, 1); mbar_init(q_empty + 8 * i, 1); }
+    for (int i = 0; i < 4; ++i) { mbar_init(s_full + 8 * i, 1); mbar_init(s_free + 8 * i, 4); }
+    for (int i = 0; i < KWT_FS; ++i) mbar_init(f_full + 8 * i, 1);
+    for (int i = 0; i < 8; ++i) mbar_init(sc_full + 8 * i, 1);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(smem_u32(tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+  auto wait = [&](uint32_t b, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(b, parity, abort_flag)) != 0; };
+
+  if (warp == 8) {
+    // ---------------------------------------------------------- producer
+    // Lane i < 8 looks after keys [16 i, +16) of a unit, one unit ahead.
+    const int box_groups = p.c.page >> 4;
+    int units = 0, tiles = 0;
+    bool go = true;
+    struct Ahead { int row; float ks; };
+    auto look = [&](const KtcWalk<KWT_QR>& w) {
+      Ahead a{-1, 1.f};
+      const KwtUnit n(p, w);
+      const int key = n.k0 + lane * 16;
+      if (lane < 8 && key < n.len) {
+        const int pid = max(0, kv8_page(p.s.table, p.s.width, p.c, n.b, key >> p.c.page_log2));   // a bad id is reported
+        const long long blk = static_cast<long long>(pid) * p.c.heads + n.h;
+        a.row = static_cast<int>((blk << p.c.page_log2) + (key & (p.c.page - 1)));
+        a.ks = __ldg(p.c.k_scale + blk);
+      }
+      return a;
+    };
+    Ahead now = look(walk);
+    while (go && !walk.done(sh)) {
+      const KwtUnit n(p, walk);
+      kwt_next(p, sh, walk);
+      Ahead next{-1, 1.f};
+      if (!walk.done(sh)) next = look(walk);
+      const int ks = units & 1;
+      go = wait(k_empty + 8 * ks, ((units >> 1) & 1) ^ 1);
+      if (!go) break;
+      if (lane < 8) reinterpret_cast<float*>(smem + L::SC_OFF)[(units & 7) * 8 + lane] = now.ks;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(sc_full + 8 * (units & 7));
+      const bool lead = now.row >= 0 && lane % box_groups == 0;
+      const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, lead)) * (p.c.page * 128);
+      __syncwarp();
+      if (lane == 0) mbar_arrive_expect_tx(k_full + 8 * ks, bytes);
+      __syncwarp();
+      if (lead) tma_load_2d(sK + ks * KTC_TILE8 + lane * 2048, &tmK, k_full + 8 * ks, 0, now.row);
+      ++units;
+      for (int qt = n.q0; qt < n.q1; ++qt, ++tiles) {
+        const int qs = tiles % KWT_QS;
+        go = wait(q_empty + 8 * qs, ((tiles / KWT_QS) & 1) ^ 1);
+        if (!go) break;
+        if (lane == 0) {
+          const int row = (n.b * p.c.heads + n.h) * rows_pad + qt * 128;
+          const uint32_t at = sQ + qs * 2 * KTC_TILE8, f = sF + (tiles % KWT_FS) * 1024;
+          mbar_arrive_expect_tx(q_full + 8 * qs, 2 * KTC_TILE8);
+          tma_load_2d(at, &tmQ, q_full + 8 * qs, 0, row);
+          tma_load_2d(at + KTC_TILE8, &tmQ, q_full + 8 * qs, 128, row);
+          // The factors live in a ring of eight with barriers of their own: the
+          // exponentials may be four tiles behind the MMAs, when the query slot
+          // has gone through another phase.
+          const uint32_t fb = f_full + 8 * (tiles % KWT_FS);
+          mbar_arrive_expect_tx(fb, 1024);
+          bulk_load(f, q_factor + row, 512, fb);
+          bulk_load(f + 512, q_neg_lse2 + row, 512, fb);
+        }
+        __syncwarp();
+      }
+      now = next;
+    }
+    // Loads still in flight must land before the CTA exits.
+    if (lane == 0 && go) {
+      for (int t = max(0, units - 2); t < units; ++t) mbar_wait_teardown(k_full + 8 * (t & 1), (t >> 1) & 1);
+      for (int t = max(0, tiles - KWT_QS); t < tiles; ++t) {
+        mbar_wait_teardown(q_full + 8 * (t % KWT_QS), (t / KWT_QS) & 1);
+        mbar_wait_teardown(f_full + 8 * (t % KWT_FS), (t / KWT_FS) & 1);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 9) {
+    // --------------------------------------------------------- MMA issuer
+    const bool issuer = elect_one();
+    uint32_t units = 0, tiles = 0;
+    bool ok = true;
+    for (; ok && !walk.done(sh); kwt_next(p, sh, walk), ++units) {
+      const KwtUnit n(p, walk);
+      const int nq = __shfl_sync(0xffffffffu, n.q1 - n.q0, 0);
+      const uint32_t ks = units & 1;
+      ok = wait(k_full + 8 * ks, (units >> 1) & 1);
+      for (int i = 0; ok && i < nq; ++i, ++tiles) {
+        const uint32_t qs = tiles % KWT_QS, sb = tiles & 3;
+        ok = wait(q_full + 8 * qs, (tiles / KWT_QS) & 1) && wait(s_free + 8 * sb, ((tiles >> 2) & 1) ^ 1);
+        if (!ok) break;
+        tc_fence_after();
+        if (issuer) {
+          // Keys are the rows here, the two query pieces the columns.
+          ktc_issue_st(tmem + sb * 128, sK + ks * KTC_TILE8, sQ + qs * 2 * KTC_TILE8);
+          umma_commit(s_full + 8 * sb);
+          umma_commit(q_empty + 8 * qs);
+          if (i == nq - 1) umma_commit(k_empty + 8 * ks);
+        }
+        __syncwarp();
+      }
+    }
+    if (issuer) {
+      umma_commit(drain);
+      mbar_wait_teardown(drain, 0);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------- exponentials
+    const int grp = warp >> 2;
+    const int r = (warp & 3) * 32 + lane;     // key within the tile == TMEM lane
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    int units = 0, tiles = 0, joins = 0;
+    bool ok = true;     // once false, the loop goes on without waiting (the groups' barrier counts on all)
+    for (; !walk.done(sh); kwt_next(p, sh, walk), ++units) {
+      const KwtUnit n(p, walk);
+      const int nq = n.q1 - n.q0, key = n.k0 + r;
+      const bool mine = nq >= 2 ? grp == 0 : (tiles & 1) == grp;   // this group writes the unit's sums
+      const long long at = (static_cast<long long>(n.b) * p.c.heads + n.h) * p.w_cap + key;
+      float from = 0.f;
+      if (mine && key < n.len && p.base != nullptr) from = __ldcg(p.base + at);
+      float sum = 0.f;
+      if (nq >= 2 || mine) {
+        ok = ok && wait(sc_full + 8 * (units & 7), (units >> 3) & 1);
+        const float ks = reinterpret_cast<const float*>(smem + L::SC_OFF)[(units & 7) * 8 + (r >> 4)];
+        const uint64_t ks2 = f2(ks, ks);
+        const long long first = p.causal ? static_cast<long long>(key - n.shift) * p.group : 0;   // first row that sees the key
+        uint64_t acc[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+        for (int qt = n.q0, i = tiles; ok && qt < n.q1; ++qt, ++i) {
+          if ((i & 1) != grp) continue;
+          const int sb = i & 3;
+          ok = wait(f_full + 8 * (i % KWT_FS), (i / KWT_FS) & 1);
+          ok = ok && wait(s_full + 8 * sb, (i >> 2) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t ts = tmem + lane_base + sb * 128;
+          const float4* f = reinterpret_cast<const float4*>(smem + L::F_OFF + (i % KWT_FS) * 1024);
+          const int lim = static_cast<int>(max(0ll, min(128ll, first - qt * 128ll)));   // rows below it do not see the key
+          const bool part = __any_sync(0xffffffffu, lim > 0);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float s[32];
+            tmem_ld32(ts + c * 32, s);
+            tmem_wait_ld();
+            if (c == 3) {   // the scores are in registers: the buffer is free
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(s_free + 8 * sb);
+            }
+            if (part) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k)
+                if (c * 32 + k < lim) s[k] = -INFINITY;
+            }
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float4 rf = f[c * 8 + k], nl = f[32 + c * 8 + k];
+#pragma unroll
+              for (int u = 0; u < 2; ++u) {
+                const uint64_t a = fmul2(f2(s[4 * k + 2 * u], s[4 * k + 2 * u + 1]), ks2);
+                const float2 x = f2_split(ffma2(a, u ? f2(rf.z, rf.w) : f2(rf.x, rf.y), u ? f2(nl.z, nl.w) : f2(nl.x, nl.y)));
+                acc[u] = fadd2(acc[u], f2(ex2_mufu(x.x), ex2_mufu(x.y)));
+              }
+            }
+          }
+        }
+        const float2 a0 = f2_split(acc[0]), a1 = f2_split(acc[1]);
+        sum = (a0.x + a0.y) + (a1.x + a1.y);
+      }
+      tiles += nq;
+      if (nq >= 2) {
+        float* xch = reinterpret_cast<float*>(smem + L::XCH_OFF) + (joins++ & 1) * 128;
+        if (grp == 1) xch[r] = sum;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (grp == 0) sum += xch[r];
+      }
+      if (mine && key < n.len) p.weights[at] = ok ? from + sum : 0.f;
     }
   }
   tc_fence_before();

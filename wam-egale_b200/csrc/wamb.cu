@@ -395,7 +395,13 @@ int wamb_kv8_write(const wamb_kv8_write_args* args, void* stream) {
 size_t wamb_kv8_attention_workspace_bytes(const wamb_kv8_attention_args* args) {
   wamb::DeviceInfo di;
   if (args == nullptr || wamb::device_info(&di) != WAMB_OK) return 0;
-  return wamb::kv8_attn_workspace(args, di);
+  return wamb::kv8_workspace(args, false, di);
+}
+
+size_t wamb_kv8_weights_workspace_bytes(const wamb_kv8_attention_args* args) {
+  wamb::DeviceInfo di;
+  if (args == nullptr || wamb::device_info(&di) != WAMB_OK) return 0;
+  return wamb::kv8_workspace(args, true, di);
 }
 
 int wamb_kv8_attention(const wamb_kv8_attention_args* args, void* stream) {

@@ -157,7 +157,7 @@ EXPORTED = (
     "wamb_draft_forward", "wamb_spec_scores", "wamb_spec_route", "wamb_spec_expand", "wamb_spec_commit",
     "wamb_cfg_combine",
     "wamb_kv8_write", "wamb_kv8_attention_workspace_bytes", "wamb_kv8_attention", "wamb_kv8_weights",
-    "wamb_kv8_evict",
+    "wamb_kv8_weights_workspace_bytes", "wamb_kv8_evict",
 )
 
 # Size of the fixed scratch array behind wamb_block_forward_noalloc.
@@ -220,6 +220,8 @@ def load():
     lib.wamb_kv8_attention_workspace_bytes.argtypes = [ctypes.POINTER(Kv8AttentionArgs)]
     lib.wamb_kv8_attention_workspace_bytes.restype = ctypes.c_size_t
     lib.wamb_kv8_attention.argtypes = [ctypes.POINTER(Kv8AttentionArgs), c_void_p]
+    lib.wamb_kv8_weights_workspace_bytes.argtypes = [ctypes.POINTER(Kv8AttentionArgs)]
+    lib.wamb_kv8_weights_workspace_bytes.restype = ctypes.c_size_t
     lib.wamb_kv8_weights.argtypes = [ctypes.POINTER(Kv8AttentionArgs), c_void_p]
     lib.wamb_kv8_evict.argtypes = [ctypes.POINTER(Kv8EvictArgs), c_void_p]
     if lib.wamb_abi_version() != ABI_VERSION:

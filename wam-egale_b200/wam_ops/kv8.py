@@ -88,13 +88,20 @@ class Kv8Cache:
                              f" on {self.device}")
         return t.data_ptr()
 
-    def _call(self, fn, args):
-        if torch.cuda.current_device() == self.device.index:
-            rc = fn(args, torch._C._cuda_getCurrentRawStream(self.device.index))
-        else:
+    def _call(self, fn, args, workspace_bytes=None):
+        """fn(args) on the current stream of the cache's device, with scratch
+        of its own from that stream's (or the captured graph's) pool."""
+        if torch.cuda.current_device() != self.device.index:
             with torch.cuda.device(self.device):
-                rc = fn(args, torch._C._cuda_getCurrentRawStream(self.device.index))
-        _lib.check(rc)
+                return self._call(fn, args, workspace_bytes)
+        if workspace_bytes is not None:
+            n = workspace_bytes(args)
+            if n:
+                ws = torch.empty(n, dtype=torch.uint8, device=self.device)
+                args.workspace, args.workspace_bytes = ws.data_ptr(), n
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(self.device.index))
+        if rc:
+            _lib.check(rc)
 
     # ---------------------------------------------------------- operators
     def write(self, k, v, table, lens, counts=None):
@@ -146,10 +153,7 @@ class Kv8Cache:
             lse = torch.empty(q.shape[:3], dtype=torch.float32, device=self.device)
         if lse is not None:
             a.lse = self._lse(lse, q)
-        n = self._lib.wamb_kv8_attention_workspace_bytes(a)
-        ws = torch.empty(n, dtype=torch.uint8, device=self.device)   # from the stream's (or the graph's) own pool
-        a.workspace, a.workspace_bytes = ws.data_ptr(), n
-        self._call(self._lib.wamb_kv8_attention, a)
+        self._call(self._lib.wamb_kv8_attention, a, self._lib.wamb_kv8_attention_workspace_bytes)
         return (out, lse) if return_lse else out
 
     def _lse(self, lse, q):
@@ -175,7 +179,7 @@ class Kv8Cache:
         if base is not None and base.shape != out.shape:
             raise ValueError("base and out must have one shape")
         a.weights_cap = out.shape[2]
-        self._call(self._lib.wamb_kv8_weights, a)
+        self._call(self._lib.wamb_kv8_weights, a, self._lib.wamb_kv8_weights_workspace_bytes)
         return out
 
     def evict(self, table, lens, weights, new_table, heavy, recent, max_len=None):
