@@ -9,12 +9,12 @@
 // r = token * group + head in group), so each cached byte is read once for
 // all of them. A warp takes 32 keys at a time, K and V codes (4 KB each) by
 // TMA into its own ring, with no barrier between warps until an item ends.
-// S = Q K^T takes the codes as they are (m16n8k32): a bf16 query has eight
-// significant bits, which are two E4M3 values of four, q 2^-n = hi + lo, so
-// S = (hi K^T + lo K^T) 2^n. n puts the row's largest magnitude into (224,
-// 448]; a value below 2^-10 of that keeps an absolute error of at most 2^-10
-// (2^-17 of the largest). For P V the codes become f16 in registers (E4M3 is a
-// subset of f16, nothing is rounded).
+// The codes become f16 in registers (E4M3 is a subset of f16, nothing is
+// rounded) and meet the queries in m16n8k16 products with fp32 sums. (The
+// E4M3 m16n8k32 form is no shortcut here: it took 1030 instructions a step
+// where this one takes about 450.) Queries go to f16 scaled per row by a power
+// of two that puts the largest magnitude into [2^13, 2^14), which keeps their
+// eight bits over 28 binades.
 //
 // The scales of a block enter the exponent: with y_ij = s_ij log2(e) +
 // log2(vs_j) the kernel sums P_ij = 2^(y_ij - M_i) against the codes, M_i a
@@ -160,6 +160,33 @@ WAMB_DEV bool kv8_share(const Kv8AttnParams& p, int cta, Kv8SchedSmem& sm, Kv8Sh
   it.n = Kv8Line<QR, TK>::units(p, it.e);
   kv8_seek<QR, TK>(p, it, sh.u0);
   return true;
+}
+
+// Weights past a sequence's keys carry the base over. Pieces of 2048 columns
+// go round the CTAs; a thread's 16 loads are in flight together.
+template <int THREADS>
+WAMB_DEV void kv8_carry_base(const Kv8AttnParams& p) {
+  if (p.weights == p.base) return;
+  constexpr int PIECE = 2048, EACH = (PIECE + THREADS - 1) / THREADS;
+  const long long pieces = (p.w_cap + PIECE - 1) / PIECE, all = pieces * p.s.batch * p.c.heads;
+  for (long long i = blockIdx.x; i < all; i += gridDim.x) {
+    const long long row = i / pieces;
+    const int b = static_cast<int>(row / p.c.heads);
+    const int seen = kv8_count(p.s, b) > 0 ? kv8_len(p.s, p.c, b) : 0;
+    const long long j0 = (i - row * pieces) * PIECE, j1 = min(p.w_cap, j0 + PIECE);
+    if (j1 <= seen) continue;
+    float v[EACH];
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) {
+      const long long j = j0 + u * THREADS + threadIdx.x;
+      v[u] = p.base != nullptr && j >= seen && j < j1 ? __ldcg(p.base + row * p.w_cap + j) : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) {
+      const long long j = j0 + u * THREADS + threadIdx.x;
+      if (j >= seen && j < j1) p.weights[row * p.w_cap + j] = v[u];
+    }
+  }
 }
 
 // Floats of a partial: O [QR][128] relative to the row's M, then M, l.
@@ -309,16 +336,10 @@ struct FewSmem {
   static_assert(sizeof(FewUnit) == 48 && 2 * (TOTAL + 1024) <= 233472, "two CTAs must fit an SM");
 };
 
-// fp32 += f16 x f16: 16 rows x 16 x 8; and E4M3 x E4M3: 16 rows x 32 x 8.
+// fp32 += f16 x f16: 16 rows x 16 x 8.
 WAMB_DEV void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-WAMB_DEV void mma_e4m3_16832(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -332,33 +353,13 @@ WAMB_DEV uint4 lds128(uint32_t a) {
   return v;
 }
 
-// Four values into their E4M3 code word `h` and the word of what it leaves.
-// A bf16 value has eight significant bits: two codes of four hold it.
-WAMB_DEV void split_e4m3x4(const float (&x)[4], uint32_t& h, uint32_t& l) {
-  const uint32_t h0 = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t h1 = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
-  const float2 f0 = e4m3x2_to_float2(h0), f1 = e4m3x2_to_float2(h1);
-  const uint32_t l0 = __nv_cvt_float2_to_fp8x2(make_float2(x[0] - f0.x, x[1] - f0.y), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t l1 = __nv_cvt_float2_to_fp8x2(make_float2(x[2] - f1.x, x[3] - f1.y), __NV_SATFINITE, __NV_E4M3);
-  h = h0 | (h1 << 16);
-  l = l0 | (l1 << 16);
-}
-// Exponent n and factor 2^-n that bring a query row's largest magnitude into
-// (224, 448]. An infinite query makes its row NaN, as the formula does (a
-// saturated one would not).
-WAMB_DEV float query_scale(float amax, int& n) {
-  const int bits = __float_as_int(fminf(amax, 3.402823466e38f));
-  n = max(-118, min(119, (bits >> 23) - 135 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0)));
-  return amax <= 3.402823466e38f ? pow2f_exact(-n) : __int_as_float(0x7fffffff);
-}
-
-// The 16 rows of an (entry, head) as E4M3 A operands of four 32-wide steps,
-// in two pieces. Thread t = lane & 3 holds dims 16 t .. 16 t + 15 in words 0-3
-// of a row and 64 + 16 t .. in words 4-7; step s takes words 2 s, 2 s + 1 (the
-// same order for queries and keys, so the sum over dims is the same).
+// The 16 rows of an (entry, head) as f16 A operands of eight 16-wide steps.
+// Thread t = lane & 3 holds dims 16 t .. 16 t + 15 in words 0-3 of a row and
+// 64 + 16 t .. in words 4-7; step w takes word w (the same order for queries
+// and keys, so the sum over dims is the same).
 struct FewQ {
-  uint32_t hi[4][4], lo[4][4];
-  float rf[2];        // row factor: 2^n * scale * log2(e); rows g, g + 8
+  uint32_t a[8][4];
+  float rf[2];        // row factor: (power-of-two row scale) * scale * log2(e); rows g, g + 8
   int seen[2];        // keys each row sees
 };
 
@@ -388,14 +389,14 @@ WAMB_DEV void few_load_q(const Kv8AttnParams& p, int e, int h, FewQ& f) {
     }
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    int n;
-    const float up = query_scale(amax, n);
+    const int ex = min(max(__float_as_int(amax) >> 23, 14), 254);
+    const float up = __int_as_float((267 - ex) << 23);
 #pragma unroll
     for (int w = 0; w < 8; ++w) {
-      const float y[4] = {x[w][0] * up, x[w][1] * up, x[w][2] * up, x[w][3] * up};
-      split_e4m3x4(y, f.hi[w >> 1][half + 2 * (w & 1)], f.lo[w >> 1][half + 2 * (w & 1)]);
+      f.a[w][half] = pack_f16(x[w][0] * up, x[w][1] * up);
+      f.a[w][2 + half] = pack_f16(x[w][2] * up, x[w][3] * up);
     }
-    f.rf[half] = pow2f_exact(n) * p.scale_log2;
+    f.rf[half] = __int_as_float((ex - 13) << 23) * p.scale_log2;
     f.seen[half] = !ok ? 0 : p.causal ? max(0, min(len, len - tokens + t + 1)) : len;
   }
 }
@@ -419,8 +420,8 @@ WAMB_DEV void few_scores(uint32_t stage, const FewQ& q, float (&s)[4][4]) {
     for (int i = 0; i < 4; ++i) s[j][i] = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {   // two chains of sums, half as long
-      mma_e4m3_16832(s[j], q.hi[k], w[2 * k], w[2 * k + 1]);
-      mma_e4m3_16832(r, q.lo[k], w[2 * k], w[2 * k + 1]);
+      mma_f16_16816(s[j], q.a[k], e4m3x2_to_f16x2(w[k]), e4m3x2_to_f16x2(w[k] >> 16));
+      mma_f16_16816(r, q.a[4 + k], e4m3x2_to_f16x2(w[4 + k]), e4m3x2_to_f16x2(w[4 + k] >> 16));
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[j][i] += r[i];
@@ -447,16 +448,7 @@ __global__ void __launch_bounds__(FEW_THREADS)
   if (threadIdx.x == 0) *abort_flag = 0;
   fence_barrier_init();
   pdl_wait();
-  if constexpr (WEIGHTS) {
-    // Columns past a sequence's keys carry the base over.
-    if (p.weights != p.base)
-      for (int i = blockIdx.x; i < p.s.batch * p.c.heads; i += gridDim.x) {
-        const int b = i / p.c.heads;
-        const int seen = kv8_count(p.s, b) > 0 ? kv8_len(p.s, p.c, b) : 0;
-        for (long long j = seen + threadIdx.x; j < p.w_cap; j += FEW_THREADS)
-          p.weights[i * p.w_cap + j] = p.base != nullptr ? p.base[i * p.w_cap + j] : 0.f;
-      }
-  }
+  if constexpr (WEIGHTS) kv8_carry_base<FEW_THREADS>(p);
   Kv8Share sh;
   Kv8Item it;
   const bool work = kv8_share<FEW_QR, FEW_TK, FEW_THREADS>(p, blockIdx.x, sched, sh, it);

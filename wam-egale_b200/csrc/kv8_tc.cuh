@@ -155,6 +155,26 @@ WAMB_DEV uint64_t ex2_poly5(uint64_t x2) {
             __int_as_float(__float_as_int(pv.y) + (__float_as_int(tv.y) << 23)));
 }
 
+// Four values into their E4M3 code word `h` and the word of what it leaves.
+// A bf16 value has eight significant bits: two codes of four hold it.
+WAMB_DEV void split_e4m3x4(const float (&x)[4], uint32_t& h, uint32_t& l) {
+  const uint32_t h0 = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t h1 = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
+  const float2 f0 = e4m3x2_to_float2(h0), f1 = e4m3x2_to_float2(h1);
+  const uint32_t l0 = __nv_cvt_float2_to_fp8x2(make_float2(x[0] - f0.x, x[1] - f0.y), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t l1 = __nv_cvt_float2_to_fp8x2(make_float2(x[2] - f1.x, x[3] - f1.y), __NV_SATFINITE, __NV_E4M3);
+  h = h0 | (h1 << 16);
+  l = l0 | (l1 << 16);
+}
+// Exponent n and factor 2^-n that bring a query row's largest magnitude into
+// (224, 448]. An infinite query makes its row NaN, as the formula does (a
+// saturated one would not).
+WAMB_DEV float query_scale(float amax, int& n) {
+  const int bits = __float_as_int(fminf(amax, 3.402823466e38f));
+  n = max(-118, min(119, (bits >> 23) - 135 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0)));
+  return amax <= 3.402823466e38f ? pow2f_exact(-n) : __int_as_float(0x7fffffff);
+}
+
 // The queries in two E4M3 pieces, for the tensor-core kernels: row
 // (b * heads + h) * rows_pad + r of q8 [., 256] holds hi (128 codes) and lo of
 // row r of (sequence b, cached head h), rf its factor 2^n * scale * log2(e);
@@ -761,14 +781,7 @@ __global__ void __launch_bounds__(KWT_THREADS, 1)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // warp: uniform
 
   pdl_wait();
-  // Columns past a sequence's keys carry the base over.
-  if (p.weights != p.base)
-    for (int i = blockIdx.x; i < p.s.batch * p.c.heads; i += gridDim.x) {
-      const int b = i / p.c.heads;
-      const int seen = kv8_count(p.s, b) > 0 ? kv8_len(p.s, p.c, b) : 0;
-      for (long long j = seen + threadIdx.x; j < p.w_cap; j += KWT_THREADS)
-        p.weights[i * p.w_cap + j] = p.base != nullptr ? p.base[i * p.w_cap + j] : 0.f;
-    }
+  kv8_carry_base<KWT_THREADS>(p);
   Kv8Share sh;
   KtcWalk<KWT_QR> walk;
   if (!kv8_share<KWT_QR, KTC_TK, KWT_THREADS>(p, blockIdx.x, sched, sh, walk.it)) return;
