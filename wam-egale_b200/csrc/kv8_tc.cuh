@@ -125,14 +125,11 @@ WAMB_DEV float max3_nan(float a, float b, float c) {
   return d;
 }
 
-// Pairs of every eight whose 2^x runs on the FMA pipe: the MUFU's 16 a cycle
-// alone would take 2048 cycles for 256 x 128 scores, as long as the products.
-constexpr int KTC_POLY = 0;
-
-// 2^x for a pair: x clamped to >= -125, x = n + f with |f| <= 1/2 by the
-// 1.5 * 2^23 shifter, 2^f by the polynomial of degree 5 with the smallest
-// largest relative error (Remez exchange; 1.6e-7 with fp32 coefficients,
-// recomputed by tests/test_host_exp2_poly5.py), n added to the exponent field.
+// 2^x for a pair on the FMA pipe: x clamped to >= -125 (NaN stays), x = n + f
+// with |f| <= 1/2 by the 1.5 * 2^23 shifter, 2^f by the polynomial of degree 5
+// with the smallest largest relative error (Remez exchange; 1.6e-7 with fp32
+// coefficients, recomputed by tests/test_host_exp2_poly5.py), times 2^n put
+// together from its exponent bits.
 constexpr float KTC_C0 = 1.0000001192092896f;
 constexpr float KTC_C1 = 0.6931469440460205f;
 constexpr float KTC_C2 = 0.24022120237350464f;
@@ -141,7 +138,7 @@ constexpr float KTC_C4 = 0.009675540961325169f;
 constexpr float KTC_C5 = 0.0013276472454890609f;
 WAMB_DEV uint64_t ex2_poly5(uint64_t x2) {
   const float2 xv = f2_split(x2);
-  const uint64_t x = f2(fmaxf(xv.x, -125.f), fmaxf(xv.y, -125.f));
+  const uint64_t x = f2(max3_nan(xv.x, -125.f, -125.f), max3_nan(xv.y, -125.f, -125.f));
   const uint64_t shifter = f2(12582912.f, 12582912.f);
   const uint64_t t = fadd2(x, shifter);
   const uint64_t f = fsub2(x, fsub2(t, shifter));
@@ -150,9 +147,9 @@ WAMB_DEV uint64_t ex2_poly5(uint64_t x2) {
   p = ffma2(p, f, f2(KTC_C2, KTC_C2));
   p = ffma2(p, f, f2(KTC_C1, KTC_C1));
   p = ffma2(p, f, f2(KTC_C0, KTC_C0));
-  const float2 pv = f2_split(p), tv = f2_split(t);
-  return f2(__int_as_float(__float_as_int(pv.x) + (__float_as_int(tv.x) << 23)),
-            __int_as_float(__float_as_int(pv.y) + (__float_as_int(tv.y) << 23)));
+  const float2 tv = f2_split(t);
+  return fmul2(p, f2(__int_as_float((__float_as_int(tv.x) << 23) + 0x3f800000),
+                     __int_as_float((__float_as_int(tv.y) << 23) + 0x3f800000)));
 }
 
 // Four values into their E4M3 code word `h` and the word of what it leaves.
@@ -593,17 +590,10 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const uint64_t x2 = ffma2(f2(s[32 * c + 16 * gq + 2 * k], s[32 * c + 16 * gq + 2 * k + 1]), f2s, c2s);
-              float2 e;
-              if (k < 8 - KTC_POLY) {
-                const float2 x = f2_split(x2);
-                e = make_float2(ex2_mufu(x.x), ex2_mufu(x.y));
-                sum2 = fadd2(sum2, f2(e.x, e.y));
-              } else {
-                const uint64_t e2 = ex2_poly5(x2);
-                sum2 = fadd2(sum2, e2);
-                e = f2_split(e2);
-              }
-              pk[8 * gq + k] = pack_f16(e.x, e.y);
+              const float2 x = f2_split(x2);
+              const float a = ex2_mufu(x.x), b = ex2_mufu(x.y);
+              sum2 = fadd2(sum2, f2(a, b));
+              pk[8 * gq + k] = pack_f16(a, b);
             }
             const float2 sv = f2_split(sum2);
             sums[2 * c + gq] = sv.x + sv.y;
@@ -636,7 +626,6 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
           sum = fmaf(sums[5], b.y, sum);
           sum = fmaf(sums[6], b.z, sum);
           sum = fmaf(sums[7], b.w, sum);
-          if (m_new == -INFINITY) sum = 0.f;   // no key seen yet (the polynomial's 2^-125 are no weights)
           l = fmaf(l, alpha, sum);
         }
         m = m_new;
@@ -725,43 +714,46 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
 // rows' factors and log-sum-exps come from shared memory, the same address for
 // a whole warp. Units are key tiles (all query rows of the sequence), cut
 // evenly over the CTAs; a unit's sums are complete, so there are no partials.
-// Bound by the exponentials: 128 x 128 of them take the SM 1024 cycles, the
-// products of the two query pieces 512.
-// 320 threads: warps 0-3 and 4-7 take the query tiles in turn (four score
-// buffers in TMEM), warp 8 loads, warp 9 issues the MMAs.
-constexpr int KWT_THREADS = 320, KWT_QS = 4, KWT_FS = 8, KWT_QR = 1 << 30;
+// Two neighbouring key tiles of a head go together: warps 0-3 take the first,
+// warps 4-7 the second, each with two score buffers in TMEM, and every query
+// tile that is loaded serves both.
+// Bound by the exponentials: 128 x 128 of them take the SM's MUFU 1024
+// cycles, the products of the two query pieces 512.
+// 320 threads: warps 0..7 exponentials, warp 8 loads, warp 9 issues the MMAs.
+constexpr int KWT_THREADS = 320, KWT_QS = 4, KWT_FS = 8, KWT_SCS = 16, KWT_QR = 1 << 30;
+constexpr int KWT_POLY = 2;      // pairs of every eight whose 2^x runs on the FMA pipe
 
 struct KwtSmem {
-  static constexpr uint32_t K_OFF = 0;                                     // 2 tiles of codes
-  static constexpr uint32_t Q_OFF = K_OFF + 2 * KTC_TILE8;                 // [4] hi, lo
+  static constexpr uint32_t K_OFF = 0;                                     // [2 pairs] 2 tiles of codes
+  static constexpr uint32_t Q_OFF = K_OFF + 4 * KTC_TILE8;                 // [4] hi, lo
   static constexpr uint32_t F_OFF = Q_OFF + KWT_QS * 2 * KTC_TILE8;        // [8] factors, -lse2 of 128 rows
-  static constexpr uint32_t SC_OFF = F_OFF + KWT_FS * 1024;                // [8 units] ks of 8 groups of 16 keys
-  static constexpr uint32_t XCH_OFF = SC_OFF + 8 * 32;                     // sums of warps 4-7, [2] x 128
-  static constexpr uint32_t BAR_OFF = XCH_OFF + 2 * 128 * 4;
-  static constexpr uint32_t NBARS = 4 + 2 * KWT_QS + 8 + 1 + KWT_FS + 8;
+  static constexpr uint32_t SC_OFF = F_OFF + KWT_FS * 1024;                // [16 pairs] ks of 16 groups of 16 keys
+  static constexpr uint32_t BAR_OFF = SC_OFF + KWT_SCS * 64;
+  static constexpr uint32_t NBARS = 4 + 2 * KWT_QS + 2 * KWT_FS + 8 + 1;
   static constexpr uint32_t SCHED_OFF = BAR_OFF + NBARS * 8;
   static constexpr uint32_t TOTAL = 1024 + SCHED_OFF + sizeof(Kv8SchedSmem) + 16;
   static_assert(TOTAL <= 232448, "shared memory exceeds 227 KB");
 };
 
-// Query tiles of one unit: [q0, q1) of 128 rows each.
-struct KwtUnit {
-  int b, h, k0, len, q0, q1, shift;   // row r sees key j when r >= group * (j - shift)
-  WAMB_DEV KwtUnit(const Kv8AttnParams& p, const KtcWalk<KWT_QR>& w) {
+// One or two neighbouring key tiles, and their query tiles [q0, q1).
+struct KwtPair {
+  int b, h, k0, len, cnt, q0, q1, shift;   // row r sees key j when r >= group * (j - shift)
+  WAMB_DEV KwtPair(const Kv8AttnParams& p, const Kv8Share& sh, const KtcWalk<KWT_QR>& w) {
     b = w.it.e;
     h = w.it.h;
     k0 = static_cast<int>(w.u - w.it.start) * KTC_TK;
+    cnt = static_cast<int>(min(2ll, min(sh.u1, w.it.start + w.it.n) - w.u));
     len = kv8_len(p.s, p.c, b);
     const int tokens = kv8_count(p.s, b);
     shift = len - tokens;
     q1 = (tokens * p.group + 127) / 128;
-    q0 = p.causal && k0 > shift ? static_cast<int>(min(static_cast<long long>(q1 - 1), static_cast<long long>(k0 - shift) * p.group / 128)) : 0;
+    q0 = p.causal && k0 > shift ? static_cast<int>(min(q1 - 1ll, static_cast<long long>(k0 - shift) * p.group / 128)) : 0;
+  }
+  WAMB_DEV void next(const Kv8AttnParams& p, const Kv8Share& sh, KtcWalk<KWT_QR>& w) const {
+    w.u += cnt;
+    if (w.u < sh.u1) kv8_seek<KWT_QR, KTC_TK>(p, w.it, w.u);
   }
 };
-// The walk goes unit by unit.
-WAMB_DEV void kwt_next(const Kv8AttnParams& p, const Kv8Share& sh, KtcWalk<KWT_QR>& w) {
-  if (++w.u < sh.u1) kv8_seek<KWT_QR, KTC_TK>(p, w.it, w.u);
-}
 
 __global__ void __launch_bounds__(KWT_THREADS, 1)
     kv8_weights_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmQ,
@@ -773,8 +765,8 @@ __global__ void __launch_bounds__(KWT_THREADS, 1)
   const uint32_t sK = base + L::K_OFF, sQ = base + L::Q_OFF, sF = base + L::F_OFF;
   uint32_t bar = base + L::BAR_OFF;
   auto bars = [&](int n) { const uint32_t b = bar; bar += 8 * n; return b; };
-  const uint32_t k_full = bars(2), k_empty = bars(2), q_full = bars(KWT_QS), q_empty = bars(KWT_QS), s_full = bars(4),
-                 s_free = bars(4), drain = bars(1), f_full = bars(KWT_FS), sc_full = bars(8);
+  const uint32_t k_full = bars(2), k_empty = bars(2), q_full = bars(KWT_QS), q_empty = bars(KWT_QS),
+                 f_full = bars(KWT_FS), f_free = bars(KWT_FS), s_full = bars(4), s_free = bars(4), drain = bars(1);
   Kv8SchedSmem& sched = *reinterpret_cast<Kv8SchedSmem*>(smem + L::SCHED_OFF);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::SCHED_OFF + sizeof(Kv8SchedSmem));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -789,9 +781,8 @@ __global__ void __launch_bounds__(KWT_THREADS, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) { mbar_init(k_full + 8 * i, 1); mbar_init(k_empty + 8 * i, 1); }
     for (int i = 0; i < KWT_QS; ++i) { mbar_init(q_full + 8 * i, 1); mbar_init(q_empty + 8 * i, 1); }
+    for (int i = 0; i < KWT_FS; ++i) { mbar_init(f_full + 8 * i, 1); mbar_init(f_free + 8 * i, 8); }
     for (int i = 0; i < 4; ++i) { mbar_init(s_full + 8 * i, 1); mbar_init(s_free + 8 * i, 4); }
-    for (int i = 0; i < KWT_FS; ++i) mbar_init(f_full + 8 * i, 1);
-    for (int i = 0; i < 8; ++i) mbar_init(sc_full + 8 * i, 1);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_barrier_init();
@@ -808,16 +799,15 @@ __global__ void __launch_bounds__(KWT_THREADS, 1)
 
   if (warp == 8) {
     // ---------------------------------------------------------- producer
-    // Lane i < 8 looks after keys [16 i, +16) of a unit, one unit ahead.
+    // Lane i < 16 looks after keys [16 i, +16) of a pair, one pair ahead.
     const int box_groups = p.c.page >> 4;
-    int units = 0, tiles = 0;
+    int pairs = 0, tiles = 0;
     bool go = true;
     struct Ahead { int row; float ks; };
-    auto look = [&](const KtcWalk<KWT_QR>& w) {
+    auto look = [&](const KwtPair& n) {
       Ahead a{-1, 1.f};
-      const KwtUnit n(p, w);
       const int key = n.k0 + lane * 16;
-      if (lane < 8 && key < n.len) {
+      if (lane < 8 * n.cnt && key < n.len) {
         const int pid = max(0, kv8_page(p.s.table, p.s.width, p.c, n.b, key >> p.c.page_log2));   // a bad id is reported
         const long long blk = static_cast<long long>(pid) * p.c.heads + n.h;
         a.row = static_cast<int>((blk << p.c.page_log2) + (key & (p.c.page - 1)));
@@ -825,42 +815,38 @@ __global__ void __launch_bounds__(KWT_THREADS, 1)
       }
       return a;
     };
-    Ahead now = look(walk);
+    Ahead now = look(KwtPair(p, sh, walk));
     while (go && !walk.done(sh)) {
-      const KwtUnit n(p, walk);
-      kwt_next(p, sh, walk);
+      const KwtPair n(p, sh, walk);
+      n.next(p, sh, walk);
       Ahead next{-1, 1.f};
-      if (!walk.done(sh)) next = look(walk);
-      const int ks = units & 1;
-      go = wait(k_empty + 8 * ks, ((units >> 1) & 1) ^ 1);
+      if (!walk.done(sh)) next = look(KwtPair(p, sh, walk));
+      const int ks = pairs & 1;
+      go = wait(k_empty + 8 * ks, ((pairs >> 1) & 1) ^ 1);
       if (!go) break;
-      if (lane < 8) reinterpret_cast<float*>(smem + L::SC_OFF)[(units & 7) * 8 + lane] = now.ks;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(sc_full + 8 * (units & 7));
+      // The pair's scales are published with the factors of its first query
+      // tile; sixteen pairs on, the factor ring has long seen them read.
+      if (lane < 16) reinterpret_cast<float*>(smem + L::SC_OFF)[(pairs % KWT_SCS) * 16 + lane] = now.ks;
       const bool lead = now.row >= 0 && lane % box_groups == 0;
       const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, lead)) * (p.c.page * 128);
       __syncwarp();
       if (lane == 0) mbar_arrive_expect_tx(k_full + 8 * ks, bytes);
       __syncwarp();
-      if (lead) tma_load_2d(sK + ks * KTC_TILE8 + lane * 2048, &tmK, k_full + 8 * ks, 0, now.row);
-      ++units;
+      if (lead) tma_load_2d(sK + ks * 2 * KTC_TILE8 + lane * 2048, &tmK, k_full + 8 * ks, 0, now.row);
+      ++pairs;
       for (int qt = n.q0; qt < n.q1; ++qt, ++tiles) {
-        const int qs = tiles % KWT_QS;
-        go = wait(q_empty + 8 * qs, ((tiles / KWT_QS) & 1) ^ 1);
+        const int qs = tiles % KWT_QS, fs = tiles % KWT_FS;
+        go = wait(q_empty + 8 * qs, ((tiles / KWT_QS) & 1) ^ 1) && wait(f_free + 8 * fs, ((tiles / KWT_FS) & 1) ^ 1);
         if (!go) break;
         if (lane == 0) {
           const int row = (n.b * p.c.heads + n.h) * rows_pad + qt * 128;
-          const uint32_t at = sQ + qs * 2 * KTC_TILE8, f = sF + (tiles % KWT_FS) * 1024;
+          const uint32_t at = sQ + qs * 2 * KTC_TILE8, f = sF + fs * 1024;
           mbar_arrive_expect_tx(q_full + 8 * qs, 2 * KTC_TILE8);
           tma_load_2d(at, &tmQ, q_full + 8 * qs, 0, row);
           tma_load_2d(at + KTC_TILE8, &tmQ, q_full + 8 * qs, 128, row);
-          // The factors live in a ring of eight with barriers of their own: the
-          // exponentials may be four tiles behind the MMAs, when the query slot
-          // has gone through another phase.
-          const uint32_t fb = f_full + 8 * (tiles % KWT_FS);
-          mbar_arrive_expect_tx(fb, 1024);
-          bulk_load(f, q_factor + row, 512, fb);
-          bulk_load(f + 512, q_neg_lse2 + row, 512, fb);
+          mbar_arrive_expect_tx(f_full + 8 * fs, 1024);
+          bulk_load(f, q_factor + row, 512, f_full + 8 * fs);
+          bulk_load(f + 512, q_neg_lse2 + row, 512, f_full + 8 * fs);
         }
         __syncwarp();
       }
@@ -868,7 +854,7 @@ __global__ void __launch_bounds__(KWT_THREADS, 1)
     }
     // Loads still in flight must land before the CTA exits.
     if (lane == 0 && go) {
-      for (int t = max(0, units - 2); t < units; ++t) mbar_wait_teardown(k_full + 8 * (t & 1), (t >> 1) & 1);
+      for (int t = max(0, pairs - 2); t < pairs; ++t) mbar_wait_teardown(k_full + 8 * (t & 1), (t >> 1) & 1);
       for (int t = max(0, tiles - KWT_QS); t < tiles; ++t) {
         mbar_wait_teardown(q_full + 8 * (t % KWT_QS), (t / KWT_QS) & 1);
         mbar_wait_teardown(f_full + 8 * (t % KWT_FS), (t / KWT_FS) & 1);
@@ -878,27 +864,41 @@ __global__ void __launch_bounds__(KWT_THREADS, 1)
   } else if (warp == 9) {
     // --------------------------------------------------------- MMA issuer
     const bool issuer = elect_one();
-    uint32_t units = 0, tiles = 0;
+    uint32_t pairs = 0, tiles = 0, made[2] = {0, 0};   // score tiles made for each group
     bool ok = true;
-    for (; ok && !walk.done(sh); kwt_next(p, sh, walk), ++units) {
-      const KwtUnit n(p, walk);
+    while (ok && !walk.done(sh)) {
+      const KwtPair n(p, sh, walk);
       const int nq = __shfl_sync(0xffffffffu, n.q1 - n.q0, 0);
-      const uint32_t ks = units & 1;
-      ok = wait(k_full + 8 * ks, (units >> 1) & 1);
+      const bool both = __shfl_sync(0xffffffffu, n.cnt, 0) == 2;
+      const uint32_t kt = sK + (pairs & 1) * 2 * KTC_TILE8;
+      ok = wait(k_full + 8 * (pairs & 1), (pairs >> 1) & 1);
       for (int i = 0; ok && i < nq; ++i, ++tiles) {
-        const uint32_t qs = tiles % KWT_QS, sb = tiles & 3;
-        ok = wait(q_full + 8 * qs, (tiles / KWT_QS) & 1) && wait(s_free + 8 * sb, ((tiles >> 2) & 1) ^ 1);
+        const uint32_t qs = tiles % KWT_QS;
+        ok = wait(q_full + 8 * qs, (tiles / KWT_QS) & 1);
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          if (g == 1 && !both) break;
+          const uint32_t sb = 2 * g + (made[g] & 1);
+          ok = ok && wait(s_free + 8 * sb, ((made[g] >> 1) & 1) ^ 1);
+          if (!ok) break;
+          ++made[g];
+          tc_fence_after();
+          if (issuer) {
+            // Keys are the rows here, the two query pieces the columns.
+            ktc_issue_st(tmem + sb * 128, kt + g * KTC_TILE8, sQ + qs * 2 * KTC_TILE8);
+            umma_commit(s_full + 8 * sb);
+          }
+          __syncwarp();
+        }
         if (!ok) break;
-        tc_fence_after();
         if (issuer) {
-          // Keys are the rows here, the two query pieces the columns.
-          ktc_issue_st(tmem + sb * 128, sK + ks * KTC_TILE8, sQ + qs * 2 * KTC_TILE8);
-          umma_commit(s_full + 8 * sb);
           umma_commit(q_empty + 8 * qs);
-          if (i == nq - 1) umma_commit(k_empty + 8 * ks);
+          if (i == nq - 1) umma_commit(k_empty + 8 * (pairs & 1));
         }
         __syncwarp();
       }
+      n.next(p, sh, walk);
+      ++pairs;
     }
     if (issuer) {
       umma_commit(drain);
@@ -909,72 +909,88 @@ __global__ void __launch_bounds__(KWT_THREADS, 1)
     // ------------------------------------------------------- exponentials
     const int grp = warp >> 2;
     const int r = (warp & 3) * 32 + lane;     // key within the tile == TMEM lane
-    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    int units = 0, tiles = 0, joins = 0;
-    bool ok = true;     // once false, the loop goes on without waiting (the groups' barrier counts on all)
-    for (; !walk.done(sh); kwt_next(p, sh, walk), ++units) {
-      const KwtUnit n(p, walk);
-      const int nq = n.q1 - n.q0, key = n.k0 + r;
-      const bool mine = nq >= 2 ? grp == 0 : (tiles & 1) == grp;   // this group writes the unit's sums
+    const uint32_t tS = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + grp * 256;
+    int pairs = 0, tiles = 0;
+    uint32_t taken = 0;     // score tiles of this group
+    bool ok = true;         // once false, the loop goes on without waiting
+    for (; !walk.done(sh); ++pairs) {
+      const KwtPair n(p, sh, walk);
+      const bool active = grp < n.cnt;
+      const int key = n.k0 + grp * KTC_TK + r;
+      const bool store = active && key < n.len;
       const long long at = (static_cast<long long>(n.b) * p.c.heads + n.h) * p.w_cap + key;
-      float from = 0.f;
-      if (mine && key < n.len && p.base != nullptr) from = __ldcg(p.base + at);
-      float sum = 0.f;
-      if (nq >= 2 || mine) {
-        ok = ok && wait(sc_full + 8 * (units & 7), (units >> 3) & 1);
-        const float ks = reinterpret_cast<const float*>(smem + L::SC_OFF)[(units & 7) * 8 + (r >> 4)];
-        const uint64_t ks2 = f2(ks, ks);
-        const long long first = p.causal ? static_cast<long long>(key - n.shift) * p.group : 0;   // first row that sees the key
-        uint64_t acc[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
-        for (int qt = n.q0, i = tiles; ok && qt < n.q1; ++qt, ++i) {
-          if ((i & 1) != grp) continue;
-          const int sb = i & 3;
-          ok = wait(f_full + 8 * (i % KWT_FS), (i / KWT_FS) & 1);
-          ok = ok && wait(s_full + 8 * sb, (i >> 2) & 1);
-          if (!ok) break;
+      const float from = store && p.base != nullptr ? __ldcg(p.base + at) : 0.f;
+      const long long first = p.causal ? static_cast<long long>(key - n.shift) * p.group : 0;   // first row that sees the key
+      uint64_t ks2 = 0, acc[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+      for (int qt = n.q0; qt < n.q1; ++qt, ++tiles) {
+        const int fs = tiles % KWT_FS;
+        ok = ok && wait(f_full + 8 * fs, (tiles / KWT_FS) & 1);
+        if (active) {
+          if (qt == n.q0) {
+            const float ks = reinterpret_cast<const float*>(smem + L::SC_OFF)[(pairs % KWT_SCS) * 16 + grp * 8 + (r >> 4)];
+            ks2 = f2(ks, ks);
+          }
+          const uint32_t sb = 2 * grp + (taken & 1), ts = tS + (taken & 1) * 128;
+          ok = ok && wait(s_full + 8 * sb, (taken >> 1) & 1);
+          ++taken;
           tc_fence_after();
-          const uint32_t ts = tmem + lane_base + sb * 128;
-          const float4* f = reinterpret_cast<const float4*>(smem + L::F_OFF + (i % KWT_FS) * 1024);
+          const float4* f = reinterpret_cast<const float4*>(smem + L::F_OFF + fs * 1024);
           const int lim = static_cast<int>(max(0ll, min(128ll, first - qt * 128ll)));   // rows below it do not see the key
-          const bool part = __any_sync(0xffffffffu, lim > 0);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float s[32];
-            tmem_ld32(ts + c * 32, s);
-            tmem_wait_ld();
-            if (c == 3) {   // the scores are in registers: the buffer is free
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(s_free + 8 * sb);
-            }
-            if (part) {
+          if (__any_sync(0xffffffffu, lim > 0)) {
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              float x[32];
+              tmem_ld32(ts + c * 32, x);
+              tmem_wait_ld();
 #pragma unroll
               for (int k = 0; k < 32; ++k)
-                if (c * 32 + k < lim) s[k] = -INFINITY;
+                if (c * 32 + k < lim) x[k] = -INFINITY;
+              tmem_st32(ts + c * 32, x);
             }
+            tmem_wait_st();
+          }
+          float sA[32], sB[32];
+          auto add = [&](const float (&s)[32], int c) {
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
               const float4 rf = f[c * 8 + k], nl = f[32 + c * 8 + k];
 #pragma unroll
               for (int u = 0; u < 2; ++u) {
                 const uint64_t a = fmul2(f2(s[4 * k + 2 * u], s[4 * k + 2 * u + 1]), ks2);
-                const float2 x = f2_split(ffma2(a, u ? f2(rf.z, rf.w) : f2(rf.x, rf.y), u ? f2(nl.z, nl.w) : f2(nl.x, nl.y)));
-                acc[u] = fadd2(acc[u], f2(ex2_mufu(x.x), ex2_mufu(x.y)));
+                const uint64_t x2 = ffma2(a, u ? f2(rf.z, rf.w) : f2(rf.x, rf.y), u ? f2(nl.z, nl.w) : f2(nl.x, nl.y));
+                if (2 * (k & 3) + u >= 8 - KWT_POLY) {
+                  acc[u] = fadd2(acc[u], ex2_poly5(x2));
+                } else {
+                  const float2 x = f2_split(x2);
+                  acc[u] = fadd2(acc[u], f2(ex2_mufu(x.x), ex2_mufu(x.y)));
+                }
               }
             }
-          }
+          };
+          tmem_ld32(ts, sA);
+          tmem_wait_ld();
+          tmem_ld32(ts + 32, sB);
+          add(sA, 0);
+          tmem_wait_ld();
+          tmem_ld32(ts + 64, sA);
+          add(sB, 1);
+          tmem_wait_ld();
+          tmem_ld32(ts + 96, sB);
+          add(sA, 2);
+          tmem_wait_ld();
+          tc_fence_before();   // the scores are in registers: the buffer is free
+          __syncwarp();
+          if (lane == 0) mbar_arrive(s_free + 8 * sb);
+          add(sB, 3);
         }
-        const float2 a0 = f2_split(acc[0]), a1 = f2_split(acc[1]);
-        sum = (a0.x + a0.y) + (a1.x + a1.y);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(f_free + 8 * fs);
       }
-      tiles += nq;
-      if (nq >= 2) {
-        float* xch = reinterpret_cast<float*>(smem + L::XCH_OFF) + (joins++ & 1) * 128;
-        if (grp == 1) xch[r] = sum;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (grp == 0) sum += xch[r];
-      }
-      if (mine && key < n.len) p.weights[at] = ok ? from + sum : 0.f;
+      const float2 a0 = f2_split(acc[0]), a1 = f2_split(acc[1]);
+      const float sum = (a0.x + a0.y) + (a1.x + a1.y);
+      // The polynomial gives 2^-125 for a row that does not see the key.
+      if (store) p.weights[at] = ok ? from + (sum < 7.9e-31f ? 0.f : sum) : 0.f;
+      n.next(p, sh, walk);
     }
   }
   tc_fence_before();
