@@ -250,30 +250,58 @@ WAMB_DEV Kv8Kept kv8_kept(const Kv8EvictParams& p, int b) {
 }
 
 constexpr int KV8_SEL_THREADS = 1024, KV8_SEL_BINS = 2048, KV8_SEL_COPIES = 4;
+constexpr int KV8_SEL_KEYS = 40960;       // keys of one head that shared memory holds
+constexpr uint32_t KV8_SEL_SMEM = KV8_SEL_KEYS * 4;
 
 // One block per (head, sequence). The heavy-th largest key is found by a
 // radix select (11, 11 and 10 bits, histograms in shared memory: whole-number
 // counts, so the order of the atomics does not matter), then one ordered pass
 // writes the kept positions: keys above the threshold, and of those equal to
-// it the lowest positions. Reads the weights four times (from L2 after the
-// first); bound by that one SM's latency.
+// it the lowest positions. The weights are read once into shared memory, or
+// from L2 in each pass where a head has more than 40960; either way eight
+// loads of a thread are in flight. Bound by that one SM's latency. A sequence
+// whose new pages overlap its old ones is refused: it keeps nothing.
 __global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8EvictParams p) {
   pdl_wait();
+  extern __shared__ uint32_t keys[];
   __shared__ int hist[KV8_SEL_COPIES][KV8_SEL_BINS];
   __shared__ int wsum[32], pick[2];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int h = blockIdx.x, b = blockIdx.y;
-  const Kv8Kept k = kv8_kept(p, b);
+  Kv8Kept k = kv8_kept(p, b);
   const float* w = p.weights + (static_cast<long long>(b) * p.c.heads + h) * p.cap;
-  const long long out0 = (static_cast<long long>(b) * p.c.heads + h) * (static_cast<long long>(p.new_width) << p.c.page_log2);
   const long long out_cap = static_cast<long long>(p.new_width) << p.c.page_log2;
+  const long long out0 = (static_cast<long long>(b) * p.c.heads + h) * out_cap;
   int* kept = p.kept + out0;
   float* nw = p.new_weights + out0;
+
+  const int new_pages = (k.total + p.c.page - 1) >> p.c.page_log2, old_pages = (k.len + p.c.page - 1) >> p.c.page_log2;
+  bool overlap = false;
+  for (long long i = tid; i < static_cast<long long>(new_pages) * old_pages; i += KV8_SEL_THREADS) {
+    const int n = static_cast<int>(i / old_pages), o = static_cast<int>(i - static_cast<long long>(n) * old_pages);
+    overlap |= __ldg(p.new_table + static_cast<long long>(b) * p.new_width + n) ==
+               __ldg(p.s.table + static_cast<long long>(b) * p.s.width + o);
+  }
+  if (__syncthreads_or(overlap)) {
+    if (tid == 0) record_error(KV8_DEV_ERROR);
+    k.heavy = k.total = 0;
+  }
   if (h == 0 && tid == 0) p.new_lens[b] = k.total;
 
+  const bool held = k.old <= KV8_SEL_KEYS;     // the keys are in shared memory
+  const bool select = k.heavy < k.old && k.heavy > 0;
+  if (held && k.heavy > 0) {
+    for (int i0 = tid; i0 < k.old; i0 += 8 * KV8_SEL_THREADS) {
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = i0 + u * KV8_SEL_THREADS < k.old ? __ldg(w + i0 + u * KV8_SEL_THREADS) : 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (i0 + u * KV8_SEL_THREADS < k.old) keys[i0 + u * KV8_SEL_THREADS] = weight_key(v[u]);
+    }
+  }
   uint32_t prefix = 0, mask = 0;   // key bits fixed so far
   int need = k.heavy;              // places left among keys that match the prefix
-  const bool select = k.heavy < k.old && k.heavy > 0;
   if (select) {
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
@@ -281,9 +309,18 @@ __global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8Ev
       const int bits = pass == 2 ? 10 : 11;
       for (int i = tid; i < KV8_SEL_COPIES * KV8_SEL_BINS; i += KV8_SEL_THREADS) (&hist[0][0])[i] = 0;
       __syncthreads();
-      for (int i = tid; i < k.old; i += KV8_SEL_THREADS) {
-        const uint32_t key = weight_key(w[i]);
-        if ((key & mask) == prefix) atomicAdd(&hist[warp & (KV8_SEL_COPIES - 1)][(key >> shift) & ((1u << bits) - 1)], 1);
+      int* mine_hist = hist[warp & (KV8_SEL_COPIES - 1)];
+      for (int i0 = tid; i0 < k.old; i0 += 8 * KV8_SEL_THREADS) {
+        uint32_t key[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int i = i0 + u * KV8_SEL_THREADS;
+          key[u] = i >= k.old ? 0u : held ? keys[i] : weight_key(__ldg(w + i));
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (i0 + u * KV8_SEL_THREADS < k.old && (key[u] & mask) == prefix)
+            atomicAdd(mine_hist + ((key[u] >> shift) & ((1u << bits) - 1)), 1);
       }
       __syncthreads();
       // Each thread owns two bins, highest first: thread t has bins 2047 - 2t, 2046 - 2t.
@@ -321,38 +358,56 @@ __global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8Ev
       __syncthreads();
     }
   }
-  // Ordered compaction of [0, old): at most `need` keys equal to the threshold.
+  // Ordered compaction of [0, old), four neighbours to a thread: keys above the
+  // threshold and at most `need` of those equal to it.
   int done = 0, eq_done = 0;
   if (k.heavy > 0) {
-    for (int i0 = 0; i0 < k.old; i0 += KV8_SEL_THREADS) {
-      const int i = i0 + tid;
-      const float v = i < k.old ? w[i] : 0.f;
-      const uint32_t key = weight_key(v);
-      const bool gt = i < k.old && (!select || key > prefix);
-      const bool eq = i < k.old && select && key == prefix;
-      const unsigned mg = __ballot_sync(0xffffffffu, gt), me = __ballot_sync(0xffffffffu, eq);
-      if (lane == 0) wsum[warp] = __popc(mg) | (__popc(me) << 16);
-      __syncthreads();
-      const int mine = wsum[lane];
+    __syncthreads();
+    for (int i0 = 0; i0 < k.old; i0 += 4 * KV8_SEL_THREADS) {
+      const int i = i0 + 4 * tid;
+      uint32_t key[4];
+      int gt = 0, eq = 0;            // bit u: neighbour u
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        key[u] = 0;
+        if (i + u < k.old) {
+          key[u] = held ? keys[i + u] : weight_key(__ldg(w + i + u));
+          if (!select || key[u] > prefix) gt |= 1 << u;
+          else if (key[u] == prefix) eq |= 1 << u;
+        }
+      }
+      const int mine = __popc(gt) | (__popc(eq) << 16);
       int inc = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xffffffffu, inc, o);
         if (lane >= o) inc += u;
       }
-      const int before = __shfl_sync(0xffffffffu, inc - mine, warp);
-      const int all = __shfl_sync(0xffffffffu, inc, 31);
-      const unsigned below = (1u << lane) - 1;
-      // Equal keys before this one, and how many of them were taken.
-      const int eq_before = eq_done + (before >> 16) + __popc(me & below);
-      const int gt_before = done + (before & 0xffff) + __popc(mg & below);
-      if (gt || (eq && eq_before < need)) {
-        const int at = gt_before + min(eq_before, select ? need : 0);
-        kept[at] = i;
-        nw[at] = v;
+      if (lane == 31) wsum[warp] = inc;
+      __syncthreads();
+      int all = wsum[lane];
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, all, o);
+        if (lane >= o) all += u;
       }
-      done += all & 0xffff;
-      eq_done += all >> 16;
+      const int before = __shfl_sync(0xffffffffu, all, (warp + 31) & 31);
+      const int block = __shfl_sync(0xffffffffu, all, 31);
+      const int mine0 = inc - mine + (warp > 0 ? before : 0);
+      int at = done + (mine0 & 0xffff), e = eq_done + (mine0 >> 16);   // keys above, and equal, before these
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const bool is_eq = (eq >> u) & 1, take = ((gt >> u) & 1) || (is_eq && e < need);
+        if (take) {
+          const int to = at + min(e, select ? need : 0);
+          kept[to] = i + u;
+          nw[to] = __ldg(w + i + u);
+        }
+        at += (gt >> u) & 1;
+        e += is_eq;
+      }
+      done += block & 0xffff;
+      eq_done += block >> 16;
       __syncthreads();   // wsum is rewritten
     }
   }
@@ -360,80 +415,80 @@ __global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8Ev
     const bool live = j < k.total;
     const int pos = k.old + static_cast<int>(j - k.heavy);
     kept[j] = live ? pos : -1;
-    nw[j] = live ? w[pos] : 0.f;
+    nw[j] = live ? __ldg(w + pos) : 0.f;
   }
 }
 
-// One block per (new page, head, sequence, K or V): gathers the kept rows
-// into registers, takes the new scale from their values and rounds them once.
+// One block per (new page, head, sequence): gathers the kept rows of K and V
+// into registers, takes the new scales from their values and rounds them once.
+// kept lists the rows, -1 behind the last.
 template <int PAGE>
 __global__ void __launch_bounds__(256) kv8_gather_kernel(const Kv8EvictParams p) {
   pdl_wait();
   constexpr int PASSES = PAGE / 16;
-  __shared__ float red[8];
-  __shared__ int bad;
-  const int h = blockIdx.y, b = blockIdx.z >> 1, which = blockIdx.z & 1;
-  const int total = kv8_kept(p, b).total;
-  const int n = min(PAGE, total - static_cast<int>(blockIdx.x) * PAGE);
-  if (n <= 0) return;
-  const int dst = kv8_page(p.new_table, p.new_width, p.c, b, blockIdx.x);
-  if (dst < 0) return;
-  // A page of the old table cannot receive rows: others still read it.
-  if (threadIdx.x == 0) bad = 0;
-  __syncthreads();
-  const int old_pages = (__ldg(p.s.lens + b) + PAGE - 1) / PAGE;
-  for (int i = threadIdx.x; i < min(old_pages, p.s.width); i += 256)
-    if (__ldg(p.s.table + static_cast<long long>(b) * p.s.width + i) == dst) bad = 1;
-  __syncthreads();
-  if (bad) {
-    if (threadIdx.x == 0) record_error(KV8_DEV_ERROR);
-    return;
-  }
+  __shared__ float red[2][8];
+  const int h = blockIdx.y, b = blockIdx.z;
   const int c8 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
   const int* kept = p.kept + ((static_cast<long long>(b) * p.c.heads + h) * p.new_width + blockIdx.x) * PAGE;
-  const uint8_t* codes = which ? p.c.v8 : p.c.k8;
-  float* scales = which ? p.c.v_scale : p.c.k_scale;
-  uint2 raw[PASSES];
-  float sc[PASSES];
-  float amax = 0.f;
+  int pos[PASSES];
+#pragma unroll
+  for (int i = 0; i < PASSES; ++i) pos[i] = kept[r0 + 16 * i];
+  if (__syncthreads_and(pos[0] < 0)) return;   // the page receives nothing (row 0 is kept first)
+  const int dst = kv8_page(p.new_table, p.new_width, p.c, b, blockIdx.x);
+  if (dst < 0) return;
+  uint2 raw[2][PASSES];
+  float sc[2][PASSES];
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
-    const int r = r0 + 16 * i;
-    raw[i] = make_uint2(0, 0);
-    sc[i] = 0.f;
-    if (r < n) {
-      const int pos = kept[r];
-      const int pid = kv8_page(p.s.table, p.s.width, p.c, b, pos / PAGE);
+    raw[0][i] = raw[1][i] = make_uint2(0, 0);
+    sc[0][i] = sc[1][i] = 0.f;
+    if (pos[i] >= 0) {
+      const int pid = kv8_page(p.s.table, p.s.width, p.c, b, pos[i] / PAGE);
       if (pid >= 0) {
         const long long blk = static_cast<long long>(pid) * p.c.heads + h;
-        sc[i] = __ldg(scales + blk);
-        raw[i] = *reinterpret_cast<const uint2*>(codes + (blk * PAGE + pos % PAGE) * 128 + c8 * 8);
+        const long long at = (blk * PAGE + pos[i] % PAGE) * 128 + c8 * 8;
+        raw[0][i] = *reinterpret_cast<const uint2*>(p.c.k8 + at);
+        raw[1][i] = *reinterpret_cast<const uint2*>(p.c.v8 + at);
+        sc[0][i] = p.c.k_scale[blk];
+        sc[1][i] = p.c.v_scale[blk];
       }
     }
   }
+  float amax[2] = {0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    float f[8];
-    e4m3x8_to_float(raw[i], f);
+  for (int x = 0; x < 2; ++x) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(f[k]) * sc[i]);
+    for (int i = 0; i < PASSES; ++i) {
+      float f[8], m = 0.f;
+      e4m3x8_to_float(raw[x][i], f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(f[k]));
+      amax[x] = fmaxf(amax[x], m * sc[x][i]);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) amax[x] = fmaxf(amax[x], __shfl_xor_sync(0xffffffffu, amax[x], o));
+    if ((threadIdx.x & 31) == 0) red[x][threadIdx.x >> 5] = amax[x];
   }
-  amax = block_max_256(amax, red);
-  const float s = pow2f_exact(kv8_scale_exp(amax));
-  const float inv = 1.f / s;
+  __syncthreads();
   const long long blk = static_cast<long long>(dst) * p.c.heads + h;
-  uint8_t* to = (which ? p.c.v8 : p.c.k8) + blk * (PAGE * 128) + c8 * 8;
 #pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    const int r = r0 + 16 * i;
-    if (r >= n) continue;
-    float f[8];
-    e4m3x8_to_float(raw[i], f);
+  for (int x = 0; x < 2; ++x) {
+    float m = red[x][0];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] = f[k] * sc[i] * inv;
-    *reinterpret_cast<uint2*>(to + r * 128) = pack_e4m3x8(f);
+    for (int i = 1; i < 8; ++i) m = fmaxf(m, red[x][i]);
+    const float s = pow2f_exact(kv8_scale_exp(m)), inv = 1.f / s;
+    uint8_t* to = (x ? p.c.v8 : p.c.k8) + blk * (PAGE * 128) + c8 * 8;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      if (pos[i] < 0) continue;
+      float f[8];
+      e4m3x8_to_float(raw[x][i], f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] = f[k] * sc[x][i] * inv;
+      *reinterpret_cast<uint2*>(to + (r0 + 16 * i) * 128) = pack_e4m3x8(f);
+    }
+    if (threadIdx.x == 0) (x ? p.c.v_scale : p.c.k_scale)[blk] = s;
   }
-  if (threadIdx.x == 0) scales[blk] = s;
 }
 
 }  // namespace wamb

@@ -81,6 +81,17 @@ inline int kv8_write_impl(const wamb_kv8_write_args* a, cudaStream_t s) {
   return a->x_is_f32 ? kv8_write_launch<true>(p, grid, s) : kv8_write_launch<false>(p, grid, s);
 }
 
+template <typename K>
+inline int kv8_smem_once(K kern, int bytes, bool* done) {
+  int dev = 0;
+  WAMB_CHECK_CUDA(cudaGetDevice(&dev));
+  if (!done[dev]) {
+    WAMB_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    done[dev] = true;
+  }
+  return WAMB_OK;
+}
+
 inline int kv8_evict_impl(const wamb_kv8_evict_args* a, cudaStream_t s) {
   WAMB_REQUIRE(a != nullptr, WAMB_ERR_ARG, "null args");
   Kv8EvictParams p{};
@@ -115,9 +126,14 @@ inline int kv8_evict_impl(const wamb_kv8_evict_args* a, cudaStream_t s) {
   p.kept = a->kept;
   p.new_weights = a->new_weights;
   p.new_lens = a->new_lens;
-  rc = launch_kernel(kv8_select_kernel, dim3(p.c.heads, p.s.batch), dim3(KV8_SEL_THREADS), 0, s, p);
+  static bool done[64] = {};
+  rc = kv8_smem_once(kv8_select_kernel, KV8_SEL_SMEM, done);
   if (rc) return rc;
-  const dim3 grid(p.new_width, p.c.heads, 2 * p.s.batch);
+  // Shared memory for the keys that the tables can hold, so that short heads leave room for more blocks.
+  const int64_t hold = cap <= KV8_SEL_KEYS ? cap : KV8_SEL_KEYS;
+  rc = launch_kernel(kv8_select_kernel, dim3(p.c.heads, p.s.batch), dim3(KV8_SEL_THREADS), static_cast<size_t>(hold) * 4, s, p);
+  if (rc) return rc;
+  const dim3 grid(p.new_width, p.c.heads, p.s.batch);
   switch (p.c.page) {
     case 16: return launch_kernel(kv8_gather_kernel<16>, grid, dim3(256), 0, s, p);
     case 32: return launch_kernel(kv8_gather_kernel<32>, grid, dim3(256), 0, s, p);
@@ -171,17 +187,6 @@ inline int kv8_split_launch(const Kv8AttnParams& p, const Kv8SplitQ& sq, uint8_t
   if (rc) return rc;
   return launch_kernel(kv8_split_q_kernel, dim3(static_cast<unsigned>((sq.total + 31) / 32)), dim3(256), 0, s, p,
                        sq.rows_pad, sq.total, at, *factor, *neg_lse2);
-}
-
-template <typename K>
-inline int kv8_smem_once(K kern, int bytes, bool* done) {
-  int dev = 0;
-  WAMB_CHECK_CUDA(cudaGetDevice(&dev));
-  if (!done[dev]) {
-    WAMB_CHECK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    done[dev] = true;
-  }
-  return WAMB_OK;
 }
 
 inline int kv8_attention_impl(const wamb_kv8_attention_args* a, bool weights, cudaStream_t s) {
