@@ -499,3 +499,17 @@ def test_weights_many_tiles(cuda_device, B, H, G, T, L, causal):
     c, table, _, n, g = _setup(B, H, 64, [L - 300 * b for b in range(B)], T, poison=False)
     counts = _i32([T - 256 * b if T > 600 else T for b in range(B)])
     _check_weights(c, _q(g, B, T, H * G, 128), table, n, table.shape[1] * 64, counts=counts, causal=causal)
+
+
+@pytest.mark.parametrize("L,heavy,kind", [(9000, 700, "equal"), (40000, 12345, "random"), (40000, 3, "two"), (12000, 11999, "bin")])
+def test_evict_long_heads(cuda_device, L, heavy, kind):
+    """More keys than shared memory holds, than its list of one bin, and all keys equal."""
+    c, table, free, n, g = _setup(1, 1, 128, [L], heavy, spare=-(-(heavy + 5) // 128), poison=False)
+    w = torch.rand(1, 1, table.shape[1] * 128, generator=g)
+    if kind == "equal":
+        w.fill_(0.75)
+    elif kind == "two":
+        w = (w > 0.5).float()
+    elif kind == "bin":
+        w = 1.0 + w * 1e-4
+    _check_evict(c, table, free, n, w.to(DEV), heavy, 5)

@@ -250,23 +250,183 @@ WAMB_DEV Kv8Kept kv8_kept(const Kv8EvictParams& p, int b) {
 }
 
 constexpr int KV8_SEL_THREADS = 1024, KV8_SEL_BINS = 2048, KV8_SEL_COPIES = 4;
-constexpr int KV8_SEL_KEYS = 40960;       // keys of one head that shared memory holds
-constexpr uint32_t KV8_SEL_SMEM = KV8_SEL_KEYS * 4;
+constexpr int KV8_SEL_KEYS = 36864;       // keys of one head that shared memory holds
+constexpr int KV8_SEL_LIST = 8192;        // keys of one bin that it holds apart
+constexpr uint32_t KV8_SEL_SMEM = (KV8_SEL_KEYS + KV8_SEL_LIST) * 4;
+
+struct Kv8SelSmem {
+  int hist[KV8_SEL_COPIES][KV8_SEL_BINS];
+  int wsum[32], pick[2], listed;
+};
+
+// The bin, counted from the highest, that holds the `need`-th largest key of
+// the histogram, and how many of that bin are needed. Whole block.
+WAMB_DEV void kv8_pick_bin(Kv8SelSmem& sm, int need) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __syncthreads();
+  // Each thread owns two bins, highest first: thread t has bins 2047 - 2t, 2046 - 2t.
+  int c[2], mine = 0;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int bin = KV8_SEL_BINS - 1 - 2 * tid - j;
+    c[j] = 0;
+#pragma unroll
+    for (int q = 0; q < KV8_SEL_COPIES; ++q) c[j] += sm.hist[q][bin];
+    mine += c[j];
+  }
+  int inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  if (lane == 31) sm.wsum[warp] = inc;
+  __syncthreads();
+  int above = inc - mine;
+  for (int q = 0; q < warp; ++q) above += sm.wsum[q];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    if (above < need && need <= above + c[j]) {
+      sm.pick[0] = KV8_SEL_BINS - 1 - 2 * tid - j;
+      sm.pick[1] = need - above;
+    }
+    above += c[j];
+  }
+  __syncthreads();
+}
+WAMB_DEV void kv8_clear_hist(Kv8SelSmem& sm) {
+  for (int i = threadIdx.x; i < KV8_SEL_COPIES * KV8_SEL_BINS; i += KV8_SEL_THREADS) (&sm.hist[0][0])[i] = 0;
+  __syncthreads();
+}
+
+// Keeps k.heavy of the positions [0, k.old) and writes them, in order.
+// HELD: the keys fit shared memory.
+template <bool HELD>
+WAMB_DEV void kv8_select_heavy(const Kv8Kept& k, const float* w, Kv8SelSmem& sm, uint32_t* keys, uint32_t* list, int* kept,
+                               float* nw) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  auto key_at = [&](int i) { return HELD ? keys[i] : weight_key(__ldg(w + i)); };
+  const bool select = k.heavy < k.old;
+  int* hist = sm.hist[warp & (KV8_SEL_COPIES - 1)];
+  uint32_t prefix = 0;             // the threshold's bits fixed so far
+  int need = k.heavy;              // places left among keys that match them
+  if (select) kv8_clear_hist(sm);
+  if (HELD || select)
+    for (int i0 = tid; i0 < k.old; i0 += 8 * KV8_SEL_THREADS) {
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = i0 + u * KV8_SEL_THREADS < k.old ? __ldg(w + i0 + u * KV8_SEL_THREADS) : 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = i0 + u * KV8_SEL_THREADS;
+        if (i < k.old) {
+          const uint32_t key = weight_key(v[u]);
+          if (HELD) keys[i] = key;
+          if (select) atomicAdd(hist + (key >> 21), 1);
+        }
+      }
+    }
+  if (select) {
+    kv8_pick_bin(sm, need);
+    prefix = static_cast<uint32_t>(sm.pick[0]) << 21;
+    need = sm.pick[1];
+    // The bin's keys go to a list of their own: the two further digits look at
+    // them alone (at all keys again where the list overflows).
+    if (tid == 0) sm.listed = 0;
+    __syncthreads();
+    for (int i0 = tid; i0 < k.old; i0 += 8 * KV8_SEL_THREADS) {
+      uint32_t key[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) key[u] = i0 + u * KV8_SEL_THREADS < k.old ? key_at(i0 + u * KV8_SEL_THREADS) : ~prefix;
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if ((key[u] ^ prefix) >> 21 == 0) {
+          const int at = atomicAdd(&sm.listed, 1);
+          if (at < KV8_SEL_LIST) list[at] = key[u];
+        }
+    }
+    __syncthreads();
+    const bool short_list = sm.listed <= KV8_SEL_LIST;
+    const int n = short_list ? sm.listed : k.old;
+#pragma unroll 1
+    for (int pass = 1; pass < 3; ++pass) {
+      const int shift = pass == 1 ? 10 : 0, above = pass == 1 ? 21 : 10;
+      const uint32_t digit = pass == 1 ? 0x7ffu : 0x3ffu;
+      kv8_clear_hist(sm);
+      for (int i = tid; i < n; i += KV8_SEL_THREADS) {
+        const uint32_t key = short_list ? list[i] : key_at(i);
+        if ((key ^ prefix) >> above == 0) atomicAdd(hist + ((key >> shift) & digit), 1);
+      }
+      kv8_pick_bin(sm, need);
+      prefix |= static_cast<uint32_t>(sm.pick[0]) << shift;
+      need = sm.pick[1];
+      __syncthreads();
+    }
+  }
+  // Ordered compaction, four neighbours to a thread: keys above the threshold
+  // and, of those equal to it, the `need` lowest positions.
+  int done = 0, eq_done = 0;
+  __syncthreads();
+  for (int i0 = 0; i0 < k.old; i0 += 4 * KV8_SEL_THREADS) {
+    const int i = i0 + 4 * tid;
+    int gt = 0, eq = 0;            // bit u: neighbour u
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (i + u < k.old) {
+        const uint32_t key = select ? key_at(i + u) : 1u;
+        gt |= (!select || key > prefix) << u;
+        eq |= (select && key == prefix) << u;
+      }
+    const int mine = __popc(gt) | (__popc(eq) << 16);
+    int inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += u;
+    }
+    if (lane == 31) sm.wsum[warp] = inc;
+    __syncthreads();
+    int all = sm.wsum[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, all, o);
+      if (lane >= o) all += u;
+    }
+    const int before = __shfl_sync(0xffffffffu, all, (warp + 31) & 31);
+    const int block = __shfl_sync(0xffffffffu, all, 31);
+    const int mine0 = inc - mine + (warp > 0 ? before : 0);
+    int at = done + (mine0 & 0xffff), e = eq_done + (mine0 >> 16);   // keys above, and equal, before these
+    if (gt | eq) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const bool is_eq = (eq >> u) & 1, is_gt = (gt >> u) & 1;
+        if (is_gt || (is_eq && e < need)) {
+          const int to = at + min(e, select ? need : 0);
+          kept[to] = i + u;
+          nw[to] = __ldg(w + i + u);
+        }
+        at += is_gt;
+        e += is_eq;
+      }
+    }
+    done += block & 0xffff;
+    eq_done += block >> 16;
+    __syncthreads();   // wsum is rewritten
+  }
+}
 
 // One block per (head, sequence). The heavy-th largest key is found by a
 // radix select (11, 11 and 10 bits, histograms in shared memory: whole-number
 // counts, so the order of the atomics does not matter), then one ordered pass
-// writes the kept positions: keys above the threshold, and of those equal to
-// it the lowest positions. The weights are read once into shared memory, or
-// from L2 in each pass where a head has more than 40960; either way eight
-// loads of a thread are in flight. Bound by that one SM's latency. A sequence
-// whose new pages overlap its old ones is refused: it keeps nothing.
-__global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8EvictParams p) {
+// writes the kept positions. The weights are read once into shared memory, or
+// from L2 in each pass where a head has more than 36864; eight loads of a
+// thread are in flight. Bound by that one SM's instructions. A sequence whose
+// new pages overlap its old ones is refused: it keeps nothing.
+__global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8EvictParams p, const int list_at) {
   pdl_wait();
   extern __shared__ uint32_t keys[];
-  __shared__ int hist[KV8_SEL_COPIES][KV8_SEL_BINS];
-  __shared__ int wsum[32], pick[2];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ Kv8SelSmem sm;
+  const int tid = threadIdx.x;
   const int h = blockIdx.x, b = blockIdx.y;
   Kv8Kept k = kv8_kept(p, b);
   const float* w = p.weights + (static_cast<long long>(b) * p.c.heads + h) * p.cap;
@@ -277,139 +437,18 @@ __global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8Ev
 
   const int new_pages = (k.total + p.c.page - 1) >> p.c.page_log2, old_pages = (k.len + p.c.page - 1) >> p.c.page_log2;
   bool overlap = false;
-  for (long long i = tid; i < static_cast<long long>(new_pages) * old_pages; i += KV8_SEL_THREADS) {
-    const int n = static_cast<int>(i / old_pages), o = static_cast<int>(i - static_cast<long long>(n) * old_pages);
-    overlap |= __ldg(p.new_table + static_cast<long long>(b) * p.new_width + n) ==
-               __ldg(p.s.table + static_cast<long long>(b) * p.s.width + o);
+  for (int o = tid; o < old_pages; o += KV8_SEL_THREADS) {
+    const int page = __ldg(p.s.table + static_cast<long long>(b) * p.s.width + o);
+    for (int n = 0; n < new_pages; ++n) overlap |= __ldg(p.new_table + static_cast<long long>(b) * p.new_width + n) == page;
   }
   if (__syncthreads_or(overlap)) {
     if (tid == 0) record_error(KV8_DEV_ERROR);
     k.heavy = k.total = 0;
   }
   if (h == 0 && tid == 0) p.new_lens[b] = k.total;
-
-  const bool held = k.old <= KV8_SEL_KEYS;     // the keys are in shared memory
-  const bool select = k.heavy < k.old && k.heavy > 0;
-  if (held && k.heavy > 0) {
-    for (int i0 = tid; i0 < k.old; i0 += 8 * KV8_SEL_THREADS) {
-      float v[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u) v[u] = i0 + u * KV8_SEL_THREADS < k.old ? __ldg(w + i0 + u * KV8_SEL_THREADS) : 0.f;
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (i0 + u * KV8_SEL_THREADS < k.old) keys[i0 + u * KV8_SEL_THREADS] = weight_key(v[u]);
-    }
-  }
-  uint32_t prefix = 0, mask = 0;   // key bits fixed so far
-  int need = k.heavy;              // places left among keys that match the prefix
-  if (select) {
-#pragma unroll 1
-    for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-      const int bits = pass == 2 ? 10 : 11;
-      for (int i = tid; i < KV8_SEL_COPIES * KV8_SEL_BINS; i += KV8_SEL_THREADS) (&hist[0][0])[i] = 0;
-      __syncthreads();
-      int* mine_hist = hist[warp & (KV8_SEL_COPIES - 1)];
-      for (int i0 = tid; i0 < k.old; i0 += 8 * KV8_SEL_THREADS) {
-        uint32_t key[8];
-#pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const int i = i0 + u * KV8_SEL_THREADS;
-          key[u] = i >= k.old ? 0u : held ? keys[i] : weight_key(__ldg(w + i));
-        }
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (i0 + u * KV8_SEL_THREADS < k.old && (key[u] & mask) == prefix)
-            atomicAdd(mine_hist + ((key[u] >> shift) & ((1u << bits) - 1)), 1);
-      }
-      __syncthreads();
-      // Each thread owns two bins, highest first: thread t has bins 2047 - 2t, 2046 - 2t.
-      int c[2], mine = 0;
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const int bin = KV8_SEL_BINS - 1 - 2 * tid - j;
-        c[j] = 0;
-#pragma unroll
-        for (int q = 0; q < KV8_SEL_COPIES; ++q) c[j] += hist[q][bin];
-        mine += c[j];
-      }
-      int inc = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
-      }
-      if (lane == 31) wsum[warp] = inc;
-      __syncthreads();
-      int above = inc - mine;
-      for (int q = 0; q < warp; ++q) above += wsum[q];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        if (above < need && need <= above + c[j]) {
-          pick[0] = KV8_SEL_BINS - 1 - 2 * tid - j;
-          pick[1] = need - above;
-        }
-        above += c[j];
-      }
-      __syncthreads();
-      prefix |= static_cast<uint32_t>(pick[0]) << shift;
-      mask |= ((1u << bits) - 1) << shift;
-      need = pick[1];
-      __syncthreads();
-    }
-  }
-  // Ordered compaction of [0, old), four neighbours to a thread: keys above the
-  // threshold and at most `need` of those equal to it.
-  int done = 0, eq_done = 0;
   if (k.heavy > 0) {
-    __syncthreads();
-    for (int i0 = 0; i0 < k.old; i0 += 4 * KV8_SEL_THREADS) {
-      const int i = i0 + 4 * tid;
-      uint32_t key[4];
-      int gt = 0, eq = 0;            // bit u: neighbour u
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        key[u] = 0;
-        if (i + u < k.old) {
-          key[u] = held ? keys[i + u] : weight_key(__ldg(w + i + u));
-          if (!select || key[u] > prefix) gt |= 1 << u;
-          else if (key[u] == prefix) eq |= 1 << u;
-        }
-      }
-      const int mine = __popc(gt) | (__popc(eq) << 16);
-      int inc = mine;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += u;
-      }
-      if (lane == 31) wsum[warp] = inc;
-      __syncthreads();
-      int all = wsum[lane];
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, all, o);
-        if (lane >= o) all += u;
-      }
-      const int before = __shfl_sync(0xffffffffu, all, (warp + 31) & 31);
-      const int block = __shfl_sync(0xffffffffu, all, 31);
-      const int mine0 = inc - mine + (warp > 0 ? before : 0);
-      int at = done + (mine0 & 0xffff), e = eq_done + (mine0 >> 16);   // keys above, and equal, before these
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const bool is_eq = (eq >> u) & 1, take = ((gt >> u) & 1) || (is_eq && e < need);
-        if (take) {
-          const int to = at + min(e, select ? need : 0);
-          kept[to] = i + u;
-          nw[to] = __ldg(w + i + u);
-        }
-        at += (gt >> u) & 1;
-        e += is_eq;
-      }
-      done += block & 0xffff;
-      eq_done += block >> 16;
-      __syncthreads();   // wsum is rewritten
-    }
+    if (k.old <= min(list_at, KV8_SEL_KEYS)) kv8_select_heavy<true>(k, w, sm, keys, keys + list_at, kept, nw);
+    else kv8_select_heavy<false>(k, w, sm, keys, keys + list_at, kept, nw);
   }
   for (long long j = k.heavy + tid; j < out_cap; j += KV8_SEL_THREADS) {
     const bool live = j < k.total;
@@ -423,19 +462,20 @@ __global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8Ev
 // into registers, takes the new scales from their values and rounds them once.
 // kept lists the rows, -1 behind the last.
 template <int PAGE>
-__global__ void __launch_bounds__(256) kv8_gather_kernel(const Kv8EvictParams p) {
+__global__ void __launch_bounds__(PAGE == 128 ? 512 : 256, PAGE == 128 ? 2 : 4) kv8_gather_kernel(const Kv8EvictParams p) {
   pdl_wait();
-  constexpr int PASSES = PAGE / 16;
-  __shared__ float red[2][8];
+  constexpr int THREADS = PAGE == 128 ? 512 : 256, ROWS = THREADS / 16, PASSES = PAGE / ROWS;
+  __shared__ float red[2][THREADS / 32];
   const int h = blockIdx.y, b = blockIdx.z;
   const int c8 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
   const int* kept = p.kept + ((static_cast<long long>(b) * p.c.heads + h) * p.new_width + blockIdx.x) * PAGE;
   int pos[PASSES];
 #pragma unroll
-  for (int i = 0; i < PASSES; ++i) pos[i] = kept[r0 + 16 * i];
+  for (int i = 0; i < PASSES; ++i) pos[i] = kept[r0 + ROWS * i];
   if (__syncthreads_and(pos[0] < 0)) return;   // the page receives nothing (row 0 is kept first)
   const int dst = kv8_page(p.new_table, p.new_width, p.c, b, blockIdx.x);
   if (dst < 0) return;
+  const int* table = p.s.table + static_cast<long long>(b) * p.s.width;
   uint2 raw[2][PASSES];
   float sc[2][PASSES];
 #pragma unroll
@@ -443,49 +483,56 @@ __global__ void __launch_bounds__(256) kv8_gather_kernel(const Kv8EvictParams p)
     raw[0][i] = raw[1][i] = make_uint2(0, 0);
     sc[0][i] = sc[1][i] = 0.f;
     if (pos[i] >= 0) {
-      const int pid = kv8_page(p.s.table, p.s.width, p.c, b, pos[i] / PAGE);
-      if (pid >= 0) {
-        const long long blk = static_cast<long long>(pid) * p.c.heads + h;
-        const long long at = (blk * PAGE + pos[i] % PAGE) * 128 + c8 * 8;
+      const int pid = __ldg(table + pos[i] / PAGE);
+      if (pid >= 0 && pid < p.c.pages) {
+        const int blk = pid * p.c.heads + h;      // rows of codes are below 2^31
+        const long long at = (static_cast<long long>(blk) * PAGE + pos[i] % PAGE) * 128 + c8 * 8;
         raw[0][i] = *reinterpret_cast<const uint2*>(p.c.k8 + at);
         raw[1][i] = *reinterpret_cast<const uint2*>(p.c.v8 + at);
         sc[0][i] = p.c.k_scale[blk];
         sc[1][i] = p.c.v_scale[blk];
+      } else {
+        record_error(KV8_DEV_ERROR);
       }
     }
   }
-  float amax[2] = {0.f, 0.f};
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
+    float amax = 0.f;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
-      float f[8], m = 0.f;
-      e4m3x8_to_float(raw[x][i], f);
+      __half2 m = __floats2half2_rn(0.f, 0.f);     // codes are exact in f16; NaN loses
 #pragma unroll
-      for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(f[k]));
-      amax[x] = fmaxf(amax[x], m * sc[x][i]);
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t u = e4m3x2_to_f16x2((k < 2 ? raw[x][i].x : raw[x][i].y) >> (16 * (k & 1)));
+        m = __hmax2(m, __habs2(*reinterpret_cast<const __half2*>(&u)));
+      }
+      const float2 v = __half22float2(m);
+      amax = fmaxf(amax, fmaxf(v.x, v.y) * sc[x][i]);
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax[x] = fmaxf(amax[x], __shfl_xor_sync(0xffffffffu, amax[x], o));
-    if ((threadIdx.x & 31) == 0) red[x][threadIdx.x >> 5] = amax[x];
+    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if ((threadIdx.x & 31) == 0) red[x][threadIdx.x >> 5] = amax;
   }
   __syncthreads();
-  const long long blk = static_cast<long long>(dst) * p.c.heads + h;
+  const int blk = dst * p.c.heads + h;
 #pragma unroll
   for (int x = 0; x < 2; ++x) {
     float m = red[x][0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) m = fmaxf(m, red[x][i]);
+    for (int i = 1; i < THREADS / 32; ++i) m = fmaxf(m, red[x][i]);
     const float s = pow2f_exact(kv8_scale_exp(m)), inv = 1.f / s;
-    uint8_t* to = (x ? p.c.v8 : p.c.k8) + blk * (PAGE * 128) + c8 * 8;
+    uint8_t* to = (x ? p.c.v8 : p.c.k8) + static_cast<long long>(blk) * (PAGE * 128) + c8 * 8;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
       if (pos[i] < 0) continue;
       float f[8];
       e4m3x8_to_float(raw[x][i], f);
+      // inv is a power of two, so the factor is exact (a block of zeros may meet a huge old scale).
+      const float factor = fminf(sc[x][i] * inv, 3.402823466e38f);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] = f[k] * sc[x][i] * inv;
-      *reinterpret_cast<uint2*>(to + (r0 + 16 * i) * 128) = pack_e4m3x8(f);
+      for (int k = 0; k < 8; ++k) f[k] *= factor;
+      *reinterpret_cast<uint2*>(to + (r0 + ROWS * i) * 128) = pack_e4m3x8(f);
     }
     if (threadIdx.x == 0) (x ? p.c.v_scale : p.c.k_scale)[blk] = s;
   }

@@ -130,15 +130,16 @@ inline int kv8_evict_impl(const wamb_kv8_evict_args* a, cudaStream_t s) {
   rc = kv8_smem_once(kv8_select_kernel, KV8_SEL_SMEM, done);
   if (rc) return rc;
   // Shared memory for the keys that the tables can hold, so that short heads leave room for more blocks.
-  const int64_t hold = cap <= KV8_SEL_KEYS ? cap : KV8_SEL_KEYS;
-  rc = launch_kernel(kv8_select_kernel, dim3(p.c.heads, p.s.batch), dim3(KV8_SEL_THREADS), static_cast<size_t>(hold) * 4, s, p);
+  const int hold = static_cast<int>(std::min<int64_t>(cap, KV8_SEL_KEYS)), list = std::min(hold, KV8_SEL_LIST);
+  rc = launch_kernel(kv8_select_kernel, dim3(p.c.heads, p.s.batch), dim3(KV8_SEL_THREADS),
+                     static_cast<size_t>(hold + list) * 4, s, p, hold);
   if (rc) return rc;
   const dim3 grid(p.new_width, p.c.heads, p.s.batch);
   switch (p.c.page) {
     case 16: return launch_kernel(kv8_gather_kernel<16>, grid, dim3(256), 0, s, p);
     case 32: return launch_kernel(kv8_gather_kernel<32>, grid, dim3(256), 0, s, p);
     case 64: return launch_kernel(kv8_gather_kernel<64>, grid, dim3(256), 0, s, p);
-    default: return launch_kernel(kv8_gather_kernel<128>, grid, dim3(256), 0, s, p);
+    default: return launch_kernel(kv8_gather_kernel<128>, grid, dim3(512), 0, s, p);
   }
 }
 
