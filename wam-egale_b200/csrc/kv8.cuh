@@ -79,7 +79,13 @@ WAMB_DEV int kv8_scale_exp(float amax) {
 // Two E4M3 codes (low 16 bits) -> f16x2, exact.
 WAMB_DEV uint32_t e4m3x2_to_f16x2(uint32_t codes) {
   uint32_t r;
-  asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(codes));
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}" : "=r"(r) : "r"(codes));
+  return r;
+}
+// The same of the high 16 bits.
+WAMB_DEV uint32_t e4m3x2_hi_to_f16x2(uint32_t codes) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(codes));
   return r;
 }
 WAMB_DEV float2 e4m3x2_to_float2(uint32_t codes) {

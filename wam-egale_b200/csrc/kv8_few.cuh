@@ -319,21 +319,24 @@ struct FewUnit {
   int pad;
 };
 
+// Three CTAs fit an SM: twelve warps, each with 12 KB of its keys on their way
+// or in use. (Two CTAs with 16 KB a warp: 104 us for one token of 8 sequences
+// of 18 to 32 thousand keys, 8 heads, 4 query heads each.)
 template <bool WEIGHTS>
 struct FewSmem {
-  static constexpr int STAGES = WEIGHTS ? 4 : 2;
-  static constexpr uint32_t K_BYTES = FEW_KEYS * 128;
+  static constexpr int STAGES = WEIGHTS ? 6 : 3;                              // of 16 keys
+  static constexpr uint32_t K_BYTES = 16 * 128;
   static constexpr uint32_t STAGE_BYTES = WEIGHTS ? K_BYTES : 2 * K_BYTES;    // K codes, V codes
   static constexpr uint32_t RING = FEW_WARPS * STAGES * STAGE_BYTES;
   static constexpr uint32_t LD = 132;                               // merge rows, padded
   static constexpr uint32_t MERGE_OFF = RING;
-  static constexpr uint32_t MERGE_BYTES = WEIGHTS ? 0 : FEW_WARPS * FEW_QR * LD * 4;
+  static constexpr uint32_t MERGE_BYTES = WEIGHTS ? 0 : FEW_QR * LD * 4;
   static constexpr uint32_t ML_OFF = MERGE_OFF + MERGE_BYTES;       // m, l [warps][16]
-  static constexpr uint32_t UNIT_OFF = ML_OFF + 2 * FEW_WARPS * FEW_QR * 4;   // [warps][2 batches][32]
-  static constexpr uint32_t BAR_OFF = UNIT_OFF + FEW_WARPS * 64 * sizeof(FewUnit);
+  static constexpr uint32_t UNIT_OFF = ML_OFF + 2 * FEW_WARPS * FEW_QR * 4;   // [warps][2 batches][16]
+  static constexpr uint32_t BAR_OFF = UNIT_OFF + FEW_WARPS * 32 * sizeof(FewUnit);
   static constexpr uint32_t SCHED_OFF = BAR_OFF + FEW_WARPS * STAGES * 8;
   static constexpr uint32_t TOTAL = 1024 + SCHED_OFF + sizeof(Kv8SchedSmem) + 16;
-  static_assert(sizeof(FewUnit) == 48 && 2 * (TOTAL + 1024) <= 233472, "two CTAs must fit an SM");
+  static_assert(sizeof(FewUnit) == 48 && 3 * (TOTAL + 1024) <= 233472, "three CTAs must fit an SM");
 };
 
 // fp32 += f16 x f16: 16 rows x 16 x 8.
@@ -397,31 +400,27 @@ WAMB_DEV void few_load_q(const Kv8AttnParams& p, int e, int h, FewQ& f) {
       f.a[w][2 + half] = pack_f16(x[w][2] * up, x[w][3] * up);
     }
     f.rf[half] = __int_as_float((ex - 13) << 23) * p.scale_log2;
-    f.seen[half] = !ok ? 0 : p.causal ? max(0, min(len, len - tokens + t + 1)) : len;
+    f.seen[half] = ok && p.causal ? max(0, min(len, len - tokens + t + 1)) : len;   // a missing row is never the one that masks
   }
 }
 
-// S [16 rows][32 keys] of a warp's keys at `stage` (swizzled rows of 128 codes).
-WAMB_DEV void few_scores(uint32_t stage, const FewQ& q, float (&s)[4][4]) {
+// S [16 rows][32 keys] of a warp's keys at its two stages (swizzled rows of 128
+// codes; eight lanes meet each bank twice, which costs less than ordering the
+// pieces by row did in selects).
+WAMB_DEV void few_scores(const uint32_t (&stage)[2], const FewQ& q, float (&s)[4][4]) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-  // The two 16-byte pieces of a row, in an order that alternates with the row
-  // so that eight lanes cover all banks.
-  const int o = (g & 1) * 4;
-  const bool sw = g & 1;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t row = stage + (8 * j + g) * 128;
-    const uint4 x = lds128(row + (((t4 + o) ^ g) << 4));
-    const uint4 y = lds128(row + (((t4 + 4 - o) ^ g) << 4));
-    const uint32_t w[8] = {sw ? y.x : x.x, sw ? y.y : x.y, sw ? y.z : x.z, sw ? y.w : x.w,
-                           sw ? x.x : y.x, sw ? x.y : y.y, sw ? x.z : y.z, sw ? x.w : y.w};
+    const uint32_t row = stage[j >> 1] + (8 * (j & 1) + g) * 128;
+    const uint4 x = lds128(row + ((t4 ^ g) << 4)), y = lds128(row + (((t4 + 4) ^ g) << 4));
+    const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
     float r[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[j][i] = 0.f;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {   // two chains of sums, half as long
-      mma_f16_16816(s[j], q.a[k], e4m3x2_to_f16x2(w[k]), e4m3x2_to_f16x2(w[k] >> 16));
-      mma_f16_16816(r, q.a[4 + k], e4m3x2_to_f16x2(w[4 + k]), e4m3x2_to_f16x2(w[4 + k] >> 16));
+      mma_f16_16816(s[j], q.a[k], e4m3x2_to_f16x2(w[k]), e4m3x2_hi_to_f16x2(w[k]));
+      mma_f16_16816(r, q.a[4 + k], e4m3x2_to_f16x2(w[4 + k]), e4m3x2_hi_to_f16x2(w[4 + k]));
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[j][i] += r[i];
@@ -431,7 +430,7 @@ WAMB_DEV void few_scores(uint32_t stage, const FewQ& q, float (&s)[4][4]) {
 // Attention (WEIGHTS = false) and attention weights (true; each unit owns its
 // keys' sums, so no sum has a racing order).
 template <bool WEIGHTS>
-__global__ void __launch_bounds__(FEW_THREADS)
+__global__ void __launch_bounds__(FEW_THREADS, 3)
     kv8_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const Kv8AttnParams p) {
   using L = FewSmem<WEIGHTS>;
@@ -442,7 +441,7 @@ __global__ void __launch_bounds__(FEW_THREADS)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
   const uint32_t ring = smem_u32(smem) + warp * (L::STAGES * L::STAGE_BYTES);
   const uint32_t bars = smem_u32(smem + L::BAR_OFF) + warp * (L::STAGES * 8);
-  FewUnit* units = reinterpret_cast<FewUnit*>(smem + L::UNIT_OFF) + warp * 64;
+  FewUnit* units = reinterpret_cast<FewUnit*>(smem + L::UNIT_OFF) + warp * 32;
   if (lane == 0)
     for (int i = 0; i < L::STAGES; ++i) mbar_init(bars + 8 * i, 1);
   if (threadIdx.x == 0) *abort_flag = 0;
@@ -459,56 +458,56 @@ __global__ void __launch_bounds__(FEW_THREADS)
   const int count = static_cast<int>(sh.u1 - sh.u0);
   bool began = it.start == sh.u0;      // the current item begins in this share
 
-  // Batches of 32 units: lane i looks up unit i's addresses and scales, a
-  // whole batch ahead of their use. `it` moves over the line with them.
+  // Batches of 16 units: lanes 2 i, 2 i + 1 look up the halves of unit i, a whole
+  // batch ahead of its use. `it` moves over the line with them.
   auto load_batch = [&](int j0) {
-    const int j = min(j0 + lane, count - 1);
+    const int j = min(j0 + (lane >> 1), count - 1), hf = lane & 1;
     kv8_seek<FEW_QR, FEW_TK>(p, it, sh.u0 + j);
     const int tile = static_cast<int>(sh.u0 + j - it.start);
-    FewUnit u;
-    u.k0 = tile * FEW_TK + warp * FEW_KEYS;
-    u.live = max(0, min(FEW_KEYS, Kv8Line<FEW_QR, FEW_TK>::visible(p, it.e) - u.k0));
-    u.e = it.e;
-    u.h = it.h;
-    u.last = tile == it.n - 1 || j == count - 1;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      u.row[i] = 0;
-      u.ks[i] = u.vs[i] = 1.f;
-      if (u.live > 16 * i) {
-        const int k = u.k0 + 16 * i;
-        int pid = kv8_page(p.s.table, p.s.width, p.c, it.e / p.qts, k >> p.c.page_log2);
-        if (pid < 0) pid = 0;   // reported
-        const long long blk = static_cast<long long>(pid) * p.c.heads + it.h;
-        u.row[i] = static_cast<int>((blk << p.c.page_log2) + (k & (p.c.page - 1)));
-        u.ks[i] = __ldg(p.c.k_scale + blk);
-        if constexpr (!WEIGHTS) u.vs[i] = __ldg(p.c.v_scale + blk);
-      }
+    const int k0 = tile * FEW_TK + warp * FEW_KEYS;
+    const int live = max(0, min(FEW_KEYS, Kv8Line<FEW_QR, FEW_TK>::visible(p, it.e) - k0));
+    int row = 0;
+    float ks = 1.f, vs = 1.f;
+    if (live > 16 * hf) {
+      const int k = k0 + 16 * hf;
+      int pid = kv8_page(p.s.table, p.s.width, p.c, it.e / p.qts, k >> p.c.page_log2);
+      if (pid < 0) pid = 0;   // reported
+      const long long blk = static_cast<long long>(pid) * p.c.heads + it.h;
+      row = static_cast<int>((blk << p.c.page_log2) + (k & (p.c.page - 1)));
+      ks = __ldg(p.c.k_scale + blk);
+      if constexpr (!WEIGHTS) vs = __ldg(p.c.v_scale + blk);
     }
-    u.pad = 0;
-    units[(j0 & 32) + lane] = u;
+    FewUnit& u = units[(j0 & 16) + (lane >> 1)];
+    u.row[hf] = row;
+    u.ks[hf] = ks;
+    u.vs[hf] = vs;
+    if (hf == 0) {
+      u.k0 = k0;
+      u.live = live;
+      u.e = it.e;
+      u.h = it.h;
+      u.last = tile == it.n - 1 || j == count - 1;
+    }
     it.e = __shfl_sync(0xffffffffu, it.e, 31);
     it.h = __shfl_sync(0xffffffffu, it.h, 31);
     it.n = __shfl_sync(0xffffffffu, it.n, 31);
     it.start = __shfl_sync(0xffffffffu, it.start, 31);
     __syncwarp();
   };
-  int issued = 0, used = 0, ahead = 0, known = 0;   // ring loads issued and consumed; next unit to issue; units looked up
+  // Ring loads, 16 keys each: issued and consumed so far; the next half to
+  // issue; units looked up.
+  uint32_t issued = 0, used = 0;
+  int ahead = 0, known = 0;
   auto issue = [&]() {
-    while (ahead < known && issued < used + L::STAGES) {
-      const FewUnit& u = units[ahead & 63];
-      const int live = u.live;
-      if (live > 0) {
-        const uint32_t st = issued % L::STAGES, at = ring + st * L::STAGE_BYTES, bar = bars + 8 * st;
+    while (ahead < 2 * known && issued < used + L::STAGES) {
+      const FewUnit& u = units[(ahead >> 1) & 31];
+      if (u.live > 16 * (ahead & 1)) {
         if (lane == 0) {
-          const int r0 = u.row[0], r1 = u.row[1];
-          mbar_arrive_expect_tx(bar, (live > 16 ? 2 : 1) * (WEIGHTS ? 2048 : 4096));
-          tma_load_2d(at, &tmK, bar, 0, r0);
-          if (live > 16) tma_load_2d(at + 2048, &tmK, bar, 0, r1);
-          if constexpr (!WEIGHTS) {
-            tma_load_2d(at + L::K_BYTES, &tmV, bar, 0, r0);
-            if (live > 16) tma_load_2d(at + L::K_BYTES + 2048, &tmV, bar, 0, r1);
-          }
+          const uint32_t st = issued % L::STAGES, at = ring + st * L::STAGE_BYTES, bar = bars + 8 * st;
+          const int row = u.row[ahead & 1];
+          mbar_arrive_expect_tx(bar, L::STAGE_BYTES);
+          tma_load_2d(at, &tmK, bar, 0, row);
+          if constexpr (!WEIGHTS) tma_load_2d(at + L::K_BYTES, &tmV, bar, 0, row);
         }
         ++issued;
       }
@@ -516,7 +515,7 @@ __global__ void __launch_bounds__(FEW_THREADS)
     }
   };
   load_batch(0);
-  known = min(32, count);
+  known = min(16, count);
   issue();
 
   FewQ q;
@@ -533,12 +532,12 @@ __global__ void __launch_bounds__(FEW_THREADS)
   bool fresh = true;
   bool ok = true;
   for (int j = 0; j < count; ++j) {
-    if ((j & 31) == 8 && known < count) {   // the batch before this one is used up: its places take the next
+    if ((j & 15) == 4 && known < count) {   // the batch before this one is used up: its places take the next
       load_batch(known);
-      known = min(known + 32, count);
+      known = min(known + 16, count);
       issue();
     }
-    const FewUnit& u = units[j & 63];
+    const FewUnit& u = units[j & 31];
     const int live = u.live, k0 = u.k0, last = u.last;
     if (fresh) {
       few_load_q(p, u.e, u.h, q);
@@ -563,18 +562,23 @@ __global__ void __launch_bounds__(FEW_THREADS)
     if (live > 0) {
       const float ks[2] = {u.ks[0], u.ks[1]};
       [[maybe_unused]] const float vs[2] = {u.vs[0], u.vs[1]};
-      const int st = used % L::STAGES;
-      const uint32_t stage = ring + st * L::STAGE_BYTES;
+      const uint32_t st0 = used % L::STAGES, st1 = st0 + 1 == L::STAGES ? 0 : st0 + 1;
+      const uint32_t stage[2] = {ring + st0 * L::STAGE_BYTES, ring + st1 * L::STAGE_BYTES};
+      const bool two = live > 16;
+      auto arrived = [&]() {
+        ok = mbar_wait(bars + 8 * st0, (used / L::STAGES) & 1, abort_flag) && ok;
+        if (two) ok = mbar_wait(bars + 8 * st1, ((used + 1) / L::STAGES) & 1, abort_flag) && ok;
+      };
       if constexpr (WEIGHTS) {
         // Lane (g, t) finishes key 8 (g / 2) + 2 t + g % 2.
         const int key = 8 * (g >> 1) + 2 * t4 + (g & 1);
         const long long at = (static_cast<long long>(u.e) * p.c.heads + u.h) * p.w_cap + k0 + key;
         const float base = p.base != nullptr && key < live ? __ldcg(p.base + at) : 0.f;
-        ok = mbar_wait(bars + 8 * st, (used / L::STAGES) & 1, abort_flag) && ok;
+        arrived();
         float s[4][4];
         few_scores(stage, q, s);
         __syncwarp();
-        ++used;
+        used += two ? 2 : 1;
         issue();
         float mine = 0.f;
 #pragma unroll
@@ -593,7 +597,7 @@ __global__ void __launch_bounds__(FEW_THREADS)
         }
         if (key < live) p.weights[at] = ok ? base + mine : 0.f;
       } else {
-        ok = mbar_wait(bars + 8 * st, (used / L::STAGES) & 1, abort_flag) && ok;
+        arrived();
         float s[4][4];
         few_scores(stage, q, s);
         const float lv[2] = {log2f(vs[0]), log2f(vs[1])}, iv[2] = {1.f / vs[0], 1.f / vs[1]};
@@ -602,11 +606,19 @@ __global__ void __launch_bounds__(FEW_THREADS)
         for (int jt = 0; jt < 4; ++jt) {
           const float f[2] = {q.rf[0] * ks[jt >> 1], q.rf[1] * ks[jt >> 1]};
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const int half = c >> 1, key = k0 + 8 * jt + 2 * t4 + (c & 1);
-            s[jt][c] = key < q.seen[half] ? fmaf(s[jt][c], f[half], lv[jt >> 1]) : -INFINITY;
-            mx[half] = fmaxf(mx[half], s[jt][c]);
-          }
+          for (int c = 0; c < 4; ++c) s[jt][c] = fmaf(s[jt][c], f[c >> 1], lv[jt >> 1]);
+        }
+        if (__any_sync(0xffffffffu, k0 + FEW_KEYS > min(q.seen[0], q.seen[1]))) {
+#pragma unroll
+          for (int jt = 0; jt < 4; ++jt)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+              if (k0 + 8 * jt + 2 * t4 + (c & 1) >= q.seen[c >> 1]) s[jt][c] = -INFINITY;
+        }
+#pragma unroll
+        for (int jt = 0; jt < 4; ++jt) {
+          mx[0] = fmax3(mx[0], s[jt][0], s[jt][1]);
+          mx[1] = fmax3(mx[1], s[jt][2], s[jt][3]);
         }
         if (__any_sync(0xffffffffu, mx[0] > m[0] + FEW_RESCALE || mx[1] > m[1] + FEW_RESCALE)) {
 #pragma unroll
@@ -641,18 +653,21 @@ __global__ void __launch_bounds__(FEW_THREADS)
           // output column n = g of product i is dim 16 g + i.
           const uint32_t a[4] = {pack_f16(s[2 * kk][0], s[2 * kk][1]), pack_f16(s[2 * kk][2], s[2 * kk][3]),
                                  pack_f16(s[2 * kk + 1][0], s[2 * kk + 1][1]), pack_f16(s[2 * kk + 1][2], s[2 * kk + 1][3])};
+          if (kk == 1 && !two) break;     // no keys there
           uint4 v[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int r = (i >> 1) * 8 + 2 * t4 + (i & 1);
-            v[i] = lds128(stage + L::K_BYTES + (16 * kk + r) * 128 + ((g ^ (r & 7)) << 4));
-            if (16 * kk + r >= live) v[i] = make_uint4(0, 0, 0, 0);   // whatever lies there (NaN codes too) counts for nothing
+            v[i] = lds128(stage[kk] + L::K_BYTES + r * 128 + ((g ^ (r & 7)) << 4));
           }
-          if (kk == 1) {
-            __syncwarp();
-            ++used;
-            issue();
+          if (live < 16 * kk + 16) {      // whatever lies behind the keys (NaN codes too) counts for nothing
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (16 * kk + (i >> 1) * 8 + 2 * t4 + (i & 1) >= live) v[i] = make_uint4(0, 0, 0, 0);
           }
+          __syncwarp();
+          ++used;
+          issue();
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             const uint32_t v0 = w == 0 ? v[0].x : w == 1 ? v[0].y : w == 2 ? v[0].z : v[0].w;
@@ -662,9 +677,9 @@ __global__ void __launch_bounds__(FEW_THREADS)
             const uint32_t lo0 = __byte_perm(v0, v1, 0x5140), hi0 = __byte_perm(v0, v1, 0x7362);
             const uint32_t lo1 = __byte_perm(v2, v3, 0x5140), hi1 = __byte_perm(v2, v3, 0x7362);
             mma_f16_16816(o[4 * w], a, e4m3x2_to_f16x2(lo0), e4m3x2_to_f16x2(lo1));
-            mma_f16_16816(o[4 * w + 1], a, e4m3x2_to_f16x2(lo0 >> 16), e4m3x2_to_f16x2(lo1 >> 16));
+            mma_f16_16816(o[4 * w + 1], a, e4m3x2_hi_to_f16x2(lo0), e4m3x2_hi_to_f16x2(lo1));
             mma_f16_16816(o[4 * w + 2], a, e4m3x2_to_f16x2(hi0), e4m3x2_to_f16x2(hi1));
-            mma_f16_16816(o[4 * w + 3], a, e4m3x2_to_f16x2(hi0 >> 16), e4m3x2_to_f16x2(hi1 >> 16));
+            mma_f16_16816(o[4 * w + 3], a, e4m3x2_hi_to_f16x2(hi0), e4m3x2_hi_to_f16x2(hi1));
           }
         }
       }
@@ -675,48 +690,62 @@ __global__ void __launch_bounds__(FEW_THREADS)
       // The item, or the share, ends: the warps' results meet in shared memory.
       float* wm = reinterpret_cast<float*>(smem + L::ML_OFF);
       float* wl = wm + FEW_WARPS * FEW_QR;
-      float* buf = reinterpret_cast<float*>(smem + L::MERGE_OFF) + warp * FEW_QR * L::LD;
+      float* buf = reinterpret_cast<float*>(smem + L::MERGE_OFF);
       const int b = u.e, h = u.h;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         l[half] += __shfl_xor_sync(0xffffffffu, l[half], 1);
         l[half] += __shfl_xor_sync(0xffffffffu, l[half], 2);
-        const int r = g + 8 * half;
         if (t4 == 0) {
-          wm[warp * FEW_QR + r] = m[half];
-          wl[warp * FEW_QR + r] = l[half];
+          wm[warp * FEW_QR + g + 8 * half] = m[half];
+          wl[warp * FEW_QR + g + 8 * half] = l[half];
         }
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<float4*>(buf + r * L::LD + 32 * t4 + 16 * c + i) =
-                make_float4(o[i][2 * half + c], o[i + 1][2 * half + c], o[i + 2][2 * half + c], o[i + 3][2 * half + c]);
       }
       __syncthreads();
       const int rows = min(FEW_QR, kv8_count(p.s, b) * p.group);
+      // One warp after another adds its rows, relative to the largest maximum.
+      for (int w = 0; w < FEW_WARPS; ++w) {
+        if (w == warp) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int r = g + 8 * half;
+            if (r < rows) {
+              float M = -INFINITY;
+#pragma unroll
+              for (int x = 0; x < FEW_WARPS; ++x) M = fmaxf(M, wm[x * FEW_QR + r]);
+              const float f = m[half] == -INFINITY && l[half] == 0.f ? 0.f : exp2f(m[half] - M);
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                  float4* to = reinterpret_cast<float4*>(buf + r * L::LD + 32 * t4 + 16 * c + i);
+                  float4 v = w == 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *to;
+                  v.x = fmaf(f, o[i][2 * half + c], v.x);
+                  v.y = fmaf(f, o[i + 1][2 * half + c], v.y);
+                  v.z = fmaf(f, o[i + 2][2 * half + c], v.z);
+                  v.w = fmaf(f, o[i + 3][2 * half + c], v.w);
+                  *to = v;
+                }
+            }
+          }
+        }
+        __syncthreads();
+      }
       // Whole only when the share holds the item's first and last unit.
       const int n = max(1, (Kv8Line<FEW_QR, FEW_TK>::visible(p, b) + FEW_TK - 1) / FEW_TK);
       const bool whole = began && (k0 - warp * FEW_KEYS) / FEW_TK == n - 1;
       float* part = p.part + static_cast<size_t>(2 * blockIdx.x + (began ? 1 : 0)) * kv8_part_floats<FEW_QR>();
-      const float* mbuf = reinterpret_cast<const float*>(smem + L::MERGE_OFF);
       for (int i = threadIdx.x; i < rows * 32; i += FEW_THREADS) {
         const int r = i >> 5, c4 = i & 31;
         float M = -INFINITY;
 #pragma unroll
         for (int w = 0; w < FEW_WARPS; ++w) M = fmaxf(M, wm[w * FEW_QR + r]);
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float4 acc = *reinterpret_cast<const float4*>(buf + r * L::LD + c4 * 4);
         float den = 0.f;
 #pragma unroll
         for (int w = 0; w < FEW_WARPS; ++w) {
-          const float mw = wm[w * FEW_QR + r];
-          const float x = mw == -INFINITY ? 0.f : exp2f(mw - M);
-          const float4 v = *reinterpret_cast<const float4*>(mbuf + (w * FEW_QR + r) * L::LD + c4 * 4);
-          den += x * wl[w * FEW_QR + r];
-          acc.x += x * v.x;
-          acc.y += x * v.y;
-          acc.z += x * v.z;
-          acc.w += x * v.w;
+          const float mw = wm[w * FEW_QR + r], lw = wl[w * FEW_QR + r];
+          if (lw != 0.f) den += exp2f(mw - M) * lw;
         }
         const float mref = M == -INFINITY ? M : M - FEW_OFFSET;
         if (!ok) den = 0.f;

@@ -143,8 +143,8 @@ inline int kv8_evict_impl(const wamb_kv8_evict_args* a, cudaStream_t s) {
   }
 }
 
-// Two CTAs of the few-row kernel fit an SM, one of the tensor-core kernel.
-inline int kv8_few_ctas(const DeviceInfo& di) { return 2 * di.sms; }
+// Three CTAs of the few-row kernel fit an SM, one of the tensor-core kernels.
+inline int kv8_few_ctas(const DeviceInfo& di) { return 3 * di.sms; }
 
 // A tile of 16 rows is one m16n8k16 operand; more rows go to the tcgen05
 // kernel, which reads each key once for 256 of them.
