@@ -314,17 +314,18 @@ constexpr float FEW_OFFSET = 6.f;     // P is 2^6 at the maximum
 struct FewUnit {
   int row[2];      // first row of each half in the [pages * heads * page, 128] code matrix
   int k0, live;    // first key position, live keys
-  float ks[2], vs[2];
+  float ks[2], lv[2], iv[2];   // scales of K; log2 and reciprocal of the scales of V
   int e, h, last;  // last: the unit ends its item or the CTA's share
   int pad;
 };
 
-// Three CTAs fit an SM: twelve warps, each with 12 KB of its keys on their way
-// or in use. (Two CTAs with 16 KB a warp: 104 us for one token of 8 sequences
-// of 18 to 32 thousand keys, 8 heads, 4 query heads each.)
+// Three CTAs fit an SM (four of the weights'): twelve warps, each with 12 KB (10)
+// of its keys on their way or in use. (Two CTAs with 16 KB a warp took 104 us
+// where this takes 84: one token of 8 sequences of 18 to 32 thousand keys, 8
+// heads, 4 query heads each.)
 template <bool WEIGHTS>
 struct FewSmem {
-  static constexpr int STAGES = WEIGHTS ? 6 : 3;                              // of 16 keys
+  static constexpr int STAGES = WEIGHTS ? 5 : 3;                              // of 16 keys
   static constexpr uint32_t K_BYTES = 16 * 128;
   static constexpr uint32_t STAGE_BYTES = WEIGHTS ? K_BYTES : 2 * K_BYTES;    // K codes, V codes
   static constexpr uint32_t RING = FEW_WARPS * STAGES * STAGE_BYTES;
@@ -336,12 +337,12 @@ struct FewSmem {
   static constexpr uint32_t BAR_OFF = UNIT_OFF + FEW_WARPS * 32 * sizeof(FewUnit);
   static constexpr uint32_t SCHED_OFF = BAR_OFF + FEW_WARPS * STAGES * 8;
   static constexpr uint32_t TOTAL = 1024 + SCHED_OFF + sizeof(Kv8SchedSmem) + 16;
-  static_assert(sizeof(FewUnit) == 48 && 3 * (TOTAL + 1024) <= 233472, "three CTAs must fit an SM");
+  static_assert(sizeof(FewUnit) == 56 && (WEIGHTS ? 4 : 3) * (TOTAL + 1024) <= 233472, "the CTAs must fit an SM");
 };
 
 // fp32 += f16 x f16: 16 rows x 16 x 8.
 WAMB_DEV void mma_f16_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -414,23 +415,17 @@ WAMB_DEV void few_scores(const uint32_t (&stage)[2], const FewQ& q, float (&s)[4
     const uint32_t row = stage[j >> 1] + (8 * (j & 1) + g) * 128;
     const uint4 x = lds128(row + ((t4 ^ g) << 4)), y = lds128(row + (((t4 + 4) ^ g) << 4));
     const uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-    float r[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 4; ++i) s[j][i] = 0.f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {   // two chains of sums, half as long
-      mma_f16_16816(s[j], q.a[k], e4m3x2_to_f16x2(w[k]), e4m3x2_hi_to_f16x2(w[k]));
-      mma_f16_16816(r, q.a[4 + k], e4m3x2_to_f16x2(w[4 + k]), e4m3x2_hi_to_f16x2(w[4 + k]));
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[j][i] += r[i];
+    for (int k = 0; k < 8; ++k) mma_f16_16816(s[j], q.a[k], e4m3x2_to_f16x2(w[k]), e4m3x2_hi_to_f16x2(w[k]));
   }
 }
 
 // Attention (WEIGHTS = false) and attention weights (true; each unit owns its
 // keys' sums, so no sum has a racing order).
 template <bool WEIGHTS>
-__global__ void __launch_bounds__(FEW_THREADS, 3)
+__global__ void __launch_bounds__(FEW_THREADS, WEIGHTS ? 4 : 3)
     kv8_few_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                    const Kv8AttnParams p) {
   using L = FewSmem<WEIGHTS>;
@@ -480,7 +475,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 3)
     FewUnit& u = units[(j0 & 16) + (lane >> 1)];
     u.row[hf] = row;
     u.ks[hf] = ks;
-    u.vs[hf] = vs;
+    u.lv[hf] = log2f(vs);
+    u.iv[hf] = 1.f / vs;
     if (hf == 0) {
       u.k0 = k0;
       u.live = live;
@@ -514,11 +510,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 3)
       ++ahead;
     }
   };
+  // The first item's queries are asked for before its pages are looked up.
+  FewQ q;
+  few_load_q(p, it.e, it.h, q);
+  bool loaded = true;
   load_batch(0);
   known = min(16, count);
   issue();
 
-  FewQ q;
   float o[16][4];
   float m[2], l[2];
   auto reset = [&]() {
@@ -540,7 +539,8 @@ __global__ void __launch_bounds__(FEW_THREADS, 3)
     const FewUnit& u = units[j & 31];
     const int live = u.live, k0 = u.k0, last = u.last;
     if (fresh) {
-      few_load_q(p, u.e, u.h, q);
+      if (!loaded) few_load_q(p, u.e, u.h, q);
+      loaded = false;
       if constexpr (WEIGHTS) {
         // The rows' log-sum-exp in log2 units; rows that see nothing add nothing.
         const int tokens = kv8_count(p.s, u.e);
@@ -561,7 +561,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 3)
     }
     if (live > 0) {
       const float ks[2] = {u.ks[0], u.ks[1]};
-      [[maybe_unused]] const float vs[2] = {u.vs[0], u.vs[1]};
+      [[maybe_unused]] const float lv[2] = {u.lv[0], u.lv[1]}, iv[2] = {u.iv[0], u.iv[1]};
       const uint32_t st0 = used % L::STAGES, st1 = st0 + 1 == L::STAGES ? 0 : st0 + 1;
       const uint32_t stage[2] = {ring + st0 * L::STAGE_BYTES, ring + st1 * L::STAGE_BYTES};
       const bool two = live > 16;
@@ -600,7 +600,6 @@ __global__ void __launch_bounds__(FEW_THREADS, 3)
         arrived();
         float s[4][4];
         few_scores(stage, q, s);
-        const float lv[2] = {log2f(vs[0]), log2f(vs[1])}, iv[2] = {1.f / vs[0], 1.f / vs[1]};
         float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int jt = 0; jt < 4; ++jt) {

@@ -143,8 +143,9 @@ inline int kv8_evict_impl(const wamb_kv8_evict_args* a, cudaStream_t s) {
   }
 }
 
-// Three CTAs of the few-row kernel fit an SM, one of the tensor-core kernels.
-inline int kv8_few_ctas(const DeviceInfo& di) { return 3 * di.sms; }
+// Three CTAs of the few-row attention fit an SM, four of its weights', one of
+// the tensor-core kernels.
+inline int kv8_few_ctas(const DeviceInfo& di, bool weights = false) { return (weights ? 4 : 3) * di.sms; }
 
 // A tile of 16 rows is one m16n8k16 operand; more rows go to the tcgen05
 // kernel, which reads each key once for 256 of them.
@@ -261,7 +262,7 @@ inline int kv8_attention_impl(const wamb_kv8_attention_args* a, bool weights, cu
   if (rc) return rc;
   rc = make_tmap_2d(&tmV, p.c.v8, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, code_rows, 128, 128, box, 128);
   if (rc) return rc;
-  p.ctas = kv8_few_ctas(di);
+  p.ctas = kv8_few_ctas(di, weights);
   p.min_units = 1;
   if (weights && few) {
     static bool done[64] = {};

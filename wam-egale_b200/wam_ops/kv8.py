@@ -47,6 +47,7 @@ class Kv8Cache:
         self._c = _lib.Kv8CacheArgs(k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), pages, heads,
                                     page)
         self._lib = _lib.load()
+        self._scratch = {}     # bytes that a call's shape needs
 
     @classmethod
     def empty(cls, pages, heads, page=64, device="cuda"):
@@ -88,18 +89,21 @@ class Kv8Cache:
                              f" on {self.device}")
         return t.data_ptr()
 
-    def _call(self, fn, args, workspace_bytes=None):
+    def _call(self, fn, args, workspace_bytes=None, shape=None):
         """fn(args) on the current stream of the cache's device, with scratch
         of its own from that stream's (or the captured graph's) pool."""
-        if torch.cuda.current_device() != self.device.index:
+        index = self.device.index
+        if torch._C._cuda_getDevice() != index:
             with torch.cuda.device(self.device):
-                return self._call(fn, args, workspace_bytes)
+                return self._call(fn, args, workspace_bytes, shape)
         if workspace_bytes is not None:
-            n = workspace_bytes(args)
+            n = self._scratch.get(shape)
+            if n is None:
+                n = self._scratch[shape] = workspace_bytes(args)
             if n:
-                ws = torch.empty(n, dtype=torch.uint8, device=self.device)
+                ws = self.k_scale.new_empty((n + 3) // 4)
                 args.workspace, args.workspace_bytes = ws.data_ptr(), n
-        rc = fn(args, torch._C._cuda_getCurrentRawStream(self.device.index))
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
         if rc:
             _lib.check(rc)
 
@@ -144,16 +148,16 @@ class Kv8Cache:
         of `out` and `lse` are left as they were."""
         a = self._attention_args(q, table, lens, counts, causal, scale)
         if out is None:
-            out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
+            out = q.new_empty(q.shape)
         elif out.shape != q.shape:
             raise ValueError("out must be shaped like q")
         a.out_stride[:] = self._rows("out", out)
         a.out = out.data_ptr()
         if lse is None and return_lse:
-            lse = torch.empty(q.shape[:3], dtype=torch.float32, device=self.device)
+            lse = self.k_scale.new_empty(q.shape[:3])
         if lse is not None:
             a.lse = self._lse(lse, q)
-        self._call(self._lib.wamb_kv8_attention, a, self._lib.wamb_kv8_attention_workspace_bytes)
+        self._call(self._lib.wamb_kv8_attention, a, self._lib.wamb_kv8_attention_workspace_bytes, ("attention", q.shape))
         return (out, lse) if return_lse else out
 
     def _lse(self, lse, q):
@@ -174,12 +178,12 @@ class Kv8Cache:
             a.base = self._weight("base", base, batch, width)
         if out is None:
             shape = base.shape if base is not None else (batch, self.heads, width * self.page)
-            out = torch.empty(shape, dtype=torch.float32, device=self.device)
+            out = self.k_scale.new_empty(shape)
         a.weights = self._weight("out", out, batch, width)
         if base is not None and base.shape != out.shape:
             raise ValueError("base and out must have one shape")
         a.weights_cap = out.shape[2]
-        self._call(self._lib.wamb_kv8_weights, a, self._lib.wamb_kv8_weights_workspace_bytes)
+        self._call(self._lib.wamb_kv8_weights, a, self._lib.wamb_kv8_weights_workspace_bytes, ("weights", q.shape))
         return out
 
     def evict(self, table, lens, weights, new_table, heavy, recent, max_len=None):
@@ -204,9 +208,8 @@ class Kv8Cache:
         a.heavy, a.recent = int(heavy), int(recent)
         a.max_len = table.shape[1] * self.page if max_len is None else int(max_len)
         shape = (batch, self.heads, a.new_width * self.page)
-        kept = torch.empty(shape, dtype=torch.int32, device=self.device)
-        new_weights = torch.empty(shape, dtype=torch.float32, device=self.device)
-        new_lens = torch.empty(batch, dtype=torch.int32, device=self.device)
+        kept, new_lens = table.new_empty(shape), table.new_empty(batch)
+        new_weights = weights.new_empty(shape)
         a.kept, a.new_weights, a.new_lens = kept.data_ptr(), new_weights.data_ptr(), new_lens.data_ptr()
         self._call(self._lib.wamb_kv8_evict, a)
         return kept, new_weights, new_lens
