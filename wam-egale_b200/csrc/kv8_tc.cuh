@@ -20,7 +20,7 @@
 //   warp 8       producer: page ids and scales (read four tiles ahead), TMA
 //                of the queries' pieces (split once by kv8_split_q_kernel)
 //                and of K and V codes, the scales of each 16 keys to a ring
-//   warp 9       its lane 0 issues the MMAs
+//   warp 9       issues the MMAs
 //   warps 10, 11 V codes -> f16
 // With more than 128 rows, slot A and slot B hold the tile's two halves and
 // meet every key tile; with fewer, both hold the same rows and take the key
@@ -38,17 +38,17 @@ namespace wamb {
 
 constexpr int KTC_THREADS = 384, KTC_QR = 256, KTC_TK = 128;
 constexpr uint32_t KTC_TILE8 = 128 * 128;      // 128 rows of 128 codes
-constexpr int KTC_KS = 3, KTC_V8S = 2, KTC_V16S = 2, KTC_SCS = 8;
+constexpr int KTC_SCS = 8;     // key tiles whose scales are kept; K, V and f16 V have rings of two
 
 struct KtcSmem {
   static constexpr uint32_t Q_OFF = 0;                                       // slot A hi, lo, slot B hi, lo
   static constexpr uint32_t K_OFF = Q_OFF + 4 * KTC_TILE8;
-  static constexpr uint32_t V8_OFF = K_OFF + KTC_KS * KTC_TILE8;
-  static constexpr uint32_t V16_OFF = V8_OFF + KTC_V8S * KTC_TILE8;
-  static constexpr uint32_t SC_OFF = V16_OFF + KTC_V16S * 2 * KTC_TILE8;     // [8 tiles] ks, log2 vs, 1 / vs of 8 groups of 16 keys
-  static constexpr uint32_t XCH_OFF = SC_OFF + KTC_SCS * 8 * 16;             // m, l of both slots
-  static constexpr uint32_t BAR_OFF = XCH_OFF + 2 * 2 * 128 * 4;
-  static constexpr uint32_t NBARS = 2 * KTC_KS + 2 * KTC_V8S + 2 * KTC_V16S + 2 + 2 + 4 + KTC_SCS;
+  static constexpr uint32_t V8_OFF = K_OFF + 2 * KTC_TILE8;
+  static constexpr uint32_t V16_OFF = V8_OFF + 2 * KTC_TILE8;
+  static constexpr uint32_t STAGE_OFF = V16_OFF + 4 * KTC_TILE8;   // output rows, 4 KB a softmax warp; before them m, l of both slots
+  static constexpr uint32_t SC_OFF = STAGE_OFF + 8 * 4096;         // [8 tiles] ks, log2 vs, 1 / vs of 8 groups of 16 keys
+  static constexpr uint32_t BAR_OFF = SC_OFF + KTC_SCS * 128;
+  static constexpr uint32_t NBARS = 12 + 2 + 2 + 5 + KTC_SCS;
   static constexpr uint32_t SCHED_OFF = BAR_OFF + NBARS * 8;
   static constexpr uint32_t TOTAL = 1024 + SCHED_OFF + sizeof(Kv8SchedSmem) + 16;
   static_assert(TOTAL <= 232448, "shared memory exceeds 227 KB");
@@ -269,9 +269,9 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
   const uint32_t sQ = base + L::Q_OFF, sK = base + L::K_OFF, sV8 = base + L::V8_OFF, sV16 = base + L::V16_OFF;
   uint32_t bar = base + L::BAR_OFF;
   auto bars = [&](int n) { const uint32_t b = bar; bar += 8 * n; return b; };
-  const uint32_t k_full = bars(KTC_KS), k_empty = bars(KTC_KS), v8_full = bars(KTC_V8S), v8_empty = bars(KTC_V8S),
-                 v16_full = bars(KTC_V16S), v16_empty = bars(KTC_V16S), s_full = bars(2), p_full = bars(2),
-                 q_full = bars(1), o_done = bars(1), o_free = bars(1), drain = bars(1), sc_full = bars(KTC_SCS);
+  const uint32_t k_full = bars(2), k_empty = bars(2), v8_full = bars(2), v8_empty = bars(2), v16_full = bars(2), v16_empty = bars(2),
+                 s_full = bars(2), p_full = bars(2), q_full = bars(1), q_free = bars(1), o_done = bars(1), o_free = bars(1),
+                 drain = bars(1), sc_full = bars(KTC_SCS);
   Kv8SchedSmem& sched = *reinterpret_cast<Kv8SchedSmem*>(smem + L::SCHED_OFF);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::SCHED_OFF + sizeof(Kv8SchedSmem));
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -285,11 +285,18 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
   if (!work) return;
   walk.u = sh.u0;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < KTC_KS; ++i) { mbar_init(k_full + 8 * i, 1); mbar_init(k_empty + 8 * i, 1); }
-    for (int i = 0; i < KTC_V8S; ++i) { mbar_init(v8_full + 8 * i, 1); mbar_init(v8_empty + 8 * i, 2); }
-    for (int i = 0; i < KTC_V16S; ++i) { mbar_init(v16_full + 8 * i, 2); mbar_init(v16_empty + 8 * i, 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(s_full + 8 * i, 1); mbar_init(p_full + 8 * i, 4); }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(k_full + 8 * i, 1);
+      mbar_init(k_empty + 8 * i, 1);
+      mbar_init(v8_full + 8 * i, 1);
+      mbar_init(v8_empty + 8 * i, 2);     // one arrival per converting warp
+      mbar_init(v16_full + 8 * i, 2);
+      mbar_init(v16_empty + 8 * i, 1);
+      mbar_init(s_full + 8 * i, 1);
+      mbar_init(p_full + 8 * i, 4);       // one arrival per softmax warp of the slot
+    }
     mbar_init(q_full, 1);
+    mbar_init(q_free, 1);
     mbar_init(o_free, 8);
     mbar_init(o_done, 1);
     mbar_init(drain, 1);
@@ -319,8 +326,8 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
     for (int seg = 0; go && !walk.done(sh); walk.next(p, sh), ++seg) {
       const KtcSeg sg(p, sh, walk);
       const int h = walk.it.h;
-      // The queries' pieces, once the last segment's products have read theirs.
-      if (seg > 0) go = __all_sync(0xffffffffu, mbar_wait(o_done, (seg - 1) & 1, abort_flag));
+      // The queries' pieces, once the last segment's scores are made.
+      if (seg > 0) go = __all_sync(0xffffffffu, mbar_wait(q_free, (seg - 1) & 1, abort_flag));
       if (!go) break;
       if (lane == 0) {
         const int row = (sg.b * p.c.heads + h) * rows_pad + sg.qt * KTC_QR;
@@ -359,7 +366,7 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
         pid = page_of(jb + 8);
         for (int i = 0; i < 4 && jb + i < sg.n; ++i, ++tiles) {
           const int sc = tiles % KTC_SCS;
-          if (to == i) {
+          if (to == i) {   // [ks x 8][log2 vs x 8][1 / vs x 8]
             float* at = reinterpret_cast<float*>(smem + L::SC_OFF) + sc * 32 + gi;
             at[0] = now.ks;
             at[8] = log2f(now.vs);
@@ -369,19 +376,18 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
           const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, lead)) * (p.c.page * 128);
           __syncwarp();
           if (lane == 0) mbar_arrive(sc_full + 8 * sc);
-          const int ks = tiles % KTC_KS, vs = tiles % KTC_V8S;
-          go = mbar_wait(k_empty + 8 * ks, ((tiles / KTC_KS) & 1) ^ 1, abort_flag);
-          go = __all_sync(0xffffffffu, go);
+          const int slot = tiles & 1;
+          const uint32_t phase = (tiles >> 1) & 1;
+          go = __all_sync(0xffffffffu, mbar_wait(k_empty + 8 * slot, phase ^ 1, abort_flag));
           if (!go) break;
-          if (lane == 0) mbar_arrive_expect_tx(k_full + 8 * ks, bytes);
+          if (lane == 0) mbar_arrive_expect_tx(k_full + 8 * slot, bytes);
           __syncwarp();
-          if (lead) tma_load_2d(sK + ks * KTC_TILE8 + gi * 2048, &tmK, k_full + 8 * ks, 0, now.row);
-          go = mbar_wait(v8_empty + 8 * vs, ((tiles / KTC_V8S) & 1) ^ 1, abort_flag);
-          go = __all_sync(0xffffffffu, go);
+          if (lead) tma_load_2d(sK + slot * KTC_TILE8 + gi * 2048, &tmK, k_full + 8 * slot, 0, now.row);
+          go = __all_sync(0xffffffffu, mbar_wait(v8_empty + 8 * slot, phase ^ 1, abort_flag));
           if (!go) break;
-          if (lane == 0) mbar_arrive_expect_tx(v8_full + 8 * vs, bytes);
+          if (lane == 0) mbar_arrive_expect_tx(v8_full + 8 * slot, bytes);
           __syncwarp();
-          if (lead) tma_load_2d(sV8 + vs * KTC_TILE8 + gi * 2048, &tmV, v8_full + 8 * vs, 0, now.row);
+          if (lead) tma_load_2d(sV8 + slot * KTC_TILE8 + gi * 2048, &tmV, v8_full + 8 * slot, 0, now.row);
         }
         now = next;
       }
@@ -389,8 +395,10 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
     // Loads still in flight must land before the CTA exits.
     if (lane == 0 && go) {
       if (queries > 0) mbar_wait_teardown(q_full, (queries - 1) & 1);
-      for (int t = max(0, tiles - KTC_KS); t < tiles; ++t) mbar_wait_teardown(k_full + 8 * (t % KTC_KS), (t / KTC_KS) & 1);
-      for (int t = max(0, tiles - KTC_V8S); t < tiles; ++t) mbar_wait_teardown(v8_full + 8 * (t % KTC_V8S), (t / KTC_V8S) & 1);
+      for (int t = max(0, tiles - 2); t < tiles; ++t) {
+        mbar_wait_teardown(k_full + 8 * (t & 1), (t >> 1) & 1);
+        mbar_wait_teardown(v8_full + 8 * (t & 1), (t >> 1) & 1);
+      }
     }
     __syncwarp();
   } else if (warp == 9) {
@@ -427,7 +435,7 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
             ktc_issue_pv(tm + 256 + t * 128, tm + t * 128, sV16 + vq * (2 * KTC_TILE8), s >= 2);
             if (last) umma_commit(v16_empty + 8 * vq);
           }
-          if (last && ++vq == KTC_V16S) { vq = 0; vpar ^= 1; }
+          if (last && ++vq == 2) { vq = 0; vpar ^= 1; }
         }
         if (s + 2 < steps) {
           if (first) ok = wait(k_full + 8 * kq, kpar);
@@ -438,12 +446,14 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
             umma_commit(s_full + 8 * t);
             if (last) umma_commit(k_empty + 8 * kq);
           }
-          if (last && ++kq == KTC_KS) { kq = 0; kpar ^= 1; }
+          if (last && ++kq == 2) { kq = 0; kpar ^= 1; }
         }
       };
       for (int s = -2; ok && s < steps; s += 2) {
         step(std::integral_constant<uint32_t, 0>{}, s);
+        if (issuer && s + 3 == steps) umma_commit(q_free);   // the last scores are made
         if (ok && s + 1 < steps) step(std::integral_constant<uint32_t, 1>{}, s + 1);
+        if (issuer && s + 4 == steps) umma_commit(q_free);
       }
       if (issuer) umma_commit(o_done);
     }
@@ -454,40 +464,37 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
     __syncwarp();
   } else {
     // --------------------------------------------- V codes -> f16 tiles
-    const int ct = threadIdx.x - 320;    // 0..63
+    // Warp 10 takes dims [0, 64), warp 11 [64, 128), 16 codes a lane and
+    // piece. Eight lanes take rows r and r ^ 5, four pieces each: loads and
+    // both stores of a piece then meet every bank once.
+    const int sub = lane >> 3, row8 = (lane & 4) ? sub ^ 5 : sub, c4 = lane & 3, half = warp - 10;
     int tiles = 0;
     bool ok = true;
     for (; ok && !walk.done(sh); walk.next(p, sh)) {
       const KtcSeg sg(p, sh, walk);
       for (int j = 0; ok && j < sg.n; ++j, ++tiles) {
-        const int vs = tiles % KTC_V8S, vd = tiles % KTC_V16S;
-        ok = mbar_wait(v8_full + 8 * vs, (tiles / KTC_V8S) & 1, abort_flag) &&
-             mbar_wait(v16_empty + 8 * vd, ((tiles / KTC_V16S) & 1) ^ 1, abort_flag);
+        const int slot = tiles & 1, live = sg.live(j);
+        const uint32_t phase = (tiles >> 1) & 1;
+        ok = mbar_wait(v8_full + 8 * slot, phase, abort_flag) && mbar_wait(v16_empty + 8 * slot, phase ^ 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        const uint32_t src = sV8 + vs * KTC_TILE8, dst = sV16 + vd * 2 * KTC_TILE8;
-        const int live = sg.live(j);
+        const uint32_t src = sV8 + slot * KTC_TILE8, dst = sV16 + slot * 2 * KTC_TILE8 + half * KTC_TILE8;
 #pragma unroll 4
         for (int i = 0; i < 16; ++i) {
-          // 16 codes (piece c of row r) -> two pieces of 8 f16 in column half c / 4.
-          const int id = i * 64 + ct, r = id >> 3, c = id & 7;
-          uint4 w = lds128(src + r * 128 + ((c ^ (r & 7)) << 4));
+          const int r = 8 * i + row8;
+          uint4 w = lds128(src + r * 128 + (((4 * half + c4) ^ row8) << 4));
           if (r >= live) w = make_uint4(0, 0, 0, 0);   // whatever lies there (NaN codes too) counts for nothing
-          const uint4 lo = make_uint4(e4m3x2_to_f16x2(w.x & 0xffffu), e4m3x2_to_f16x2(w.x >> 16),
-                                      e4m3x2_to_f16x2(w.y & 0xffffu), e4m3x2_to_f16x2(w.y >> 16));
-          const uint4 hi = make_uint4(e4m3x2_to_f16x2(w.z & 0xffffu), e4m3x2_to_f16x2(w.z >> 16),
-                                      e4m3x2_to_f16x2(w.w & 0xffffu), e4m3x2_to_f16x2(w.w >> 16));
-          // The lanes of the two halves store their pieces in opposite order: no bank twice.
-          const uint32_t at = dst + (c >> 2) * KTC_TILE8 + r * 128;
-          const int k0 = (c & 3) * 2, first = c >> 2;
-          sts128(at + (((k0 + first) ^ (r & 7)) << 4), first ? hi : lo);
-          sts128(at + (((k0 + 1 - first) ^ (r & 7)) << 4), first ? lo : hi);
+          const uint32_t at = dst + r * 128;
+          sts128(at + (((2 * c4) ^ row8) << 4), make_uint4(e4m3x2_to_f16x2(w.x), e4m3x2_hi_to_f16x2(w.x),
+                                                           e4m3x2_to_f16x2(w.y), e4m3x2_hi_to_f16x2(w.y)));
+          sts128(at + (((2 * c4 + 1) ^ row8) << 4), make_uint4(e4m3x2_to_f16x2(w.z), e4m3x2_hi_to_f16x2(w.z),
+                                                               e4m3x2_to_f16x2(w.w), e4m3x2_hi_to_f16x2(w.w)));
         }
         fence_proxy_async();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(v16_full + 8 * vd);
-          mbar_arrive(v8_empty + 8 * vs);
+          mbar_arrive(v16_full + 8 * slot);
+          mbar_arrive(v8_empty + 8 * slot);
         }
       }
     }
@@ -639,11 +646,10 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
       float* part = p.part + static_cast<size_t>(2 * blockIdx.x + (sg.begins ? 1 : 0)) * kv8_part_floats<KTC_QR>();
       const int prow = (sg.two ? t * 128 : 0) + r;
       const int hq = h * p.group + rr - tok * p.group;
-      __nv_bfloat16* orow = p.out + sg.b * p.o_sb + tok * p.o_st + hq * p.o_sh;
       float wA = 1.f, wB = 0.f, den = l, M = m;
       if (!sg.two) {
         // Both slots hold the same rows: slot t finishes columns [64 t, +64).
-        float* xm = reinterpret_cast<float*>(smem + L::XCH_OFF);
+        float* xm = reinterpret_cast<float*>(smem + L::STAGE_OFF);
         xm[t * 256 + r] = m;
         xm[t * 256 + 128 + r] = l;
         asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -659,6 +665,11 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
       const int chunks = sg.two ? 4 : 2;
       const uint32_t src = sg.two ? tO : tmem + lane_base + 256 + t * 64;
       const int col0 = sg.two ? 0 : t * 64;
+      // 32 columns at a time go through 4 KB of the warp's own, so that global
+      // memory sees whole 128-byte (bf16: 64-byte) pieces of rows. (A thread
+      // storing its own row took ~9400 cycles a segment.)
+      const uint32_t stage = base + L::STAGE_OFF + warp * 4096;
+      const int row0 = sg.qt * KTC_QR + prow - lane;        // first row of the warp
 #pragma unroll 1
       for (int c = 0; ok && c < chunks; ++c) {
         float o[32];
@@ -674,16 +685,35 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
 #pragma unroll
           for (int k = 0; k < 32; ++k) o[k] = has_b ? o[k] * wA + o1[k] * wB : o[k] * wA;
         }
-        if (valid && whole) {
-          uint4* dst = reinterpret_cast<uint4*>(orow + col0 + c * 32);
+        __syncwarp();     // the last columns have been read
+        const int sub = lane >> 3, c8 = lane & 7;
+        if (whole) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            dst[k] = make_uint4(pack_bf16(o[8 * k] * inv, o[8 * k + 1] * inv), pack_bf16(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
-                                pack_bf16(o[8 * k + 4] * inv, o[8 * k + 5] * inv), pack_bf16(o[8 * k + 6] * inv, o[8 * k + 7] * inv));
-        } else if (valid) {
-          float4* dst = reinterpret_cast<float4*>(part + prow * 128 + col0 + c * 32);
+            sts128(stage + lane * 128 + ((k ^ (lane & 7)) << 4),
+                   make_uint4(pack_bf16(o[8 * k] * inv, o[8 * k + 1] * inv), pack_bf16(o[8 * k + 2] * inv, o[8 * k + 3] * inv),
+                              pack_bf16(o[8 * k + 4] * inv, o[8 * k + 5] * inv), pack_bf16(o[8 * k + 6] * inv, o[8 * k + 7] * inv)));
+          __syncwarp();
+          // Four lanes to a row, eight rows at a time.
+          for (int i = 0; i < 4; ++i) {
+            const int rl = 8 * i + (lane >> 2), row = row0 + rl, k = lane & 3;
+            if (row >= sg.qt * KTC_QR + sg.rows) continue;
+            const int tk = row / p.group;
+            __nv_bfloat16* to = p.out + sg.b * p.o_sb + tk * p.o_st + (h * p.group + row - tk * p.group) * p.o_sh;
+            *reinterpret_cast<uint4*>(to + col0 + c * 32 + k * 8) = lds128(stage + rl * 128 + ((k ^ (rl & 7)) << 4));
+          }
+        } else {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) dst[k] = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          for (int k = 0; k < 8; ++k)
+            sts128(stage + lane * 128 + ((k ^ (lane & 7)) << 4),
+                   make_uint4(__float_as_uint(o[4 * k]), __float_as_uint(o[4 * k + 1]), __float_as_uint(o[4 * k + 2]),
+                              __float_as_uint(o[4 * k + 3])));
+          __syncwarp();
+          for (int i = 0; i < 8; ++i) {
+            const int rl = 4 * i + sub, pr = prow - lane + rl;
+            if (pr < sg.rows)
+              *reinterpret_cast<uint4*>(part + pr * 128 + col0 + c * 32 + c8 * 4) = lds128(stage + rl * 128 + ((c8 ^ (rl & 7)) << 4));
+          }
         }
       }
       tc_fence_before();
