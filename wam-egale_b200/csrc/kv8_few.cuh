@@ -242,9 +242,11 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
     float l = 0.f;
     if (row < rows) {
       float m = -INFINITY;
-      for (int i = lane; i < cnt; i += 32) m = fmaxf(m, __ldcg(slot(i) + QR * 128 + row));
+      if (step == 8) {
+        for (int i = lane; i < cnt; i += 32) m = fmaxf(m, __ldcg(slot(i) + QR * 128 + row));
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      }
       for (int i0 = from; i0 < cnt; i0 += 8 * step) {
         float4 v[8];
         float mk[8], lk[8];
@@ -257,6 +259,11 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
             mk[u] = __ldcg(slot(i) + QR * 128 + row);
             lk[u] = __ldcg(slot(i) + QR * 129 + row);
           }
+        }
+        if (step == 1) {   // all partials of the row are here
+#pragma unroll
+          for (int u = 0; u < 8; ++u)
+            if (lk[u] != 0.f) m = fmaxf(m, mk[u]);
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
