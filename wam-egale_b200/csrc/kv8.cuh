@@ -466,35 +466,42 @@ __global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8Ev
 
 // One block per (new page, head, sequence): gathers the kept rows of K and V
 // into registers, takes the new scales from their values and rounds them once.
-// kept lists the rows, -1 behind the last.
+// kept lists the rows, -1 behind the last. Eight lanes take 16 bytes each of a
+// row, so that a warp's load spans four rows and a thread holds all its loads of
+// K and V in flight at once; half as many threads with twice the bytes each
+// measured 16 us less at 8 sequences x 8 heads of 32k tokens than 16 lanes of 8.
 template <int PAGE>
-__global__ void __launch_bounds__(PAGE == 128 ? 512 : 256, PAGE == 128 ? 2 : 4) kv8_gather_kernel(const Kv8EvictParams p) {
+__global__ void __launch_bounds__(PAGE == 128 ? 256 : 128, PAGE == 128 ? 3 : 6) kv8_gather_kernel(const Kv8EvictParams p) {
   pdl_wait();
-  constexpr int THREADS = PAGE == 128 ? 512 : 256, ROWS = THREADS / 16, PASSES = PAGE / ROWS;
+  // Eight lanes hold a row, 16 codes each.
+  constexpr int THREADS = PAGE == 128 ? 256 : 128, ROWS = THREADS / 8, PASSES = PAGE / ROWS;
   __shared__ float red[2][THREADS / 32];
   const int h = blockIdx.y, b = blockIdx.z;
-  const int c8 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+  const int c16 = threadIdx.x & 7, r0 = threadIdx.x >> 3;
   const int* kept = p.kept + ((static_cast<long long>(b) * p.c.heads + h) * p.new_width + blockIdx.x) * PAGE;
   int pos[PASSES];
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) pos[i] = kept[r0 + ROWS * i];
+  const int dst = __ldg(p.new_table + static_cast<long long>(b) * p.new_width + blockIdx.x);
   if (__syncthreads_and(pos[0] < 0)) return;   // the page receives nothing (row 0 is kept first)
-  const int dst = kv8_page(p.new_table, p.new_width, p.c, b, blockIdx.x);
-  if (dst < 0) return;
+  if (dst < 0 || dst >= p.c.pages) {
+    if (threadIdx.x == 0) record_error(KV8_DEV_ERROR);
+    return;
+  }
   const int* table = p.s.table + static_cast<long long>(b) * p.s.width;
-  uint2 raw[2][PASSES];
+  uint4 raw[2][PASSES];
   float sc[2][PASSES];
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
-    raw[0][i] = raw[1][i] = make_uint2(0, 0);
+    raw[0][i] = raw[1][i] = make_uint4(0, 0, 0, 0);
     sc[0][i] = sc[1][i] = 0.f;
     if (pos[i] >= 0) {
       const int pid = __ldg(table + pos[i] / PAGE);
       if (pid >= 0 && pid < p.c.pages) {
         const int blk = pid * p.c.heads + h;      // rows of codes are below 2^31
-        const long long at = (static_cast<long long>(blk) * PAGE + pos[i] % PAGE) * 128 + c8 * 8;
-        raw[0][i] = *reinterpret_cast<const uint2*>(p.c.k8 + at);
-        raw[1][i] = *reinterpret_cast<const uint2*>(p.c.v8 + at);
+        const long long at = (static_cast<long long>(blk) * PAGE + pos[i] % PAGE) * 128 + c16 * 16;
+        raw[0][i] = *reinterpret_cast<const uint4*>(p.c.k8 + at);
+        raw[1][i] = *reinterpret_cast<const uint4*>(p.c.v8 + at);
         sc[0][i] = p.c.k_scale[blk];
         sc[1][i] = p.c.v_scale[blk];
       } else {
@@ -508,10 +515,12 @@ __global__ void __launch_bounds__(PAGE == 128 ? 512 : 256, PAGE == 128 ? 2 : 4) 
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
       __half2 m = __floats2half2_rn(0.f, 0.f);     // codes are exact in f16; NaN loses
+      const uint32_t w[4] = {raw[x][i].x, raw[x][i].y, raw[x][i].z, raw[x][i].w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const uint32_t u = e4m3x2_to_f16x2((k < 2 ? raw[x][i].x : raw[x][i].y) >> (16 * (k & 1)));
-        m = __hmax2(m, __habs2(*reinterpret_cast<const __half2*>(&u)));
+        const uint32_t lo = e4m3x2_to_f16x2(w[k]), hi = e4m3x2_hi_to_f16x2(w[k]);
+        m = __hmax2(m, __habs2(*reinterpret_cast<const __half2*>(&lo)));
+        m = __hmax2(m, __habs2(*reinterpret_cast<const __half2*>(&hi)));
       }
       const float2 v = __half22float2(m);
       amax = fmaxf(amax, fmaxf(v.x, v.y) * sc[x][i]);
@@ -528,17 +537,22 @@ __global__ void __launch_bounds__(PAGE == 128 ? 512 : 256, PAGE == 128 ? 2 : 4) 
 #pragma unroll
     for (int i = 1; i < THREADS / 32; ++i) m = fmaxf(m, red[x][i]);
     const float s = pow2f_exact(kv8_scale_exp(m)), inv = 1.f / s;
-    uint8_t* to = (x ? p.c.v8 : p.c.k8) + static_cast<long long>(blk) * (PAGE * 128) + c8 * 8;
+    uint8_t* to = (x ? p.c.v8 : p.c.k8) + static_cast<long long>(blk) * (PAGE * 128) + c16 * 16;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
       if (pos[i] < 0) continue;
-      float f[8];
-      e4m3x8_to_float(raw[x][i], f);
       // inv is a power of two, so the factor is exact (a block of zeros may meet a huge old scale).
       const float factor = fminf(sc[x][i] * inv, 3.402823466e38f);
+      uint2 part[2];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] *= factor;
-      *reinterpret_cast<uint2*>(to + (r0 + ROWS * i) * 128) = pack_e4m3x8(f);
+      for (int k = 0; k < 2; ++k) {
+        float f[8];
+        e4m3x8_to_float(k ? make_uint2(raw[x][i].z, raw[x][i].w) : make_uint2(raw[x][i].x, raw[x][i].y), f);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) f[q] *= factor;
+        part[k] = pack_e4m3x8(f);
+      }
+      *reinterpret_cast<uint4*>(to + (r0 + ROWS * i) * 128) = make_uint4(part[0].x, part[0].y, part[1].x, part[1].y);
     }
     if (threadIdx.x == 0) (x ? p.c.v_scale : p.c.k_scale)[blk] = s;
   }

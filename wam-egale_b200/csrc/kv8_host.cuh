@@ -136,10 +136,10 @@ inline int kv8_evict_impl(const wamb_kv8_evict_args* a, cudaStream_t s) {
   if (rc) return rc;
   const dim3 grid(p.new_width, p.c.heads, p.s.batch);
   switch (p.c.page) {
-    case 16: return launch_kernel(kv8_gather_kernel<16>, grid, dim3(256), 0, s, p);
-    case 32: return launch_kernel(kv8_gather_kernel<32>, grid, dim3(256), 0, s, p);
-    case 64: return launch_kernel(kv8_gather_kernel<64>, grid, dim3(256), 0, s, p);
-    default: return launch_kernel(kv8_gather_kernel<128>, grid, dim3(512), 0, s, p);
+    case 16: return launch_kernel(kv8_gather_kernel<16>, grid, dim3(128), 0, s, p);
+    case 32: return launch_kernel(kv8_gather_kernel<32>, grid, dim3(128), 0, s, p);
+    case 64: return launch_kernel(kv8_gather_kernel<64>, grid, dim3(128), 0, s, p);
+    default: return launch_kernel(kv8_gather_kernel<128>, grid, dim3(256), 0, s, p);
   }
 }
 
@@ -148,7 +148,9 @@ inline int kv8_evict_impl(const wamb_kv8_evict_args* a, cudaStream_t s) {
 inline int kv8_few_ctas(const DeviceInfo& di, bool weights = false) { return (weights ? 4 : 3) * di.sms; }
 
 // A tile of 16 rows is one m16n8k16 operand; more rows go to the tcgen05
-// kernel, which reads each key once for 256 of them.
+// kernel, which reads each key once for 256 of them. Two tiles of 16 measured
+// slower: 17 rows over 16k keys 93 us against 85, 32 rows of 4 sequences 59
+// against 48 (only short caches gain: 32 rows over 2000 keys 24 against 33).
 inline bool kv8_is_few(int64_t rows) { return rows <= FEW_QR; }
 
 // Query rows of a sequence and cached head.
