@@ -424,8 +424,10 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
         constexpr uint32_t t = decltype(slot)::value;
         const bool last = t == 1 || !two;     // of the key tile
         const bool first = t == 0 || !two;
+        // What is there long before P is waited for first.
+        if (s + 2 < steps && first) ok = wait(k_full + 8 * kq, kpar);
         if (s >= 0) {
-          if (s == 0 && seg > 0) ok = wait(o_free, (seg - 1) & 1);   // the last segment's output has left TMEM
+          if (s == 0 && seg > 0) ok = ok && wait(o_free, (seg - 1) & 1);   // the last segment's output has left TMEM
           if (first) ok = ok && wait(v16_full + 8 * vq, vpar);
           ok = ok && wait(p_full + 8 * t, (ppar >> t) & 1);
           if (!ok) return;
@@ -438,7 +440,6 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
           if (last && ++vq == 2) { vq = 0; vpar ^= 1; }
         }
         if (s + 2 < steps) {
-          if (first) ok = wait(k_full + 8 * kq, kpar);
           if (!ok) return;
           tc_fence_after();
           if (issuer) {
