@@ -483,7 +483,7 @@ WAMB_API int wamb_cfg_combine(const void* cond, const void* uncond, int32_t io_i
  * is 2^n, n the smallest whole number in [-40, 119] with the block's largest
  * magnitude <= 448 * 2^n; a value is e4m3(x / scale), rounded to nearest
  * even, saturating; NaN stays NaN. (Scales written by others may be any
- * positive finite number.)
+ * positive finite number.) At most 2^30 positions a sequence.
  *
  * lens, counts, tables live on the device and are read there: a call can be
  * captured in a graph and replayed with other lengths. A page id outside
@@ -571,8 +571,9 @@ WAMB_API int wamb_kv8_weights(const wamb_kv8_attention_args* args, void* stream)
  * kept [batch, heads, new_width * page] lists their old positions (-1 behind
  * the last), new_weights their weights (0 behind the last), new_lens their
  * number min(lens[b], heavy + recent). The old pages are not changed and may
- * be freed afterwards; a page of a sequence's old table in its new one is
- * refused (WAMB_DEV_KV8), and no new page may be in use elsewhere.
+ * be freed afterwards; a sequence with a page of its old table in its new
+ * one, or with one new page twice, is refused (WAMB_DEV_KV8: it keeps nothing),
+ * and no new page may be in use by another sequence of the call or elsewhere.
  * max_len: an upper bound of lens that the caller knows (at most
  * table_width * page); min(heavy + recent, max_len) must fit new_width pages. */
 typedef struct wamb_kv8_evict_args {

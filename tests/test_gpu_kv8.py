@@ -491,6 +491,54 @@ def test_bad_pages_and_lengths_are_reported(cuda_device):
     assert _lib.device_status() == 0
 
 
+def test_evict_refuses_a_new_page_named_twice(cuda_device):
+    """Two blocks would write it: the sequence keeps nothing, the other one is served."""
+    c, table, free, n, g = _setup(2, 2, 16, [200, 150], 47, spare=6, poison=False)
+    w = torch.rand(2, 2, table.shape[1] * 16, generator=g).to(DEV)
+    new = free[:6].view(2, 3).contiguous()
+    new[0, 2] = new[0, 0]
+    before = c.k8[new[0].long()].view(torch.uint8).clone()
+    kept, weights, lens = c.evict(table, n, w, new, heavy=30, recent=10)
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 5
+    assert lens.tolist() == [0, 40]
+    assert (kept[0] == -1).all() and (weights[0] == 0).all()
+    assert torch.equal(c.k8[new[0].long()].view(torch.uint8), before)
+    for h in range(2):
+        assert kept[1, h, :40].tolist() == list(ok.keep(w[1, h].cpu(), 150, 30, 10))
+    # A repeat behind the pages that receive rows does no harm.
+    new = free[:6].view(2, 3).contiguous()
+    new[:, 2] = new[:, 0]
+    _, _, lens = c.evict(table, n, w, new, heavy=20, recent=10)
+    torch.cuda.synchronize()
+    assert _lib.device_status() == 0 and lens.tolist() == [30, 30]
+
+
+# ------------------------------------------------- refusals of the handle
+def test_handle_refuses_gradients_and_expanded_outputs(cuda_device):
+    c, table, free, n, g = _setup(2, 2, 16, [40, 20], 43)
+    q = _q(g, 2, 3, 4, 128)
+    leaf = q.clone().requires_grad_()
+    for f in (lambda: c.attention(leaf, table, n), lambda: c.write(q[:, :, :2], leaf[:, :, :2], table, n)):
+        with pytest.raises(RuntimeError, match="inference-only"):
+            f()
+    with pytest.raises(ValueError, match="expanded"):
+        c.attention(q, table, n, out=q.new_empty(1, 3, 4, 128).expand(2, 3, 4, 128))
+    with torch.no_grad():
+        got = c.attention(leaf, table, n)
+    assert torch.equal(got, c.attention(q, table, n))
+
+
+def test_strides_of_single_entries_are_free(cuda_device):
+    """One token's stride, or one sequence's, may be any number."""
+    c, table, free, n, g = _setup(1, 2, 16, [40], 44)
+    q = _q(g, 1, 1, 4, 128)
+    odd = torch.as_strided(q, (1, 1, 4, 128), (3, 5, 128, 1))
+    out = torch.empty_like(q)
+    c.attention(odd, table, n, out=torch.as_strided(out, (1, 1, 4, 128), (7, 1, 128, 1)))
+    assert torch.equal(out, c.attention(q, table, n))
+
+
 # ------------------------------------------- many tiles behind one another
 @pytest.mark.parametrize("B,H,G,T,L,causal", [(1, 2, 1, 880, 4400, False), (2, 1, 2, 700, 3000, True), (3, 2, 1, 100, 2500, False)])
 def test_weights_many_tiles(cuda_device, B, H, G, T, L, causal):

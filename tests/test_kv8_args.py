@@ -168,3 +168,13 @@ def test_oracle_keep():
     assert ok.keep([1.0, 3.0, 3.0, 0.0, 9.0], 4, 2, 1) == [1, 2, 3]
     assert ok.keep([1.0, float("nan"), 0.0], 3, 1, 0) == [1]
     assert ok.keep([1.0, 2.0], 2, 0, 5) == [0, 1]
+
+
+@pytest.mark.parametrize("make,call", [(_write, "wamb_kv8_write"), (_attention, "wamb_kv8_attention"),
+                                       (_attention, "wamb_kv8_weights"), (_evict, "wamb_kv8_evict")])
+def test_refuses_more_positions_than_tiles_can_count(make, call):
+    """2^30 cached positions and one new token: 32-bit tile ends behind them must not wrap."""
+    lib = _lib.load()
+    assert getattr(lib, call)(make(s_table_width=1 << 24, s_tokens=1), None) == 2
+    assert b"2^30" in lib.wamb_last_error()
+

@@ -427,7 +427,7 @@ WAMB_DEV void kv8_select_heavy(const Kv8Kept& k, const float* w, Kv8SelSmem& sm,
 // writes the kept positions. The weights are read once into shared memory, or
 // from L2 in each pass where a head has more than 36864; eight loads of a
 // thread are in flight. Bound by that one SM's instructions. A sequence whose
-// new pages overlap its old ones is refused: it keeps nothing.
+// new pages overlap its old ones, or one another, is refused: it keeps nothing.
 __global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8EvictParams p, const int list_at) {
   pdl_wait();
   extern __shared__ uint32_t keys[];
@@ -442,10 +442,15 @@ __global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8Ev
   float* nw = p.new_weights + out0;
 
   const int new_pages = (k.total + p.c.page - 1) >> p.c.page_log2, old_pages = (k.len + p.c.page - 1) >> p.c.page_log2;
+  const int* fresh = p.new_table + static_cast<long long>(b) * p.new_width;
   bool overlap = false;
+  for (int n = tid; n < new_pages; n += KV8_SEL_THREADS) {   // a page that is named twice would be written by two blocks
+    const int page = __ldg(fresh + n);
+    for (int m = 0; m < n; ++m) overlap |= __ldg(fresh + m) == page;
+  }
   for (int o = tid; o < old_pages; o += KV8_SEL_THREADS) {
     const int page = __ldg(p.s.table + static_cast<long long>(b) * p.s.width + o);
-    for (int n = 0; n < new_pages; ++n) overlap |= __ldg(p.new_table + static_cast<long long>(b) * p.new_width + n) == page;
+    for (int n = 0; n < new_pages; ++n) overlap |= __ldg(fresh + n) == page;
   }
   if (__syncthreads_or(overlap)) {
     if (tid == 0) record_error(KV8_DEV_ERROR);

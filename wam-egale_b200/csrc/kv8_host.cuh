@@ -30,8 +30,9 @@ inline int kv8_cache_check(const wamb_kv8_cache* c, Kv8Cache* out) {
 inline int kv8_seqs_check(const wamb_kv8_seqs* s, int page, Kv8Seqs* out) {
   WAMB_REQUIRE(s->batch >= 0 && s->batch <= 32767 && s->tokens >= 0 && s->table_width > 0, WAMB_ERR_SHAPE,
                "kv8: batch %d (0..32767), tokens %d, table_width %d", s->batch, s->tokens, s->table_width);
-  WAMB_REQUIRE(static_cast<int64_t>(s->table_width) * page + s->tokens <= INT32_MAX, WAMB_ERR_SHAPE,
-               "kv8: %d pages of %d tokens and %d new tokens exceed 2^31 - 1 positions", s->table_width, page, s->tokens);
+  // Positions and their tiles' ends stay far from the 32-bit limit.
+  WAMB_REQUIRE(static_cast<int64_t>(s->table_width) * page + s->tokens <= (1 << 30), WAMB_ERR_SHAPE,
+               "kv8: %d pages of %d tokens and %d new tokens exceed 2^30 positions", s->table_width, page, s->tokens);
   WAMB_REQUIRE(s->batch == 0 || (s->table && s->lens), WAMB_ERR_ARG, "kv8: null table or lens");
   out->table = s->table;
   out->lens = s->lens;
@@ -101,7 +102,7 @@ inline int kv8_evict_impl(const wamb_kv8_evict_args* a, cudaStream_t s) {
   if (rc) return rc;
   p.s.counts = nullptr;
   WAMB_REQUIRE(a->heavy >= 0 && a->recent >= 0, WAMB_ERR_ARG, "kv8 evict: heavy %d, recent %d", a->heavy, a->recent);
-  WAMB_REQUIRE(a->new_width > 0 && static_cast<int64_t>(a->new_width) * p.c.page <= INT32_MAX, WAMB_ERR_SHAPE,
+  WAMB_REQUIRE(a->new_width > 0 && static_cast<int64_t>(a->new_width) * p.c.page <= (1 << 30), WAMB_ERR_SHAPE,
                "kv8 evict: new_width %d", a->new_width);
   const int64_t cap = static_cast<int64_t>(p.s.width) * p.c.page;
   const int64_t most = std::min<int64_t>(static_cast<int64_t>(a->heavy) + a->recent, a->max_len);

@@ -73,14 +73,18 @@ class Kv8Cache:
             seqs.counts = self._ints("counts", counts, (batch,))
 
     def _rows(self, name, t, heads=None, dtypes=(torch.bfloat16,)):
-        """[batch, tokens, heads, 128] with rows of 128 contiguous values."""
+        """Strides of [batch, tokens, heads, 128] with rows of 128 contiguous values."""
         if t.dim() != 4 or t.shape[3] != HEAD_DIM or t.dtype not in dtypes or t.device != self.device:
             raise ValueError(f"{name} must be [batch, tokens, heads, 128] {' or '.join(map(str, dtypes))} on {self.device}")
         if heads is not None and t.shape[2] != heads:
             raise ValueError(f"{name} has {t.shape[2]} heads, the cache {heads}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError("Kv8Cache is inference-only; use no_grad/inference_mode")
         if t.stride(3) != 1:
             raise ValueError(f"{name} must have unit stride along the head dim")
-        return t.stride()[:3]
+        b, s = t.shape, t.stride()
+        # The stride of a single entry may be anything; the C ABI is told 0.
+        return s[0] if b[0] > 1 else 0, s[1] if b[1] > 1 else 0, s[2] if b[2] > 1 else 0
 
     def _weight(self, name, t, batch, width):
         if t.dtype != torch.float32 or t.dim() != 3 or t.shape[:2] != (batch, self.heads) or not t.is_contiguous() \
@@ -110,7 +114,7 @@ class Kv8Cache:
     # ---------------------------------------------------------- operators
     def write(self, k, v, table, lens, counts=None):
         """Rows t < counts[b] (all without `counts`) of k, v [batch, tokens,
-        heads, 128] (bf16 or fp32, any strides that are multiples of 8) go to
+        heads, 128] (bf16 or fp32, any strides that are multiples of 8 elements) go to
         positions lens[b] + t. A page that already holds positions keeps the
         larger of its scale and the new rows'; its codes follow. `lens` is not
         changed."""
@@ -151,6 +155,8 @@ class Kv8Cache:
             out = q.new_empty(q.shape)
         elif out.shape != q.shape:
             raise ValueError("out must be shaped like q")
+        elif any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
+            raise ValueError("out must not be an expanded tensor")
         a.out_stride[:] = self._rows("out", out)
         a.out = out.data_ptr()
         if lse is None and return_lse:
@@ -190,7 +196,7 @@ class Kv8Cache:
         """Keeps, for each sequence and cached head, the last `recent` positions
         and the `heavy` earlier ones with the largest weights (ties: the lowest
         positions), and moves their rows, in order, to the pages of new_table
-        (int32 [batch, new_width]; pages that no live table names). Returns
+        (int32 [batch, new_width]; pages that no live table names, each once). Returns
         (kept [batch, heads, new_width * page] int32 old positions, -1 behind
         the last; their weights, 0 behind the last; new lengths int32 [batch]).
         max_len: an upper bound of lens (default: the table's capacity);
