@@ -262,13 +262,36 @@ constexpr uint32_t KV8_SEL_SMEM = (KV8_SEL_KEYS + KV8_SEL_LIST) * 4;
 
 struct Kv8SelSmem {
   int hist[KV8_SEL_COPIES][KV8_SEL_BINS];
-  int wsum[32], pick[2], listed;
+  uint32_t wsum[32];
+  int pick[2], listed;
 };
+
+// Exclusive sum over the block's threads of v, and the sum of all.
+WAMB_DEV uint32_t kv8_block_scan(Kv8SelSmem& sm, uint32_t v, uint32_t& all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  uint32_t inc = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t u = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += u;
+  }
+  if (lane == 31) sm.wsum[warp] = inc;
+  __syncthreads();
+  uint32_t sums = sm.wsum[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint32_t u = __shfl_up_sync(0xffffffffu, sums, o);
+    if (lane >= o) sums += u;
+  }
+  const uint32_t before = __shfl_sync(0xffffffffu, sums, (warp + 31) & 31);
+  all = __shfl_sync(0xffffffffu, sums, 31);
+  return inc - v + (warp > 0 ? before : 0);
+}
 
 // The bin, counted from the highest, that holds the `need`-th largest key of
 // the histogram, and how many of that bin are needed. Whole block.
 WAMB_DEV void kv8_pick_bin(Kv8SelSmem& sm, int need) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x;
   __syncthreads();
   // Each thread owns two bins, highest first: thread t has bins 2047 - 2t, 2046 - 2t.
   int c[2], mine = 0;
@@ -280,16 +303,8 @@ WAMB_DEV void kv8_pick_bin(Kv8SelSmem& sm, int need) {
     for (int q = 0; q < KV8_SEL_COPIES; ++q) c[j] += sm.hist[q][bin];
     mine += c[j];
   }
-  int inc = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += v;
-  }
-  if (lane == 31) sm.wsum[warp] = inc;
-  __syncthreads();
-  int above = inc - mine;
-  for (int q = 0; q < warp; ++q) above += sm.wsum[q];
+  uint32_t all;
+  int above = kv8_block_scan(sm, mine, all);
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     if (above < need && need <= above + c[j]) {
@@ -305,12 +320,37 @@ WAMB_DEV void kv8_clear_hist(Kv8SelSmem& sm) {
   __syncthreads();
 }
 
+// A thread's run of a piece of keys, of an odd length so that the threads of a
+// warp meet different banks, and at most 31 so that a word marks its keys.
+constexpr int KV8_SEL_PIECE = 31 * KV8_SEL_THREADS;
+struct Kv8Run {
+  int from, len;
+  WAMB_DEV explicit Kv8Run(int n) {
+    const int c = (n + KV8_SEL_THREADS - 1) / KV8_SEL_THREADS | 1;
+    from = min(n, static_cast<int>(threadIdx.x) * c);
+    len = min(n - from, c);
+  }
+  // Bit j: f(key j of the run).
+  template <typename F>
+  WAMB_DEV uint32_t mark(const uint32_t* keys, F f) const {
+    uint32_t m = 0;
+    for (int j0 = 0; j0 < len; j0 += 8) {
+      uint32_t part = 0;
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        if (j0 + u < len && f(keys[from + j0 + u])) part |= 1u << u;
+      m |= part << j0;
+    }
+    return m;
+  }
+};
+
 // Keeps k.heavy of the positions [0, k.old) and writes them, in order.
 // HELD: the keys fit shared memory.
 template <bool HELD>
 WAMB_DEV void kv8_select_heavy(const Kv8Kept& k, const float* w, Kv8SelSmem& sm, uint32_t* keys, uint32_t* list, int* kept,
                                float* nw) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, warp = tid >> 5;
   auto key_at = [&](int i) { return HELD ? keys[i] : weight_key(__ldg(w + i)); };
   const bool select = k.heavy < k.old;
   int* hist = sm.hist[warp & (KV8_SEL_COPIES - 1)];
@@ -340,16 +380,31 @@ WAMB_DEV void kv8_select_heavy(const Kv8Kept& k, const float* w, Kv8SelSmem& sm,
     // them alone (at all keys again where the list overflows).
     if (tid == 0) sm.listed = 0;
     __syncthreads();
-    for (int i0 = tid; i0 < k.old; i0 += 8 * KV8_SEL_THREADS) {
-      uint32_t key[8];
+    if (HELD) {          // (atomics on one counter took 7 cycles a key)
+      int listed = 0;
+      for (int base = 0; base < k.old; base += KV8_SEL_PIECE) {
+        const Kv8Run run(min(KV8_SEL_PIECE, k.old - base));
+        uint32_t m = run.mark(keys + base, [&](uint32_t key) { return (key ^ prefix) >> 21 == 0; });
+        uint32_t all;
+        int at = listed + static_cast<int>(kv8_block_scan(sm, __popc(m), all));
+        for (; m != 0; m &= m - 1, ++at)
+          if (at < KV8_SEL_LIST) list[at] = keys[base + run.from + __ffs(m) - 1];
+        listed += static_cast<int>(all);
+        __syncthreads();            // the sums are rewritten
+      }
+      if (tid == 0) sm.listed = listed;
+    } else {
+      for (int i0 = tid; i0 < k.old; i0 += 8 * KV8_SEL_THREADS) {
+        uint32_t key[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) key[u] = i0 + u * KV8_SEL_THREADS < k.old ? key_at(i0 + u * KV8_SEL_THREADS) : ~prefix;
+        for (int u = 0; u < 8; ++u) key[u] = i0 + u * KV8_SEL_THREADS < k.old ? key_at(i0 + u * KV8_SEL_THREADS) : ~prefix;
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if ((key[u] ^ prefix) >> 21 == 0) {
-          const int at = atomicAdd(&sm.listed, 1);
-          if (at < KV8_SEL_LIST) list[at] = key[u];
-        }
+        for (int u = 0; u < 8; ++u)
+          if ((key[u] ^ prefix) >> 21 == 0) {
+            const int at = atomicAdd(&sm.listed, 1);
+            if (at < KV8_SEL_LIST) list[at] = key[u];
+          }
+      }
     }
     __syncthreads();
     const bool short_list = sm.listed <= KV8_SEL_LIST;
@@ -369,55 +424,48 @@ WAMB_DEV void kv8_select_heavy(const Kv8Kept& k, const float* w, Kv8SelSmem& sm,
       __syncthreads();
     }
   }
-  // Ordered compaction, four neighbours to a thread: keys above the threshold
-  // and, of those equal to it, the `need` lowest positions.
+  // Ordered compaction: keys above the threshold and, of those equal to it, the
+  // `need` lowest positions. A thread marks the kept ones of its run; the runs
+  // before it tell their places; the positions then lie in shared memory, over
+  // the keys, and leave it in order. (Ballots and population counts of a warp's
+  // neighbouring keys took twice as long.)
   int done = 0, eq_done = 0;
-  __syncthreads();
-  for (int i0 = 0; i0 < k.old; i0 += 4 * KV8_SEL_THREADS) {
-    const int i = i0 + 4 * tid;
-    int gt = 0, eq = 0;            // bit u: neighbour u
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-      if (i + u < k.old) {
-        const uint32_t key = select ? key_at(i + u) : 1u;
-        gt |= (!select || key > prefix) << u;
-        eq |= (select && key == prefix) << u;
-      }
-    const int mine = __popc(gt) | (__popc(eq) << 16);
-    int inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += u;
+  for (int base = 0; base < k.old; base += KV8_SEL_PIECE) {
+    const int n = min(KV8_SEL_PIECE, k.old - base);
+    if (!HELD && select) {
+      for (int i = tid; i < n; i += KV8_SEL_THREADS) keys[i] = weight_key(__ldg(w + base + i));
     }
-    if (lane == 31) sm.wsum[warp] = inc;
     __syncthreads();
-    int all = sm.wsum[lane];
+    const Kv8Run run(n);
+    const uint32_t* piece = HELD ? keys + base : keys;
+    uint32_t keep = select ? run.mark(piece, [&](uint32_t key) { return key > prefix; }) : (1u << run.len) - 1;
+    uint32_t equal = select ? run.mark(piece, [&](uint32_t key) { return key == prefix; }) : 0u;
+    uint32_t all;
+    const uint32_t before = kv8_block_scan(sm, __popc(keep) + (static_cast<uint32_t>(__popc(equal)) << 16), all);
+    int e = eq_done + static_cast<int>(before >> 16);
+    const int first = done + min(eq_done, need);           // of this piece, among all kept
+    int to = done + static_cast<int>(before & 0xffff) + min(e, need) - first;
+    for (; equal != 0 && e < need; equal &= equal - 1, ++e) keep |= equal & (0u - equal);
+    for (; keep != 0; keep &= keep - 1) keys[to++] = base + run.from + __ffs(keep) - 1;
+    done += static_cast<int>(all & 0xffff);
+    eq_done += static_cast<int>(all >> 16);
+    const int last = done + min(eq_done, need);
+    __syncthreads();
+    for (int j0 = first + tid; j0 < last; j0 += 4 * KV8_SEL_THREADS) {
+      int at[4];
+      float v[4];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(0xffffffffu, all, o);
-      if (lane >= o) all += u;
-    }
-    const int before = __shfl_sync(0xffffffffu, all, (warp + 31) & 31);
-    const int block = __shfl_sync(0xffffffffu, all, 31);
-    const int mine0 = inc - mine + (warp > 0 ? before : 0);
-    int at = done + (mine0 & 0xffff), e = eq_done + (mine0 >> 16);   // keys above, and equal, before these
-    if (gt | eq) {
+      for (int u = 0; u < 4; ++u) at[u] = j0 + u * KV8_SEL_THREADS < last ? keys[j0 + u * KV8_SEL_THREADS - first] : -1;
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const bool is_eq = (eq >> u) & 1, is_gt = (gt >> u) & 1;
-        if (is_gt || (is_eq && e < need)) {
-          const int to = at + min(e, select ? need : 0);
-          kept[to] = i + u;
-          nw[to] = __ldg(w + i + u);
+      for (int u = 0; u < 4; ++u) v[u] = at[u] >= 0 ? __ldg(w + at[u]) : 0.f;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (at[u] >= 0) {
+          kept[j0 + u * KV8_SEL_THREADS] = at[u];
+          nw[j0 + u * KV8_SEL_THREADS] = v[u];
         }
-        at += is_gt;
-        e += is_eq;
-      }
     }
-    done += block & 0xffff;
-    eq_done += block >> 16;
-    __syncthreads();   // wsum is rewritten
+    __syncthreads();        // the sums and the keys are rewritten
   }
 }
 
@@ -425,9 +473,11 @@ WAMB_DEV void kv8_select_heavy(const Kv8Kept& k, const float* w, Kv8SelSmem& sm,
 // radix select (11, 11 and 10 bits, histograms in shared memory: whole-number
 // counts, so the order of the atomics does not matter), then one ordered pass
 // writes the kept positions. The weights are read once into shared memory, or
-// from L2 in each pass where a head has more than 36864; eight loads of a
-// thread are in flight. Bound by that one SM's instructions. A sequence whose
-// new pages overlap its old ones, or one another, is refused: it keeps nothing.
+// from L2 in each pass where a head has more than 36864. Bound by that one
+// SM's instructions (an instruction a key is 240 cycles at 31k keys): 64 heads
+// of 31k weights take 22 us of the 76 that an eviction of 8 x 32k tokens takes,
+// 24 heads of 3520 take 10 of 16. A sequence whose new pages overlap its old
+// ones, or one another, is refused: it keeps nothing.
 __global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8EvictParams p, const int list_at) {
   pdl_wait();
   extern __shared__ uint32_t keys[];
@@ -443,14 +493,28 @@ __global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8Ev
 
   const int new_pages = (k.total + p.c.page - 1) >> p.c.page_log2, old_pages = (k.len + p.c.page - 1) >> p.c.page_log2;
   const int* fresh = p.new_table + static_cast<long long>(b) * p.new_width;
+  // No page may be named twice by the new pages, nor be one of the old. A bit
+  // for each page id (modulo their number) tells almost always.
+  uint32_t* bits = reinterpret_cast<uint32_t*>(&sm.hist[0][0]);
+  constexpr uint32_t WORDS = KV8_SEL_COPIES * KV8_SEL_BINS;
+  const int* used = p.s.table + static_cast<long long>(b) * p.s.width;
+  kv8_clear_hist(sm);
   bool overlap = false;
-  for (int n = tid; n < new_pages; n += KV8_SEL_THREADS) {   // a page that is named twice would be written by two blocks
-    const int page = __ldg(fresh + n);
-    for (int m = 0; m < n; ++m) overlap |= __ldg(fresh + m) == page;
+  for (int n = tid; n < new_pages; n += KV8_SEL_THREADS) {
+    const uint32_t page = static_cast<uint32_t>(__ldg(fresh + n));
+    overlap |= atomicOr(bits + (page >> 5) % WORDS, 1u << (page & 31)) >> (page & 31) & 1;
   }
+  __syncthreads();
   for (int o = tid; o < old_pages; o += KV8_SEL_THREADS) {
-    const int page = __ldg(p.s.table + static_cast<long long>(b) * p.s.width + o);
-    for (int n = 0; n < new_pages; ++n) overlap |= __ldg(fresh + n) == page;
+    const uint32_t page = static_cast<uint32_t>(__ldg(used + o));
+    overlap |= bits[(page >> 5) % WORDS] >> (page & 31) & 1;
+  }
+  if (__syncthreads_or(overlap)) {       // look closely
+    overlap = false;
+    for (int n = tid; n < new_pages; n += KV8_SEL_THREADS)
+      for (int m = 0; m < n; ++m) overlap |= __ldg(fresh + m) == __ldg(fresh + n);
+    for (int o = tid; o < old_pages; o += KV8_SEL_THREADS)
+      for (int n = 0; n < new_pages; ++n) overlap |= __ldg(fresh + n) == __ldg(used + o);
   }
   if (__syncthreads_or(overlap)) {
     if (tid == 0) record_error(KV8_DEV_ERROR);
@@ -475,6 +539,7 @@ __global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8Ev
 // row, so that a warp's load spans four rows and a thread holds all its loads of
 // K and V in flight at once; half as many threads with twice the bytes each
 // measured 16 us less at 8 sequences x 8 heads of 32k tokens than 16 lanes of 8.
+// Bound by memory: 54 us there, 264 MB, 4.9 TB/s.
 template <int PAGE>
 __global__ void __launch_bounds__(PAGE == 128 ? 256 : 128, PAGE == 128 ? 3 : 6) kv8_gather_kernel(const Kv8EvictParams p) {
   pdl_wait();
