@@ -229,11 +229,62 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = j.e / p.qts, qt = j.e - b * p.qts;
   const int rows = min(QR, kv8_count(p.s, b) * p.group - qt * QR);
+  constexpr size_t PF = kv8_part_floats<QR>();
+  const int cnt = c - j.first + 1;      // two at least
+  auto slot = [&](int i) { return p.part + static_cast<size_t>(2 * (j.first + i) + (i == 0 ? 1 : 0)) * PF; };
+  // Row `row` of the tile from its sums.
+  auto finish = [&](int row, const float4& acc, float l, float m) {
+    const int rr = qt * QR + row, t = rr / p.group, hq = j.h * p.group + rr - t * p.group;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<uint2*>(p.out + b * p.o_sb + t * p.o_st + hq * p.o_sh + lane * 4) =
+        make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+    if (p.lse != nullptr && lane == 0)
+      p.lse[(static_cast<long long>(b) * p.s.tokens + t) * (p.c.heads * p.group) + hq] = kv8_row_lse(m, l);
+  };
+  if constexpr (RB > 1) {
+    // Two partials, as where there are more items than CTAs: four rows to a
+    // warp, all their loads in flight, by a quarter of the blocks.
+    if (cnt == 2) {
+      constexpr int EACH = 4;
+      const int r0 = (blockIdx.y * 8 + warp) * EACH;
+      float4 v[EACH][2];
+      float mk[EACH][2], lk[EACH][2];
+#pragma unroll
+      for (int q = 0; q < EACH; ++q)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          lk[q][i] = 0.f;
+          if (r0 + q < rows) {
+            v[q][i] = __ldcg(reinterpret_cast<const float4*>(slot(i) + (r0 + q) * 128) + lane);
+            mk[q][i] = __ldcg(slot(i) + QR * 128 + r0 + q);
+            lk[q][i] = __ldcg(slot(i) + QR * 129 + r0 + q);
+          }
+        }
+#pragma unroll
+      for (int q = 0; q < EACH; ++q) {
+        if (r0 + q >= rows) continue;
+        float m = -INFINITY, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          if (lk[q][i] != 0.f) m = fmaxf(m, mk[q][i]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (lk[q][i] == 0.f) continue;   // no key seen there
+          const float w = exp2f(mk[q][i] - m);
+          l += w * lk[q][i];
+          acc.x += w * v[q][i].x;
+          acc.y += w * v[q][i].y;
+          acc.z += w * v[q][i].z;
+          acc.w += w * v[q][i].w;
+        }
+        finish(r0 + q, acc, l, m);
+      }
+      return;
+    }
+  }
   const int row0 = blockIdx.y * RB;
   if (row0 >= rows) return;
-  constexpr size_t PF = kv8_part_floats<QR>();
-  const int cnt = c - j.first + 1;
-  auto slot = [&](int i) { return p.part + static_cast<size_t>(2 * (j.first + i) + (i == 0 ? 1 : 0)) * PF; };
   // Few partials: a warp per row. Many: all warps on each row.
   const int step = cnt > 8 || RB == 1 ? 8 : 1, from = step == 8 ? warp : 0;
   for (int q = step == 8 ? 0 : warp; q < RB; q += step == 8 ? 1 : 8) {
@@ -290,7 +341,6 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
   __syncthreads();
   const int parts = step == 8 ? 8 : 1;
   for (int q = warp; q < RB; q += 8) {
-    const int rr = qt * QR + row0 + q;
     if (row0 + q >= rows) continue;
     float4 acc = sum[q][0][lane];
     float l = den[q][0];
@@ -302,12 +352,7 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
       acc.w += v.w;
       l += den[q][i];
     }
-    const int t = rr / p.group, hq = j.h * p.group + rr - t * p.group;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    *reinterpret_cast<uint2*>(p.out + b * p.o_sb + t * p.o_st + hq * p.o_sh + lane * 4) =
-        make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
-    if (p.lse != nullptr && lane == 0)
-      p.lse[(static_cast<long long>(b) * p.s.tokens + t) * (p.c.heads * p.group) + hq] = kv8_row_lse(row_max[q], l);
+    finish(row0 + q, acc, l, row_max[q]);
   }
 }
 

@@ -185,13 +185,13 @@ inline size_t kv8_workspace(const wamb_kv8_attention_args* a, bool weights, cons
 // Splits the queries into `at`; returns the map of its rows and the factors.
 inline int kv8_split_launch(const Kv8AttnParams& p, const Kv8SplitQ& sq, uint8_t* at, bool weights, CUtensorMap* map,
                             float** factor, float** neg_lse2, cudaStream_t s) {
-  WAMB_REQUIRE(sq.total <= INT32_MAX, WAMB_ERR_SHAPE, "kv8: %lld query rows", sq.total);
+  WAMB_REQUIRE(sq.total <= INT32_MAX - 64, WAMB_ERR_SHAPE, "kv8: %lld query rows", sq.total);
   *factor = reinterpret_cast<float*>(at + sq.total * 256);
   *neg_lse2 = weights ? *factor + sq.total : nullptr;
   int rc = make_tmap_2d(map, at, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, sq.total, 256, 256, 128, 128);
   if (rc) return rc;
-  return launch_kernel(kv8_split_q_kernel, dim3(static_cast<unsigned>((sq.total + 31) / 32)), dim3(256), 0, s, p,
-                       sq.rows_pad, sq.total, at, *factor, *neg_lse2);
+  return launch_kernel(kv8_split_q_kernel, dim3(static_cast<unsigned>((sq.total + 63) / 64)), dim3(256), 0, s, p,
+                       sq.rows_pad, static_cast<int>(sq.total), at, *factor, *neg_lse2);
 }
 
 inline int kv8_attention_impl(const wamb_kv8_attention_args* a, bool weights, cudaStream_t s) {
