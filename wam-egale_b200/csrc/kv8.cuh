@@ -102,17 +102,21 @@ WAMB_DEV void e4m3x8_to_float(uint2 w, float (&f)[8]) {
   }
 }
 
-// Largest of a value over a 256-thread block (fmaxf: NaN loses).
-WAMB_DEV float block_max_256(float v, float* red) {
+// Largest of a value over the block (fmaxf: NaN loses).
+template <int THREADS>
+WAMB_DEV float kv8_block_max(float v, float* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
   __syncthreads();
   v = red[0];
 #pragma unroll
-  for (int i = 1; i < 8; ++i) v = fmaxf(v, red[i]);
+  for (int i = 1; i < THREADS / 32; ++i) v = fmaxf(v, red[i]);
   return v;
 }
+
+// Threads of a block that holds a page's rows of one head in registers.
+__host__ __device__ constexpr int kv8_page_threads(int page) { return page < 128 ? 128 : 256; }
 
 // ------------------------------------------------------------------- write
 struct Kv8WriteParams {
@@ -124,13 +128,16 @@ struct Kv8WriteParams {
 
 // One block per (touched page, head, sequence, K or V): the block's new rows
 // stay in registers between the amax and the rounding, so each is read once.
-// 16 threads hold a row (8 values each), 16 rows per pass, PAGE / 16 passes.
-// Bound by memory for chunks, by the launch for single tokens.
+// Eight threads hold a row, 16 values each.
+// Bound by memory for chunks: 8 x 880 rows of 24 heads (130 MB) take 24.7 us,
+// 5.3 TB/s; 27.5 with twice the threads and half the loads of each in flight,
+// 28.4 with 8 values a thread. By the launch for single tokens (2.2 us).
 template <bool F32, int PAGE>
-__global__ void __launch_bounds__(256) kv8_write_kernel(const Kv8WriteParams p) {
+__global__ void __launch_bounds__(kv8_page_threads(PAGE)) kv8_write_kernel(const Kv8WriteParams p) {
   pdl_wait();
-  constexpr int PASSES = PAGE / 16;
-  __shared__ float red[8];
+  constexpr int THREADS = kv8_page_threads(PAGE), ROWS = THREADS / 8, PASSES = PAGE / ROWS;
+  constexpr int WORDS = F32 ? 4 : 2;      // 16-byte pieces of 16 values
+  __shared__ float red[THREADS / 32];
   const int h = blockIdx.y, b = blockIdx.z >> 1, which = blockIdx.z & 1;
   const int start = kv8_len(p.s, p.c, b);
   int cnt = kv8_count(p.s, b);
@@ -146,31 +153,26 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(const Kv8WriteParams p) 
   const int pid = kv8_page(p.s.table, p.s.width, p.c, b, pi);
   if (pid < 0) return;
   const int held = lo - pi * PAGE, n = hi - lo;
-  const int c8 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
-  const long long base = b * p.sb[which] + h * p.sh[which] + (lo - start) * p.st[which] + c8 * 8;
+  const int c16 = threadIdx.x & 7, r0 = threadIdx.x >> 3;
+  const long long base = b * p.sb[which] + h * p.sh[which] + (lo - start) * p.st[which] + c16 * 16;
 
-  uint4 raw[F32 ? 2 * PASSES : PASSES];
-  float amax = 0.f;
+  uint4 raw[PASSES][WORDS];
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
-    const int r = r0 + 16 * i;
-    const long long off = base + r * p.st[which];
-    if constexpr (F32) {
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(p.x[which]) + off);
-      raw[2 * i] = r < n ? __ldg(src) : make_uint4(0, 0, 0, 0);
-      raw[2 * i + 1] = r < n ? __ldg(src + 1) : make_uint4(0, 0, 0, 0);
-    } else {
-      raw[i] = r < n ? __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.x[which]) + off))
-                     : make_uint4(0, 0, 0, 0);
-    }
+    const int r = r0 + ROWS * i;
+    const uint4* src = reinterpret_cast<const uint4*>(static_cast<const char*>(p.x[which]) +
+                                                      (base + r * p.st[which]) * (F32 ? 4 : 2));
+#pragma unroll
+    for (int k = 0; k < WORDS; ++k) raw[i][k] = r < n ? __ldg(src + k) : make_uint4(0, 0, 0, 0);
   }
-  auto value = [&](int i, float (&f)[8]) {
+  // Values 8 half .. 8 half + 7 of row i.
+  auto value = [&](int i, int half, float (&f)[8]) {
     if constexpr (F32) {
-      const uint4 a = raw[2 * i], d = raw[2 * i + 1];
+      const uint4 a = raw[i][2 * half], d = raw[i][2 * half + 1];
       f[0] = __uint_as_float(a.x); f[1] = __uint_as_float(a.y); f[2] = __uint_as_float(a.z); f[3] = __uint_as_float(a.w);
       f[4] = __uint_as_float(d.x); f[5] = __uint_as_float(d.y); f[6] = __uint_as_float(d.z); f[7] = __uint_as_float(d.w);
     } else {
-      const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+      const uint32_t w[4] = {raw[i][half].x, raw[i][half].y, raw[i][half].z, raw[i][half].w};
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float2 v = unpack_bf16(w[k]);
@@ -179,39 +181,53 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(const Kv8WriteParams p) 
       }
     }
   };
+  float amax = 0.f;
 #pragma unroll
-  for (int i = 0; i < PASSES; ++i) {
-    float f[8];
-    value(i, f);
+  for (int i = 0; i < PASSES; ++i)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(f[k]));
-  }
-  amax = block_max_256(amax, red);
+    for (int half = 0; half < 2; ++half) {
+      float f[8];
+      value(i, half, f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) amax = fmaxf(amax, fabsf(f[k]));
+    }
+  amax = kv8_block_max<THREADS>(amax, red);
   const long long blk = static_cast<long long>(pid) * p.c.heads + h;
   float* scale = (which ? p.c.v_scale : p.c.k_scale) + blk;
-  uint8_t* codes = (which ? p.c.v8 : p.c.k8) + blk * (PAGE * 128) + c8 * 8;
+  uint8_t* codes = (which ? p.c.v8 : p.c.k8) + blk * (PAGE * 128) + c16 * 16;
   const float s_old = held > 0 ? *scale : 0.f;
   const float s = fmaxf(pow2f_exact(kv8_scale_exp(amax)), s_old);
   const float inv = 1.f / s;
 #pragma unroll
   for (int i = 0; i < PASSES; ++i) {
-    const int r = r0 + 16 * i;
+    const int r = r0 + ROWS * i;
     if (r >= n) continue;
-    float f[8];
-    value(i, f);
+    uint2 part[2];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) f[k] *= inv;
-    *reinterpret_cast<uint2*>(codes + (held + r) * 128) = pack_e4m3x8(f);
+    for (int half = 0; half < 2; ++half) {
+      float f[8];
+      value(i, half, f);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) f[k] *= inv;
+      part[half] = pack_e4m3x8(f);
+    }
+    *reinterpret_cast<uint4*>(codes + (held + r) * 128) = make_uint4(part[0].x, part[0].y, part[1].x, part[1].y);
   }
   if (s > s_old) {   // earlier tokens of the block move to the larger scale
     const float ratio = s_old * inv;
-    for (int r = r0; r < held; r += 16) {
-      uint2* at = reinterpret_cast<uint2*>(codes + r * 128);
-      float f[8];
-      e4m3x8_to_float(*at, f);
+    for (int r = r0; r < held; r += ROWS) {
+      uint4* at = reinterpret_cast<uint4*>(codes + r * 128);
+      const uint4 was = *at;
+      uint2 part[2];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) f[k] *= ratio;
-      *at = pack_e4m3x8(f);
+      for (int half = 0; half < 2; ++half) {
+        float f[8];
+        e4m3x8_to_float(half ? make_uint2(was.z, was.w) : make_uint2(was.x, was.y), f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] *= ratio;
+        part[half] = pack_e4m3x8(f);
+      }
+      *at = make_uint4(part[0].x, part[0].y, part[1].x, part[1].y);
     }
     __syncthreads();   // every thread has read the old scale
     if (threadIdx.x == 0) *scale = s;
@@ -541,10 +557,10 @@ __global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8Ev
 // measured 16 us less at 8 sequences x 8 heads of 32k tokens than 16 lanes of 8.
 // Bound by memory: 54 us there, 264 MB, 4.9 TB/s.
 template <int PAGE>
-__global__ void __launch_bounds__(PAGE == 128 ? 256 : 128, PAGE == 128 ? 3 : 6) kv8_gather_kernel(const Kv8EvictParams p) {
+__global__ void __launch_bounds__(kv8_page_threads(PAGE), PAGE == 128 ? 3 : 6) kv8_gather_kernel(const Kv8EvictParams p) {
   pdl_wait();
   // Eight lanes hold a row, 16 codes each.
-  constexpr int THREADS = PAGE == 128 ? 256 : 128, ROWS = THREADS / 8, PASSES = PAGE / ROWS;
+  constexpr int THREADS = kv8_page_threads(PAGE), ROWS = THREADS / 8, PASSES = PAGE / ROWS;
   __shared__ float red[2][THREADS / 32];
   const int h = blockIdx.y, b = blockIdx.z;
   const int c16 = threadIdx.x & 7, r0 = threadIdx.x >> 3;

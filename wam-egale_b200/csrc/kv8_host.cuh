@@ -46,10 +46,10 @@ inline int kv8_seqs_check(const wamb_kv8_seqs* s, int page, Kv8Seqs* out) {
 template <bool F32>
 inline int kv8_write_launch(const Kv8WriteParams& p, dim3 grid, cudaStream_t s) {
   switch (p.c.page) {
-    case 16: return launch_kernel(kv8_write_kernel<F32, 16>, grid, dim3(256), 0, s, p);
-    case 32: return launch_kernel(kv8_write_kernel<F32, 32>, grid, dim3(256), 0, s, p);
-    case 64: return launch_kernel(kv8_write_kernel<F32, 64>, grid, dim3(256), 0, s, p);
-    default: return launch_kernel(kv8_write_kernel<F32, 128>, grid, dim3(256), 0, s, p);
+    case 16: return launch_kernel(kv8_write_kernel<F32, 16>, grid, dim3(kv8_page_threads(16)), 0, s, p);
+    case 32: return launch_kernel(kv8_write_kernel<F32, 32>, grid, dim3(kv8_page_threads(32)), 0, s, p);
+    case 64: return launch_kernel(kv8_write_kernel<F32, 64>, grid, dim3(kv8_page_threads(64)), 0, s, p);
+    default: return launch_kernel(kv8_write_kernel<F32, 128>, grid, dim3(kv8_page_threads(128)), 0, s, p);
   }
 }
 
@@ -137,10 +137,10 @@ inline int kv8_evict_impl(const wamb_kv8_evict_args* a, cudaStream_t s) {
   if (rc) return rc;
   const dim3 grid(p.new_width, p.c.heads, p.s.batch);
   switch (p.c.page) {
-    case 16: return launch_kernel(kv8_gather_kernel<16>, grid, dim3(128), 0, s, p);
-    case 32: return launch_kernel(kv8_gather_kernel<32>, grid, dim3(128), 0, s, p);
-    case 64: return launch_kernel(kv8_gather_kernel<64>, grid, dim3(128), 0, s, p);
-    default: return launch_kernel(kv8_gather_kernel<128>, grid, dim3(256), 0, s, p);
+    case 16: return launch_kernel(kv8_gather_kernel<16>, grid, dim3(kv8_page_threads(16)), 0, s, p);
+    case 32: return launch_kernel(kv8_gather_kernel<32>, grid, dim3(kv8_page_threads(32)), 0, s, p);
+    case 64: return launch_kernel(kv8_gather_kernel<64>, grid, dim3(kv8_page_threads(64)), 0, s, p);
+    default: return launch_kernel(kv8_gather_kernel<128>, grid, dim3(kv8_page_threads(128)), 0, s, p);
   }
 }
 
