@@ -11,8 +11,8 @@
 // TMA into its own ring, with no barrier between warps until an item ends.
 // The codes become f16 in registers (E4M3 is a subset of f16, nothing is
 // rounded) and meet the queries in m16n8k16 products with fp32 sums. (The
-// E4M3 m16n8k32 form is no shortcut here: it took 1030 instructions a step
-// where this one takes about 450.) Queries go to f16 scaled per row by a power
+// E4M3 m16n8k32 form is no shortcut here: with it a step took about twice the
+// instructions.) Queries go to f16 scaled per row by a power
 // of two that puts the largest magnitude into [2^13, 2^14), which keeps their
 // eight bits over 28 binades.
 //
@@ -21,6 +21,13 @@
 // running maximum of y (moved only when it grows by more than 2^8), and
 // l_i = sum_j P_ij / vs_j. P goes to the product as f16 with an offset of 2^6:
 // 11 bits down to 2^-20 of the row's maximum and whole steps of 2^-30 below.
+//
+// Bound by instruction issue: one token of 8 sequences of 18 to 32 thousand
+// keys (8 heads, 4 query heads each, 420 MB) takes 82 us, 5.1 TB/s, with 35 M
+// warp instructions, half of them the conversions of codes and the products;
+// its attention weights (K alone, 227 MB) take 49 us, 4.7 TB/s. The smallest calls
+// (2 sequences of 500 keys, 12 heads) take 11 us, nearly all of it the latency of two
+// launches and of table -> scale -> codes.
 #pragma once
 #include "attention.cuh"
 #include "kv8.cuh"
@@ -373,8 +380,7 @@ struct FewUnit {
 
 // Three CTAs fit an SM (four of the weights'): twelve warps, each with 12 KB (10)
 // of its keys on their way or in use. (Two CTAs with 16 KB a warp took 104 us
-// where this takes 84: one token of 8 sequences of 18 to 32 thousand keys, 8
-// heads, 4 query heads each.)
+// where this took 89: one token of 8 sequences of 18 to 32 thousand keys.)
 template <bool WEIGHTS>
 struct FewSmem {
   static constexpr int STAGES = WEIGHTS ? 5 : 3;                              // of 16 keys

@@ -28,6 +28,16 @@
 // beside the other's products. In both cases the work is a row of steps, step
 // s on slot s & 1: S(s + 2) is issued behind PV(s).
 // TMEM columns: S/P of A [0,128), of B [128,256), O_A [256,384), O_B [384,512).
+//
+// Bound by the softmax's issue slots and the chain S -> softmax -> P -> PV of a
+// slot: a key tile of 256 rows takes about 5000 cycles where its MMAs take
+// 2048. 8 x 880 rows over up to 4400 keys of 24 heads (297 GFLOP): 434 us, 0.68
+// PFLOP/s, 19 of them the split of the queries; 32 rows of 4 sequences (75 MB
+// of cache) 46 us. Slower forms of the same chain, at that size and before the
+// last 30 us were taken elsewhere (this one: 468): P through shared memory 549
+// to 590 (two or one buffers), PV in two halves 556, scores in 64-key halves
+// 753, V's codes read by the converting warps from global memory 505, an eighth
+// of the exponentials as a polynomial 510, no register split 758.
 #pragma once
 #include "attention.cuh"
 #include "glue.cuh"
@@ -759,9 +769,12 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
 // tile that is loaded serves both.
 // Bound by the exponentials: 128 x 128 of them take the SM's MUFU 1024
 // cycles, the products of the two query pieces 512.
+// 880 rows over 4400 keys of 24 heads (23.8 GFLOP): 50 us, 7 of them the split
+// of the queries; 8 such sequences of up to 4400 keys 271 us, 0.55 PFLOP/s. 17
+// rows over 16 k keys of 8 x 8 heads: 47 us (63 with the columns behind the rows).
 // 320 threads: warps 0..7 exponentials, warp 8 loads, warp 9 issues the MMAs.
 constexpr int KWT_THREADS = 320, KWT_QS = 4, KWT_FS = 8, KWT_SCS = 16, KWT_QR = 1 << 30;
-constexpr int KWT_POLY = 2;      // pairs of every eight whose 2^x runs on the FMA pipe
+constexpr int KWT_POLY = 2;      // pairs of every eight whose 2^x runs on the FMA pipe: 0, 1, 2, 3, 4 took 58, 52, 50, 50, 52 us (below)
 
 struct KwtSmem {
   static constexpr uint32_t K_OFF = 0;                                     // [2 pairs] 2 tiles of codes
@@ -777,7 +790,7 @@ struct KwtSmem {
 
 // One or two neighbouring key tiles, and their query tiles [q0, q1).
 struct KwtPair {
-  int b, h, k0, len, cnt, q0, q1, shift;   // row r sees key j when r >= group * (j - shift)
+  int b, h, k0, len, cnt, rows, q0, q1, shift;   // row r sees key j when r >= group * (j - shift)
   WAMB_DEV KwtPair(const Kv8AttnParams& p, const Kv8Share& sh, const KtcWalk<KWT_QR>& w) {
     b = w.it.e;
     h = w.it.h;
@@ -786,7 +799,8 @@ struct KwtPair {
     len = kv8_len(p.s, p.c, b);
     const int tokens = kv8_count(p.s, b);
     shift = len - tokens;
-    q1 = (tokens * p.group + 127) / 128;
+    rows = tokens * p.group;
+    q1 = (rows + 127) / 128;
     q0 = p.causal && k0 > shift ? static_cast<int>(min(q1 - 1ll, static_cast<long long>(k0 - shift) * p.group / 128)) : 0;
   }
   WAMB_DEV void next(const Kv8AttnParams& p, const Kv8Share& sh, KtcWalk<KWT_QR>& w) const {
@@ -1010,18 +1024,20 @@ __global__ void __launch_bounds__(KWT_THREADS, 1)
           tmem_ld32(ts, sA);
           tmem_wait_ld();
           tmem_ld32(ts + 32, sB);
+          // 32 columns that lie behind the rows have nothing to add.
+          const int live = n.rows - qt * 128;
           add(sA, 0);
           tmem_wait_ld();
           tmem_ld32(ts + 64, sA);
-          add(sB, 1);
+          if (live > 32) add(sB, 1);
           tmem_wait_ld();
           tmem_ld32(ts + 96, sB);
-          add(sA, 2);
+          if (live > 64) add(sA, 2);
           tmem_wait_ld();
           tc_fence_before();   // the scores are in registers: the buffer is free
           __syncwarp();
           if (lane == 0) mbar_arrive(s_free + 8 * sb);
-          add(sB, 3);
+          if (live > 96) add(sB, 3);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(f_free + 8 * fs);
