@@ -45,8 +45,9 @@ WAMB_DEV void record_error(int code) { atomicCAS(&g_error, 0, code); }
 WAMB_DEV void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Early trigger: the dependent grid may launch once every CTA of this grid
 // has issued it (so it never takes an SM from a CTA of this grid that has
-// not started). Used only where a GEMM that requests weights before its
-// pdl_wait follows; elsewhere the implicit trigger at exit measured faster.
+// not started). Used only where the next grid has work before its pdl_wait (a
+// GEMM that requests weights, the E4M3 cache's tensor-core kernels that find
+// their share); elsewhere the implicit trigger at exit measured faster.
 WAMB_DEV void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 // ----------------------------------------------------------------- mbarrier

@@ -33,7 +33,7 @@
 // slot: a key tile of 256 rows takes about 5000 cycles where its MMAs take
 // 2048. 8 x 880 rows over up to 4400 keys of 24 heads (297 GFLOP): 434 us, 0.68
 // PFLOP/s, 19 of them the split of the queries; 32 rows of 4 sequences (75 MB
-// of cache) 46 us. Slower forms of the same chain, at that size and before the
+// of cache) 44 us. Slower forms of the same chain, at that size and before the
 // last 30 us were taken elsewhere (this one: 468): P through shared memory 549
 // to 590 (two or one buffers), PV in two halves 556, scores in 64-key halves
 // 753, V's codes read by the converting warps from global memory 505, an eighth
@@ -193,6 +193,7 @@ WAMB_DEV float query_scale(float amax, int& n) {
 __global__ void __launch_bounds__(256) kv8_split_q_kernel(const Kv8AttnParams p, const int rows_pad, const int total,
                                                           uint8_t* q8, float* rf, float* neg_lse2) {
   pdl_wait();
+  pdl_trigger();   // the kernel behind it finds its work meanwhile (one chunk 92 -> 90 us)
   constexpr int AT_ONCE = 2;
   const int c = threadIdx.x & 7, first = blockIdx.x * (32 * AT_ONCE) + (threadIdx.x >> 3);
   uint4 w[AT_ONCE][2];
@@ -296,12 +297,16 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // warp: uniform
 
-  pdl_wait();
+  // The split of the queries let this kernel start when everything before it
+  // was complete: only what it writes is waited for.
   Kv8Share sh;
   KtcWalk<KTC_QR> walk;
   const bool work = kv8_share<KTC_QR, KTC_TK, KTC_THREADS>(p, blockIdx.x, sched, sh, walk.it);
   if (threadIdx.x == 0) kv8_leave_join(p, sh, work, walk.it);
-  if (!work) return;
+  if (!work) {
+    pdl_wait();    // the kernel is not complete before the split is
+    return;
+  }
   walk.u = sh.u0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -327,6 +332,7 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
     tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
   }
+  pdl_wait();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -826,11 +832,14 @@ __global__ void __launch_bounds__(KWT_THREADS, 1)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;   // warp: uniform
 
-  pdl_wait();
+  // As in kv8_tc_kernel, only the split of the queries is waited for.
   kv8_carry_base<KWT_THREADS>(p);
   Kv8Share sh;
   KtcWalk<KWT_QR> walk;
-  if (!kv8_share<KWT_QR, KTC_TK, KWT_THREADS>(p, blockIdx.x, sched, sh, walk.it)) return;
+  if (!kv8_share<KWT_QR, KTC_TK, KWT_THREADS>(p, blockIdx.x, sched, sh, walk.it)) {
+    pdl_wait();
+    return;
+  }
   walk.u = sh.u0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) { mbar_init(k_full + 8 * i, 1); mbar_init(k_empty + 8 * i, 1); }
@@ -845,6 +854,7 @@ __global__ void __launch_bounds__(KWT_THREADS, 1)
     tmem_alloc(smem_u32(tmem_slot), 512);
     tmem_relinquish();
   }
+  pdl_wait();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
