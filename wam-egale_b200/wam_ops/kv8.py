@@ -152,7 +152,7 @@ class Kv8Cache:
         of `out` and `lse` are left as they were."""
         a = self._attention_args(q, table, lens, counts, causal, scale)
         if out is None:
-            out = q.new_empty(q.shape)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != q.shape:
             raise ValueError("out must be shaped like q")
         elif any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
@@ -160,7 +160,7 @@ class Kv8Cache:
         a.out_stride[:] = self._rows("out", out)
         a.out = out.data_ptr()
         if lse is None and return_lse:
-            lse = self.k_scale.new_empty(q.shape[:3])
+            lse = self.k_scale.new_empty((a.seqs.batch, a.seqs.tokens, a.q_heads))
         if lse is not None:
             a.lse = self._lse(lse, q)
         self._call(self._lib.wamb_kv8_attention, a, self._lib.wamb_kv8_attention_workspace_bytes, ("attention", q.shape))
