@@ -64,25 +64,26 @@ class Kv8Cache:
         return t.data_ptr()
 
     def _seqs(self, seqs, batch, tokens, table, lens, counts):
-        if table.dim() != 2 or table.shape[0] != batch:
+        shape = table.shape
+        if len(shape) != 2 or shape[0] != batch:
             raise ValueError(f"table must be [batch {batch}, width]")
-        seqs.batch, seqs.tokens, seqs.table_width = batch, tokens, table.shape[1]
-        seqs.table = self._ints("table", table, table.shape)
+        seqs.batch, seqs.tokens, seqs.table_width = batch, tokens, shape[1]
+        seqs.table = self._ints("table", table, shape)
         seqs.lens = self._ints("lens", lens, (batch,))
         if counts is not None:
             seqs.counts = self._ints("counts", counts, (batch,))
 
     def _rows(self, name, t, heads=None, dtypes=(torch.bfloat16,)):
         """Strides of [batch, tokens, heads, 128] with rows of 128 contiguous values."""
-        if t.dim() != 4 or t.shape[3] != HEAD_DIM or t.dtype not in dtypes or t.device != self.device:
+        b, s = t.shape, t.stride()
+        if len(b) != 4 or b[3] != HEAD_DIM or t.dtype not in dtypes or t.device != self.device:
             raise ValueError(f"{name} must be [batch, tokens, heads, 128] {' or '.join(map(str, dtypes))} on {self.device}")
-        if heads is not None and t.shape[2] != heads:
-            raise ValueError(f"{name} has {t.shape[2]} heads, the cache {heads}")
+        if heads is not None and b[2] != heads:
+            raise ValueError(f"{name} has {b[2]} heads, the cache {heads}")
         if t.requires_grad and torch.is_grad_enabled():
             raise RuntimeError("Kv8Cache is inference-only; use no_grad/inference_mode")
-        if t.stride(3) != 1:
+        if s[3] != 1:
             raise ValueError(f"{name} must have unit stride along the head dim")
-        b, s = t.shape, t.stride()
         # The stride of a single entry may be anything; the C ABI is told 0.
         return s[0] if b[0] > 1 else 0, s[1] if b[1] > 1 else 0, s[2] if b[2] > 1 else 0
 
