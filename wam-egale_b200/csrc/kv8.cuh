@@ -491,8 +491,8 @@ WAMB_DEV void kv8_select_heavy(const Kv8Kept& k, const float* w, Kv8SelSmem& sm,
 // writes the kept positions. The weights are read once into shared memory, or
 // from L2 in each pass where a head has more than 36864. Bound by that one
 // SM's instructions (an instruction a key is 240 cycles at 31k keys): 64 heads
-// of 31k weights take 22 us of the 76 that an eviction of 8 x 32k tokens takes,
-// 24 heads of 3520 take 10 of 16. A sequence whose new pages overlap its old
+// of 31k weights take 22 us of the 72 that an eviction of 8 x 32k tokens takes,
+// 24 heads of 3520 take 10 of 17. A sequence whose new pages overlap its old
 // ones, or one another, is refused: it keeps nothing.
 __global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8EvictParams p, const int list_at) {
   pdl_wait();
@@ -555,9 +555,10 @@ __global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8Ev
 // row, so that a warp's load spans four rows and a thread holds all its loads of
 // K and V in flight at once; half as many threads with twice the bytes each
 // measured 16 us less at 8 sequences x 8 heads of 32k tokens than 16 lanes of 8.
-// Bound by memory: 54 us there, 264 MB, 4.9 TB/s.
+// Bound by memory: 50 us there, 264 MB, 5.3 TB/s, with nine blocks an SM (six
+// took 54, ten and twelve 51 to 55; K and V in blocks of their own 53 to 57).
 template <int PAGE>
-__global__ void __launch_bounds__(kv8_page_threads(PAGE), PAGE == 128 ? 3 : 6) kv8_gather_kernel(const Kv8EvictParams p) {
+__global__ void __launch_bounds__(kv8_page_threads(PAGE), PAGE == 128 ? 5 : 9) kv8_gather_kernel(const Kv8EvictParams p) {
   pdl_wait();
   // Eight lanes hold a row, 16 codes each.
   constexpr int THREADS = kv8_page_threads(PAGE), ROWS = THREADS / 8, PASSES = PAGE / ROWS;
