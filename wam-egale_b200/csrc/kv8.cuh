@@ -558,7 +558,7 @@ __global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8Ev
 // Bound by memory: 50 us there, 264 MB, 5.3 TB/s, with nine blocks an SM (six
 // took 54, ten and twelve 51 to 55; K and V in blocks of their own 53 to 57).
 template <int PAGE>
-__global__ void __launch_bounds__(kv8_page_threads(PAGE), PAGE == 128 ? 5 : 9) kv8_gather_kernel(const Kv8EvictParams p) {
+__global__ void __launch_bounds__(kv8_page_threads(PAGE), PAGE == 128 ? 3 : 9) kv8_gather_kernel(const Kv8EvictParams p) {
   pdl_wait();
   // Eight lanes hold a row, 16 codes each.
   constexpr int THREADS = kv8_page_threads(PAGE), ROWS = THREADS / 8, PASSES = PAGE / ROWS;
