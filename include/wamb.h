@@ -531,9 +531,13 @@ WAMB_API int wamb_kv8_write(const wamb_kv8_write_args* args, void* stream);
  * A row that sees nothing gives zeros and lse -inf; rows past counts[b] are
  * left as they were. What lies past lens[b] in a page counts for nothing,
  * but a NaN that was written as V reaches every row of the call that is
- * computed beside its key. workspace: wamb_kv8_attention_workspace_bytes()
- * bytes of scratch (256-byte aligned, any contents), not shared with a call that may run at the
- * same time. Results do not depend on timing. */
+ * computed beside its key. Scores are summed in fp32. With more than 16 rows
+ * a sequence and cached head, an element of q below 2^-14 of its row's largest
+ * magnitude is taken to within 2^-21 of that magnitude; all others, and with
+ * up to 16 rows all down to 2^-28, count with their full eight bits. workspace:
+ * wamb_kv8_attention_workspace_bytes() bytes of scratch (256-byte aligned, any
+ * contents), not shared with a call that may run at the same time. Results do
+ * not depend on timing. */
 typedef struct wamb_kv8_attention_args {
   wamb_kv8_cache cache;
   wamb_kv8_seqs seqs;

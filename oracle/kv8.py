@@ -86,13 +86,13 @@ def _rows(q, k, n, t, causal, scale):
 
     The products are summed in fp32 (128 terms: at most 130 roundings of the
     sum of magnitudes, a tensor core may truncate: 2^-23 each); a query may be
-    held in two E4M3 pieces, off by at most 2^-10 when its row's largest
-    magnitude is at least 224; the score meets its factors, the log-sum-exp
+    held in an E4M3 and an E5M2 piece, off by at most 2^-14 when its row's
+    largest magnitude is at least 224; the score meets its factors, the log-sum-exp
     or the maximum in a few more fp32 roundings of numbers of its own size.
     """
     s = q @ k.T * scale
     mag = q.abs() @ k.abs().T * scale
-    piece = q.abs().amax(1, keepdim=True) / 224.0 * 2.0 ** -10 * (k.abs().sum(1)[None] * scale)
+    piece = q.abs().amax(1, keepdim=True) / 224.0 * 2.0 ** -14 * (k.abs().sum(1)[None] * scale)
     err = mag * (130 * 2.0 ** -23) + piece + s.abs() * 2.0 ** -21
     if causal:
         hidden = torch.arange(n, device=q.device)[None] > n - t + torch.arange(t, device=q.device)[:, None]

@@ -4,12 +4,16 @@
 // units of 128 keys.
 //
 // S = Q K^T reads K's codes as they lie in the cache (kind::f8f6f4, no
-// conversion): a bf16 query has eight significant bits, which are two E4M3
-// values of four, q 2^-n = hi + lo, so S = (hi K^T + lo K^T) 2^n costs what
-// one bf16 product does. n puts the row's largest magnitude in (224, 448]; a
-// value smaller than 2^-10 of it keeps an absolute error of at most 2^-10
-// (2^-18 of the largest). The E4M3 product sums in full fp32 here (measured:
-// 9e-9 relative error against 64 bits at K 128, bf16's is 1.2e-7).
+// conversion): q 2^-n = hi + lo, hi the nearest E4M3 value and lo the nearest
+// E5M2 value of what it leaves, so S = (hi K^T + lo K^T) 2^n costs what one
+// bf16 product does. n puts the row's largest magnitude in (224, 448]. From
+// 2^-6 on (2^-14 of the largest) hi + lo has all eight bits of a bf16 query:
+// hi has four, and what it leaves is at most 8 units in the last of the eight,
+// which E5M2's three bits hold. Below, hi leaves at most 2^-10 and lo is off by
+// half its step, 2^-14 (2^-21 of the row's largest). With E4M3 for lo, whose
+// steps end at 2^-9, the error was 2^-10 already from 2^-2 down. The products
+// are summed in full fp32 here (measured: 9e-9 relative error against 64 bits
+// at K 128, bf16's is 1.2e-7).
 // O += P V needs more range than two E4M3 pieces of P hold (a long flat tail
 // beside a sharp maximum), so P is f16 as in kv8_few.cuh and V's codes become
 // f16 in shared memory, once for 256 rows, by two warps of their own.
@@ -75,9 +79,10 @@ __host__ __device__ constexpr uint32_t idesc_f16_mn(int M, int N) {
 constexpr uint32_t KTC_DESC_HI = (1024u >> 4) | (1u << 14) | (2u << 29);
 WAMB_DEV uint32_t ktc_desc_lo(uint32_t addr, uint32_t lbo) { return (addr >> 4) | ((lbo >> 4) << 16); }
 
-// S [128 rows][128 keys] = (hi + lo) K^T: 4 x 32 dims of each piece.
+// S [128 rows][128 keys] = (hi + lo) K^T: 4 x 32 dims of each piece. The
+// instruction descriptor's type fields: A in bits 7-9, B in 10-12, 1 is E5M2.
 WAMB_DEV void ktc_issue_s(uint32_t d, uint32_t q, uint32_t k) {
-  constexpr uint32_t IDESC = idesc_e4m3(128, 128);
+  constexpr uint32_t IDESC = idesc_e4m3(128, 128), IDESC_LO = IDESC | (1u << 7);
   const uint32_t qd = ktc_desc_lo(q, 16), kd = ktc_desc_lo(k, 16);
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -85,13 +90,13 @@ WAMB_DEV void ktc_issue_s(uint32_t d, uint32_t q, uint32_t k) {
         "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
         "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %4, p;\n\t}" ::"r"(d),
-        "r"(qd + (i >> 2) * (KTC_TILE8 >> 4) + (i & 3) * 2), "r"(kd + (i & 3) * 2), "n"(KTC_DESC_HI), "n"(IDESC),
+        "r"(qd + (i >> 2) * (KTC_TILE8 >> 4) + (i & 3) * 2), "r"(kd + (i & 3) * 2), "n"(KTC_DESC_HI), "r"(i < 4 ? IDESC : IDESC_LO),
         "r"(i > 0 ? 1u : 0u)
         : "memory");
 }
 // S^T [128 keys][128 rows] = K (hi + lo)^T.
 WAMB_DEV void ktc_issue_st(uint32_t d, uint32_t k, uint32_t q) {
-  constexpr uint32_t IDESC = idesc_e4m3(128, 128);
+  constexpr uint32_t IDESC = idesc_e4m3(128, 128), IDESC_LO = IDESC | (1u << 10);
   const uint32_t qd = ktc_desc_lo(q, 16), kd = ktc_desc_lo(k, 16);
 #pragma unroll
   for (int i = 0; i < 8; ++i)
@@ -99,7 +104,7 @@ WAMB_DEV void ktc_issue_st(uint32_t d, uint32_t k, uint32_t q) {
         "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
         "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\tsetp.ne.b32 p, %5, 0;\n\t"
         "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %4, p;\n\t}" ::"r"(d),
-        "r"(kd + (i & 3) * 2), "r"(qd + (i >> 2) * (KTC_TILE8 >> 4) + (i & 3) * 2), "n"(KTC_DESC_HI), "n"(IDESC),
+        "r"(kd + (i & 3) * 2), "r"(qd + (i >> 2) * (KTC_TILE8 >> 4) + (i & 3) * 2), "n"(KTC_DESC_HI), "r"(i < 4 ? IDESC : IDESC_LO),
         "r"(i > 0 ? 1u : 0u)
         : "memory");
 }
@@ -162,14 +167,13 @@ WAMB_DEV uint64_t ex2_poly5(uint64_t x2) {
                      __int_as_float((__float_as_int(tv.y) << 23) + 0x3f800000)));
 }
 
-// Four values into their E4M3 code word `h` and the word of what it leaves.
-// A bf16 value has eight significant bits: two codes of four hold it.
-WAMB_DEV void split_e4m3x4(const float (&x)[4], uint32_t& h, uint32_t& l) {
+// Four values into their E4M3 code word `h` and the E5M2 word of what it leaves.
+WAMB_DEV void split_8bit_x4(const float (&x)[4], uint32_t& h, uint32_t& l) {
   const uint32_t h0 = __nv_cvt_float2_to_fp8x2(make_float2(x[0], x[1]), __NV_SATFINITE, __NV_E4M3);
   const uint32_t h1 = __nv_cvt_float2_to_fp8x2(make_float2(x[2], x[3]), __NV_SATFINITE, __NV_E4M3);
   const float2 f0 = e4m3x2_to_float2(h0), f1 = e4m3x2_to_float2(h1);
-  const uint32_t l0 = __nv_cvt_float2_to_fp8x2(make_float2(x[0] - f0.x, x[1] - f0.y), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t l1 = __nv_cvt_float2_to_fp8x2(make_float2(x[2] - f1.x, x[3] - f1.y), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t l0 = __nv_cvt_float2_to_fp8x2(make_float2(x[0] - f0.x, x[1] - f0.y), __NV_SATFINITE, __NV_E5M2);
+  const uint32_t l1 = __nv_cvt_float2_to_fp8x2(make_float2(x[2] - f1.x, x[3] - f1.y), __NV_SATFINITE, __NV_E5M2);
   h = h0 | (h1 << 16);
   l = l0 | (l1 << 16);
 }
@@ -182,7 +186,7 @@ WAMB_DEV float query_scale(float amax, int& n) {
   return amax <= 3.402823466e38f ? pow2f_exact(-n) : __int_as_float(0x7fffffff);
 }
 
-// The queries in two E4M3 pieces, for the tensor-core kernels: row
+// The queries in two 8-bit pieces, for the tensor-core kernels: row
 // (b * heads + h) * rows_pad + r of q8 [., 256] holds hi (128 codes) and lo of
 // row r of (sequence b, cached head h), rf its factor 2^n * scale * log2(e);
 // rows past the sequence's are zeros. With neg_lse2 (weights): -lse * log2(e),
@@ -235,7 +239,7 @@ __global__ void __launch_bounds__(256) kv8_split_q_kernel(const Kv8AttnParams p,
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const float x[4] = {v[2 * k].x * up, v[2 * k].y * up, v[2 * k + 1].x * up, v[2 * k + 1].y * up};
-      split_e4m3x4(x, hi[k], lo[k]);
+      split_8bit_x4(x, hi[k], lo[k]);
     }
     if (row >= total) continue;
     uint4* dst = reinterpret_cast<uint4*>(q8 + static_cast<long long>(row) * 256) + c;
