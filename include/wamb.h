@@ -532,7 +532,7 @@ WAMB_API int wamb_kv8_write(const wamb_kv8_write_args* args, void* stream);
  * left as they were. What lies past lens[b] in a page counts for nothing,
  * but a NaN that was written as V reaches every row of the call that is
  * computed beside its key. Scores are summed in fp32. With more than 16 rows
- * a sequence and cached head, an element of q below 2^-14 of its row's largest
+ * a sequence and cached head, an element of q below 2^-13 of its row's largest
  * magnitude is taken to within 2^-21 of that magnitude; all others, and with
  * up to 16 rows all down to 2^-28, count with their full eight bits. workspace:
  * wamb_kv8_attention_workspace_bytes() bytes of scratch (256-byte aligned, any

@@ -5,7 +5,7 @@ are the small ones.
 Up to 16 query rows the kernels hold a query in f16 scaled by its row (exact
 over 28 binades), above in an E4M3 and an E5M2 value: an element is off by at
 most 2^-14 when its row's largest is scaled into (224, 448], and by nothing
-when it is at least 2^-14 of that largest. fp32 sums of 128 products are off
+when it is then at least 2^-6. fp32 sums of 128 products are off
 by at most 130 roundings of their sum of magnitudes (a tensor core may
 truncate: 2^-23 each), and a score takes a few more roundings of its own size.
 """

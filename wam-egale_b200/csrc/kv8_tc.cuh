@@ -7,7 +7,7 @@
 // conversion): q 2^-n = hi + lo, hi the nearest E4M3 value and lo the nearest
 // E5M2 value of what it leaves, so S = (hi K^T + lo K^T) 2^n costs what one
 // bf16 product does. n puts the row's largest magnitude in (224, 448]. From
-// 2^-6 on (2^-14 of the largest) hi + lo has all eight bits of a bf16 query:
+// 2^-6 on (2^-13.8 of the largest, or less) hi + lo has all eight bits of a bf16 query:
 // hi has four, and what it leaves is at most 8 units in the last of the eight,
 // which E5M2's three bits hold. Below, hi leaves at most 2^-10 and lo is off by
 // half its step, 2^-14 (2^-21 of the row's largest). With E4M3 for lo, whose
