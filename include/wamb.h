@@ -489,7 +489,11 @@ WAMB_API int wamb_cfg_combine(const void* cond, const void* uncond, int32_t io_i
  * captured in a graph and replayed with other lengths. A page id outside
  * [0, pages), a length outside [0, table_width * page] or a count outside
  * [0, tokens] is recorded as WAMB_DEV_KV8; the call then touches nothing
- * outside the cache, but its result is not to be used.
+ * outside the cache, but its result is not to be used. A sequence whose length
+ * or count is out of range is taken as empty: write leaves its pages as they
+ * were (also where its rows do not fit its table), weights carries its base
+ * over, attention answers its rows with 0 and -inf (a bad count: leaves them),
+ * evict keeps nothing. The other sequences are served.
  * ------------------------------------------------------------------------ */
 typedef struct wamb_kv8_cache {
   void* k8; void* v8;               /* [pages, heads, page, 128] E4M3, 16-byte aligned */

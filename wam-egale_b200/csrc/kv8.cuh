@@ -37,22 +37,24 @@ struct Kv8Seqs {
   int batch, width, tokens;
 };
 
-// Cached tokens of sequence b; out-of-range lengths are clamped and reported.
-WAMB_DEV int kv8_len(const Kv8Seqs& s, const Kv8Cache& c, int b) {
+// Cached tokens of sequence b. A length out of range is reported and counts as
+// `bad`: none, so that nothing is read, added up or kept by a wrong length.
+WAMB_DEV int kv8_len(const Kv8Seqs& s, const Kv8Cache& c, int b, int bad = 0) {
   const int n = __ldg(s.lens + b);
   const long long cap = static_cast<long long>(s.width) << c.page_log2;
   if (n < 0 || n > cap) {
     record_error(KV8_DEV_ERROR);
-    return n < 0 ? 0 : static_cast<int>(cap);
+    return bad;
   }
   return n;
 }
+// Valid rows of sequence b in this call; none (reported) for a count out of range.
 WAMB_DEV int kv8_count(const Kv8Seqs& s, int b) {
   if (s.counts == nullptr) return s.tokens;
   const int n = __ldg(s.counts + b);
   if (n < 0 || n > s.tokens) {
     record_error(KV8_DEV_ERROR);
-    return n < 0 ? 0 : s.tokens;
+    return 0;
   }
   return n;
 }
@@ -139,12 +141,15 @@ __global__ void __launch_bounds__(kv8_page_threads(PAGE)) kv8_write_kernel(const
   constexpr int WORDS = F32 ? 4 : 2;      // 16-byte pieces of 16 values
   __shared__ float red[THREADS / 32];
   const int h = blockIdx.y, b = blockIdx.z >> 1, which = blockIdx.z & 1;
-  const int start = kv8_len(p.s, p.c, b);
-  int cnt = kv8_count(p.s, b);
-  const long long cap = static_cast<long long>(p.s.width) * PAGE;
-  if (start + static_cast<long long>(cnt) > cap) {   // the table has no room for the last tokens
+  // A sequence with a length or count out of range, or without room in its table
+  // for all of its rows, is left as it was: its history must not be written over,
+  // nor rounded again to a scale that rows at wrong places would set.
+  const int start = kv8_len(p.s, p.c, b, -1);
+  if (start < 0) return;
+  const int cnt = kv8_count(p.s, b);
+  if (start + static_cast<long long>(cnt) > static_cast<long long>(p.s.width) * PAGE) {
     if (threadIdx.x == 0) record_error(KV8_DEV_ERROR);
-    cnt = static_cast<int>(cap - start);
+    return;
   }
   const int pi = start / PAGE + blockIdx.x;
   const int lo = max(start, pi * PAGE);
