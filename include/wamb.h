@@ -583,7 +583,9 @@ WAMB_API int wamb_kv8_weights(const wamb_kv8_attention_args* args, void* stream)
  * one, or with one new page twice, is refused (WAMB_DEV_KV8: it keeps nothing),
  * and no new page may be in use by another sequence of the call or elsewhere.
  * max_len: an upper bound of lens that the caller knows (at most
- * table_width * page); min(heavy + recent, max_len) must fit new_width pages. */
+ * table_width * page); min(heavy + recent, max_len) must fit new_width pages. A
+ * sequence that is longer and would keep more than they hold is refused in the
+ * same way. */
 typedef struct wamb_kv8_evict_args {
   wamb_kv8_cache cache;
   wamb_kv8_seqs seqs;               /* counts and tokens are not read */

@@ -268,11 +268,16 @@ struct Kv8Kept {
 WAMB_DEV Kv8Kept kv8_kept(const Kv8EvictParams& p, int b) {
   Kv8Kept k;
   k.len = kv8_len(p.s, p.c, b);
-  const int cap = static_cast<int>(min(2147483647ll, static_cast<long long>(p.new_width) << p.c.page_log2));
-  const int recent = min(min(p.recent, k.len), cap);
+  const int recent = min(p.recent, k.len);
   k.old = k.len - recent;
-  k.heavy = min(min(p.heavy, k.old), cap - recent);
+  k.heavy = min(p.heavy, k.old);
   k.total = k.heavy + recent;
+  // More than the new pages hold (the length is above the caller's max_len):
+  // cut, the sequence would lose its latest positions. It keeps nothing.
+  if (k.total > static_cast<long long>(p.new_width) << p.c.page_log2) {
+    record_error(KV8_DEV_ERROR);
+    k.heavy = k.total = 0;
+  }
   return k;
 }
 

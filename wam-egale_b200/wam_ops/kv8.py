@@ -201,7 +201,8 @@ class Kv8Cache:
         (kept [batch, heads, new_width * page] int32 old positions, -1 behind
         the last; their weights, 0 behind the last; new lengths int32 [batch]).
         max_len: an upper bound of lens (default: the table's capacity);
-        min(heavy + recent, max_len) tokens must fit the new pages."""
+        min(heavy + recent, max_len) tokens must fit the new pages. A sequence
+        that would keep more than they hold keeps nothing and is reported."""
         batch = lens.shape[0] if lens.dim() == 1 else -1
         a = _lib.Kv8EvictArgs()
         a.cache = self._c
