@@ -18,11 +18,19 @@ and lengths are reported by _lib.device_status() (code 5).
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
 HEAD_DIM = 128
 PAGES = (16, 32, 64, 128)
+
+
+def _inference_only(t):
+    """Refuses a tensor whose derivatives, backward or forward, a call would drop (or a leaf that it would write)."""
+    if (t.requires_grad and torch.is_grad_enabled()) or \
+            (forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None):
+        raise RuntimeError("Kv8Cache is inference-only; use no_grad/inference_mode")
 
 
 class Kv8Cache:
@@ -80,8 +88,7 @@ class Kv8Cache:
             raise ValueError(f"{name} must be [batch, tokens, heads, 128] {' or '.join(map(str, dtypes))} on {self.device}")
         if heads is not None and b[2] != heads:
             raise ValueError(f"{name} has {b[2]} heads, the cache {heads}")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise RuntimeError("Kv8Cache is inference-only; use no_grad/inference_mode")
+        _inference_only(t)
         if s[3] != 1:
             raise ValueError(f"{name} must have unit stride along the head dim")
         # The stride of a single entry may be anything; the C ABI is told 0.
@@ -92,6 +99,7 @@ class Kv8Cache:
                 or t.device != self.device or t.shape[2] < width * self.page:
             raise ValueError(f"{name} must be contiguous fp32 [batch {batch}, heads {self.heads}, >= {width * self.page}]"
                              f" on {self.device}")
+        _inference_only(t)
         return t.data_ptr()
 
     def _call(self, fn, args, workspace_bytes=None, shape=None):
@@ -170,6 +178,7 @@ class Kv8Cache:
     def _lse(self, lse, q):
         if lse.dtype != torch.float32 or lse.shape != q.shape[:3] or not lse.is_contiguous() or lse.device != self.device:
             raise ValueError("lse must be contiguous fp32 [batch, tokens, q_heads]")
+        _inference_only(lse)
         return lse.data_ptr()
 
     def weights(self, q, table, lens, lse, base=None, out=None, counts=None, causal=False, scale=None):
