@@ -101,3 +101,33 @@ def test_in_place_sum_of_a_leaf_is_refused(cache):
     with pytest.raises(RuntimeError, match="inference-only"):
         c.weights(q, TABLE, LENS, lse, base=w, out=w)
     assert not calls
+
+
+@pytest.mark.parametrize("heavy,recent,max_len", [(2 ** 32 + 5, 10, None), (20, 2 ** 32, None), (2 ** 31, 0, None),
+                                                  (20, -2 ** 32, None), (20, 10, 2 ** 64 + 30)])
+def test_evict_refuses_numbers_that_would_wrap(cache, heavy, recent, max_len):
+    """2^32 'keep all' would be taken as 0, and the latest tokens dropped."""
+    c, calls = cache
+    w = _inputs()[2]
+    with pytest.raises(ValueError, match="heavy, recent"):
+        c.evict(TABLE, LENS, w, NEW, heavy=heavy, recent=recent, max_len=max_len)
+    assert not calls
+
+
+def test_evict_takes_the_largest_numbers(cache):
+    c, calls = cache
+    w = _inputs()[2]
+    c.evict(TABLE, LENS, w, NEW, heavy=2 ** 31 - 1, recent=2 ** 31 - 1, max_len=30)
+    assert (calls[0].heavy, calls[0].recent, calls[0].max_len) == (2 ** 31 - 1, 2 ** 31 - 1, 30)
+
+
+def test_sizes_that_would_wrap_are_refused(cache):
+    """Expanded inputs can have more rows than 32 bits count."""
+    c, calls = cache
+    k = torch.zeros(1, 1, HEADS, 128).bfloat16().expand(1, 2 ** 32 + 1, HEADS, 128)
+    with pytest.raises(ValueError, match="2\\^31"):
+        c.write(k, k, TABLE[:1], LENS[:1])
+    q = torch.zeros(1, 1, 1, 128).bfloat16().expand(1, 1, 2 ** 32 + HEADS, 128)
+    with pytest.raises(ValueError, match="2\\^31"):
+        c.weights(q, TABLE[:1], LENS[:1], torch.zeros(1, 1, HEADS))
+    assert not calls

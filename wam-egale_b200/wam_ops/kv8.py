@@ -24,6 +24,7 @@ from . import _lib
 
 HEAD_DIM = 128
 PAGES = (16, 32, 64, 128)
+INT32_MAX = 2 ** 31 - 1      # the C ABI's sizes; a larger number would wrap without a word
 
 
 def _inference_only(t):
@@ -75,6 +76,8 @@ class Kv8Cache:
         shape = table.shape
         if len(shape) != 2 or shape[0] != batch:
             raise ValueError(f"table must be [batch {batch}, width]")
+        if tokens > INT32_MAX:
+            raise ValueError(f"{tokens} tokens: sizes are below 2^31")
         seqs.batch, seqs.tokens, seqs.table_width = batch, tokens, shape[1]
         seqs.table = self._ints("table", table, shape)
         seqs.lens = self._ints("lens", lens, (batch,))
@@ -145,6 +148,8 @@ class Kv8Cache:
         batch, tokens, heads, _ = q.shape
         if heads == 0 or heads % self.heads:
             raise ValueError(f"q has {heads} heads, no multiple of the cache's {self.heads}")
+        if heads > INT32_MAX:
+            raise ValueError(f"{heads} query heads: sizes are below 2^31")
         scale = HEAD_DIM ** -0.5 if scale is None else float(scale)
         if not (scale > 0 and math.isfinite(scale)):
             raise ValueError("scale must be positive and finite")
@@ -222,8 +227,11 @@ class Kv8Cache:
         a.new_width = new_table.shape[1]
         a.weights = self._weight("weights", weights, batch, table.shape[1])
         a.weights_cap = weights.shape[2]
-        a.heavy, a.recent = int(heavy), int(recent)
-        a.max_len = table.shape[1] * self.page if max_len is None else int(max_len)
+        heavy, recent = int(heavy), int(recent)
+        max_len = table.shape[1] * self.page if max_len is None else int(max_len)
+        if max(abs(heavy), abs(recent)) > INT32_MAX or abs(max_len) > 2 ** 62:
+            raise ValueError(f"heavy, recent and max_len ({heavy}, {recent}, {max_len}) must be below 2^31, 2^31 and 2^62")
+        a.heavy, a.recent, a.max_len = heavy, recent, max_len
         shape = (batch, self.heads, a.new_width * self.page)
         kept, new_lens = table.new_empty(shape), table.new_empty(batch)
         new_weights = weights.new_empty(shape)
