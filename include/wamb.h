@@ -580,7 +580,8 @@ WAMB_API int wamb_kv8_weights(const wamb_kv8_attention_args* args, void* stream)
  * the last), new_weights their weights (0 behind the last), new_lens their
  * number min(lens[b], heavy + recent). The old pages are not changed and may
  * be freed afterwards; a sequence with a page of its old table in its new
- * one, or with one new page twice, is refused (WAMB_DEV_KV8: it keeps nothing),
+ * one, with one new page twice, or with a new page outside [0, pages) is refused
+ * (WAMB_DEV_KV8: it keeps nothing),
  * and no new page may be in use by another sequence of the call or elsewhere.
  * max_len: an upper bound of lens that the caller knows (at most
  * table_width * page); min(heavy + recent, max_len) must fit new_width pages. A

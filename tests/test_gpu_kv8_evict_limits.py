@@ -97,3 +97,23 @@ def test_evict_time_does_not_depend_on_where_the_pages_lie(cuda_device):
     print(f"evict with distinct ids {distinct:.3f} ms, colliding {collide:.3f} ms")
     assert _lib.device_status() == 0
     assert collide <= 2 * distinct
+
+
+def test_evict_onto_a_page_that_is_none_keeps_nothing(cuda_device):
+    """Rows for it would be lost although `kept` lists them."""
+    c, table, free, g = _setup(2, 2, 16, 6, 58, spare=4)
+    w = torch.rand(2, 2, 96, generator=g).to(DEV)
+    for value in (c.pages, -1, 2 ** 31 - 1, -2 ** 31):
+        for at in (0, 1):
+            new = free.view(2, 2).clone()
+            new[0, at] = value
+            before = c.k8.view(torch.uint8)[free.long()].clone()
+            kept, nw, lens = c.evict(table, _i32([90, 50]), w, new, heavy=20, recent=10)
+            assert _reported()
+            assert lens.tolist() == [0, 30] and (kept[0] == -1).all() and (nw[0] == 0).all()
+            assert torch.equal(c.k8.view(torch.uint8)[free[:2].long()], before[:2])
+            new[1, 1] = value
+            new[0] = free[:2]
+            kept, nw, lens = c.evict(table, _i32([90, 50]), w, new, heavy=10, recent=5)
+            torch.cuda.synchronize()
+            assert _lib.device_status() == 0 and lens.tolist() == [15, 15]      # a page that receives nothing may be any

@@ -503,7 +503,7 @@ WAMB_DEV void kv8_select_heavy(const Kv8Kept& k, const float* w, Kv8SelSmem& sm,
 // SM's instructions (an instruction a key is 240 cycles at 31k keys): 64 heads
 // of 31k weights take 22 us of the 72 that an eviction of 8 x 32k tokens takes,
 // 24 heads of 3520 take 10 of 17. A sequence whose new pages overlap its old
-// ones, or one another, is refused: it keeps nothing.
+// ones, or one another, or do not exist is refused: it keeps nothing.
 __global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8EvictParams p, const int list_at) {
   pdl_wait();
   extern __shared__ uint32_t keys[];
@@ -525,9 +525,10 @@ __global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8Ev
   constexpr uint32_t WORDS = KV8_SEL_COPIES * KV8_SEL_BINS;
   const int* used = p.s.table + static_cast<long long>(b) * p.s.width;
   kv8_clear_hist(sm);
-  bool overlap = false;
+  bool overlap = false, none = false;      // none: a new page that does not exist (its rows would be lost)
   for (int n = tid; n < new_pages; n += KV8_SEL_THREADS) {
     const uint32_t page = static_cast<uint32_t>(__ldg(fresh + n));
+    none |= page >= static_cast<uint32_t>(p.c.pages);
     overlap |= atomicOr(bits + (page >> 5) % WORDS, 1u << (page & 31)) >> (page & 31) & 1;
   }
   __syncthreads();
@@ -555,7 +556,7 @@ __global__ void __launch_bounds__(KV8_SEL_THREADS) kv8_select_kernel(const Kv8Ev
       __syncthreads();       // the bits are cleared
     }
   }
-  if (__syncthreads_or(overlap)) {
+  if (__syncthreads_or(overlap || none)) {
     if (tid == 0) record_error(KV8_DEV_ERROR);
     k.heavy = k.total = 0;
   }
