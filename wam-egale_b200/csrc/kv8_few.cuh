@@ -825,6 +825,12 @@ __global__ void __launch_bounds__(FEW_THREADS, WEIGHTS ? 4 : 3)
       began = true;
     }
   }
+  // Every load has been waited for, unless a wait ran out or ended early because
+  // another warp's did: a CTA must not exit with loads on their way, so it stays
+  // for a thousand times the latency of memory. (Counting what is on its way
+  // into the loop's end cost 8% of the one-token attention.)
+  if (*abort_flag)
+    for (const uint64_t t0 = globaltimer(); globaltimer() - t0 < 1000000;) {}
 }
 
 }  // namespace wamb

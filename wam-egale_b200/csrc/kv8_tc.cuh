@@ -351,6 +351,7 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
     const int to = lane >> 3, gi = lane & 7;
     const int box_groups = p.c.page >> 4;   // 16-key groups of one page
     int tiles = 0, queries = 0;             // key tiles and query tiles so far
+    int k_loads = 0, v_loads = 0;           // loads issued: tiles, but for the last where a wait ran out
     bool go = true;
     for (int seg = 0; go && !walk.done(sh); walk.next(p, sh), ++seg) {
       const KtcSeg sg(p, sh, walk);
@@ -412,22 +413,22 @@ __global__ void __launch_bounds__(KTC_THREADS, 1)
           if (lane == 0) mbar_arrive_expect_tx(k_full + 8 * slot, bytes);
           __syncwarp();
           if (lead) tma_load_2d(sK + slot * KTC_TILE8 + gi * 2048, &tmK, k_full + 8 * slot, 0, now.row);
+          ++k_loads;
           go = __all_sync(0xffffffffu, mbar_wait(v8_empty + 8 * slot, phase ^ 1, abort_flag));
           if (!go) break;
           if (lane == 0) mbar_arrive_expect_tx(v8_full + 8 * slot, bytes);
           __syncwarp();
           if (lead) tma_load_2d(sV8 + slot * KTC_TILE8 + gi * 2048, &tmV, v8_full + 8 * slot, 0, now.row);
+          ++v_loads;
         }
         now = next;
       }
     }
-    // Loads still in flight must land before the CTA exits.
-    if (lane == 0 && go) {
+    // Loads still in flight must land before the CTA exits, after a wait that ran out too.
+    if (lane == 0) {
       if (queries > 0) mbar_wait_teardown(q_full, (queries - 1) & 1);
-      for (int t = max(0, tiles - 2); t < tiles; ++t) {
-        mbar_wait_teardown(k_full + 8 * (t & 1), (t >> 1) & 1);
-        mbar_wait_teardown(v8_full + 8 * (t & 1), (t >> 1) & 1);
-      }
+      for (int t = max(0, k_loads - 2); t < k_loads; ++t) mbar_wait_teardown(k_full + 8 * (t & 1), (t >> 1) & 1);
+      for (int t = max(0, v_loads - 2); t < v_loads; ++t) mbar_wait_teardown(v8_full + 8 * (t & 1), (t >> 1) & 1);
     }
     __syncwarp();
   } else if (warp == 9) {
@@ -920,8 +921,8 @@ __global__ void __launch_bounds__(KWT_THREADS, 1)
       }
       now = next;
     }
-    // Loads still in flight must land before the CTA exits.
-    if (lane == 0 && go) {
+    // Loads still in flight must land before the CTA exits, after a wait that ran out too.
+    if (lane == 0) {
       for (int t = max(0, pairs - 2); t < pairs; ++t) mbar_wait_teardown(k_full + 8 * (t & 1), (t >> 1) & 1);
       for (int t = max(0, tiles - KWT_QS); t < tiles; ++t) {
         mbar_wait_teardown(q_full + 8 * (t % KWT_QS), (t / KWT_QS) & 1);
