@@ -49,8 +49,8 @@ struct Kv8AttnParams {
   const float* base;               // [batch, heads, w_cap] or null (zeros)
   float* weights;                  // like base; may be base
   long long w_cap;
-  // stream-K: query tiles per sequence, CTAs, smallest share, partials
-  int qts, ctas, min_units;
+  // stream-K: query tiles per sequence, CTAs, partials
+  int qts, ctas;
   float* part;
 };
 
@@ -130,7 +130,7 @@ WAMB_DEV bool kv8_share(const Kv8AttnParams& p, int cta, Kv8SchedSmem& sm, Kv8Sh
 #pragma unroll
   for (int i = 0; i < THREADS / 32; ++i) total += sm.warp[i];
   sh.units = total * p.c.heads;
-  sh.ctas = static_cast<int>(min(static_cast<long long>(p.ctas), max(1ll, sh.units / p.min_units)));
+  sh.ctas = static_cast<int>(min(static_cast<long long>(p.ctas), max(1ll, sh.units)));   // a unit each at least
   if (sh.units == 0 || cta >= sh.ctas) return false;
   sh.u0 = sh.first(cta);
   sh.u1 = sh.first(cta + 1);

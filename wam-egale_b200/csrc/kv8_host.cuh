@@ -266,7 +266,6 @@ inline int kv8_attention_impl(const wamb_kv8_attention_args* a, bool weights, cu
   rc = make_tmap_2d(&tmV, p.c.v8, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, code_rows, 128, 128, box, 128);
   if (rc) return rc;
   p.ctas = kv8_few_ctas(di, weights);
-  p.min_units = 1;
   if (weights && few) {
     static bool done[64] = {};
     rc = kv8_smem_once(kv8_few_kernel<true>, FewSmem<true>::TOTAL, done);
