@@ -483,10 +483,12 @@ WAMB_API int wamb_cfg_combine(const void* cond, const void* uncond, int32_t io_i
  * is 2^n, n the smallest whole number in [-40, 119] with the block's largest
  * magnitude <= 448 * 2^n; a value is e4m3(x / scale), rounded to nearest
  * even, saturating; NaN stays NaN. (Scales written by others may be any
- * positive finite number.) At most 2^30 positions a sequence.
+ * positive finite number; x / scale is then x times its rounded reciprocal.)
+ * At most 2^30 positions a sequence.
  *
  * lens, counts, tables live on the device and are read there: a call can be
- * captured in a graph and replayed with other lengths. A page id outside
+ * captured in a graph and replayed with other lengths (they must not change
+ * while it runs). A page id outside
  * [0, pages), a length outside [0, table_width * page] or a count outside
  * [0, tokens] is recorded as WAMB_DEV_KV8; the call then touches nothing
  * outside the cache, but its result is not to be used. A sequence whose length
@@ -565,8 +567,8 @@ WAMB_API int wamb_kv8_attention(const wamb_kv8_attention_args* args, void* strea
  * weights[b, h, j] = base[b, h, j] + sum over the valid query rows of cached
  * head h that see j of exp(scale q k_j - lse), lse as wamb_kv8_attention gave
  * it for the same q, lens, counts, causal and scale (rows with lse -inf add
- * nothing). Columns that no row sees carry the base over. out, out_stride and
- * v8 are not read. workspace: wamb_kv8_weights_workspace_bytes() bytes (0
+ * nothing). Columns that no row sees carry the base over; with more than 16
+ * rows a sum below 2^-100 counts as 0. out, out_stride and v8 are not read. workspace: wamb_kv8_weights_workspace_bytes() bytes (0
  * for few rows), as for wamb_kv8_attention. */
 WAMB_API size_t wamb_kv8_weights_workspace_bytes(const wamb_kv8_attention_args* args);
 WAMB_API int wamb_kv8_weights(const wamb_kv8_attention_args* args, void* stream);

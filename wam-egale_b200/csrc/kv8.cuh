@@ -6,10 +6,12 @@
 // position p of sequence b is row p % page of page table[b, p / page].
 // A scale is a power of two, 2^n with n the smallest whole number in
 // [-40, 119] such that the block's largest magnitude is at most 448 * 2^n.
-// A power of two makes x / s exact, so that a value is rounded once (by at
-// most 2^-4 of itself), and moving a block's codes to a larger scale (a later
-// token of the block is larger) rounds again only what falls below E4M3's
-// normal range: a general scale would add a rounding at every growth.
+// A power of two makes x / s exact, so that a value is rounded once: by at most
+// 2^-4 of itself from 2^-6 s on, by at most 2^-10 s below, where E4M3's steps
+// no longer shrink (what is below 2^-10 s becomes 0). Moving a block's codes to a
+// larger scale (a later token of the block is larger) rounds again only what
+// falls below that normal range: a general scale would add a rounding at every
+// growth.
 #pragma once
 #include <cuda_fp16.h>
 

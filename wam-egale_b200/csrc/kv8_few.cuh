@@ -22,10 +22,12 @@
 // l_i = sum_j P_ij / vs_j. P goes to the product as f16 with an offset of 2^6:
 // 11 bits down to 2^-20 of the row's maximum and whole steps of 2^-30 below.
 //
-// Bound by instruction issue: one token of 8 sequences of 18 to 32 thousand
-// keys (8 heads, 4 query heads each, 420 MB) takes 82 us, 5.1 TB/s, with 35 M
-// warp instructions, half of them the conversions of codes and the products;
-// its attention weights (K alone, 227 MB) take 49 us, 4.7 TB/s. The smallest calls
+// Bound by the latency of a warp's step (load -> convert -> product -> exponential ->
+// product, one unit at a time) with twelve to sixteen warps an SM: one token of 8
+// sequences of 18 to 32 thousand keys (8 heads, 4 query heads each, 420 MB)
+// takes 82 us, 5.1 TB/s, with 35 M warp instructions, half of them the
+// conversions of codes and the products, and issue active 44% of the cycles;
+// its attention weights (K alone, 227 MB) take 49 us, 4.7 TB/s, at 53%. The smallest calls
 // (2 sequences of 500 keys, 12 heads) take 11 us, nearly all of it the latency of two
 // launches and of table -> scale -> codes.
 #pragma once

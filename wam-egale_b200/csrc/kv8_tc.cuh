@@ -33,9 +33,9 @@
 // s on slot s & 1: S(s + 2) is issued behind PV(s).
 // TMEM columns: S/P of A [0,128), of B [128,256), O_A [256,384), O_B [384,512).
 //
-// Bound by the softmax's issue slots and the chain S -> softmax -> P -> PV of a
-// slot: a key tile of 256 rows takes about 5000 cycles where its MMAs take
-// 2048. 8 x 880 rows over up to 4400 keys of 24 heads (297 GFLOP): 434 us, 0.68
+// Bound by the latency of the chain S -> softmax -> P -> PV of a slot (two softmax
+// warps a scheduler; issue active 36%, tensor pipe 41%): a key tile of 256 rows
+// takes about 5000 cycles where its MMAs take 2048. 8 x 880 rows over up to 4400 keys of 24 heads (297 GFLOP): 434 us, 0.68
 // PFLOP/s, 19 of them the split of the queries; 32 rows of 4 sequences (75 MB
 // of cache) 44 us. Slower forms of the same chain, at that size and before the
 // last 30 us were taken elsewhere (this one: 468): P through shared memory 549
